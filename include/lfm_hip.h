@@ -267,6 +267,101 @@ int lfm_argmax(const float *v_dev, uint32_t n, uint32_t *index, float *value);
  * that device's array: calls that overlap on one device race. */
 int lfm_argmax_noalloc(const float *v_dev, uint32_t n, uint32_t *index, float *value);
 
+/* ---- attention over key/value caches --------------------------------------
+ * Grouped-query attention of new rows over the caches of a batch of sequences, and the
+ * eviction of cache slots (no counterpart in the reference, whose one session attends
+ * every position, engine/src/lfm.rs:395-437).  Every call enqueues kernels on `stream`
+ * (a hipStream_t of the current device, NULL the default stream) and returns: it
+ * allocates nothing, copies nothing and does not wait, so it can be captured into a
+ * graph; the device's first call of these loads the code object and has to come before
+ * a capture.  Pointers are device memory of the current device.  `workspace` holds at
+ * least the bytes that the operator's _workspace call returns for the same arguments
+ * (16-byte aligned; it depends on sizes and types, never on the contents of device
+ * arrays) and belongs to the call until its kernels are done: calls that may overlap,
+ * captured graphs among them, each have their own.  Arguments are checked before
+ * anything is enqueued (LFM_EINVAL). */
+#define LFM_TYPE_F32 0u
+#define LFM_TYPE_F16 1u
+#define LFM_TYPE_BF16 2u
+
+/* K and V of n_seq sequences.  Element (b, h, slot, d) lies at b * seq_stride + h *
+ * head_stride + slot * slot_stride + d of k and of v (strides in elements, multiples of
+ * 8 and not negative; a sequence stride of 0 shares one cache; k and v 16-byte aligned).
+ * len[b] is the number of slots in use, read on the device when the kernels run: below 0
+ * counts as 0, above `slots` as `slots`.  Slots past it are never used, whatever they
+ * hold. */
+typedef struct lfm_kv {
+    void *k, *v;
+    int32_t *len;
+    int64_t seq_stride, head_stride, slot_stride;
+    uint32_t type;     /* LFM_TYPE_F16 or LFM_TYPE_BF16 */
+    uint32_t n_seq, kv_heads, slots;
+    uint32_t head_dim; /* 64 or 128 */
+} lfm_kv;
+
+/* Query rows and their outputs, q[row][head][d]: row and head strides in elements, in
+ * multiples of 16 bytes, not negative; q and out 16-byte aligned and apart.  Types: F16
+ * or BF16 as the cache's, or F32 with an F16 cache.  heads is a multiple of the cache's
+ * kv_heads; head h reads kv head h * kv_heads / heads.
+ * start (device, n_seq + 1 ascending entries) gives sequence b the rows start[b] ..
+ * start[b + 1] - 1; NULL: one row per sequence (n_rows = n_seq).  Rows of no sequence
+ * are left as they are.  A sequence's rows are its newest tokens, whose K and V are in
+ * the cache: row i of n is at position len - n + i and sees the slots up to it.
+ * lse (nullable) receives log(sum of exp(score)) per row and head. */
+typedef struct lfm_rows {
+    const void *q;
+    void *out;
+    float *lse; /* [n_rows][heads] */
+    const int32_t *start;
+    int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride;
+    uint32_t type;
+    uint32_t heads, n_rows;
+    float scale; /* scores are scale * q . k; positive */
+} lfm_rows;
+
+/* out = softmax(scale * q K^T) V over the slots a row sees: of the positions up to its
+ * own, the newest `window` (0: all) and the first `sinks`.  A row that sees nothing gets
+ * zeros and an lse of -infinity.  Scores, weights' sums and outputs are held in 32 bits;
+ * weights meet V as 16-bit numbers, as two of them (22 bits) for F32 rows. */
+int lfm_attn_window(const lfm_kv *kv, const lfm_rows *rows, uint32_t window, uint32_t sinks,
+                    void *workspace, size_t workspace_bytes, void *stream);
+int lfm_attn_window_workspace(const lfm_kv *kv, const lfm_rows *rows, uint32_t window,
+                              uint32_t sinks, size_t *bytes);
+
+/* The same over all positions, and the weights each slot receives: for every sequence, kv
+ * head and slot in use, acc_out = acc_in + the weights summed over the sequence's rows and
+ * the kv head's query heads (acc [n_seq][kv_heads][slots] f32; acc_in NULL counts as
+ * zeros and may be acc_out; slots not in use are left as they are).  Sums are in a fixed
+ * order: equal calls give equal bits. */
+int lfm_attn_scored(const lfm_kv *kv, const lfm_rows *rows, const float *acc_in, float *acc_out,
+                    void *workspace, size_t workspace_bytes, void *stream);
+int lfm_attn_scored_workspace(const lfm_kv *kv, const lfm_rows *rows, size_t *bytes);
+
+/* Attention of a batch whose sequences share a prefix: every row sees all slots in use of
+ * `prefix` (n_seq 1; heads, head_dim and type as kv's), then its own sequence's up to its
+ * position.  The prefix is read once for all rows of the batch. */
+int lfm_attn_prefix(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *rows,
+                    void *workspace, size_t workspace_bytes, void *stream);
+int lfm_attn_prefix_workspace(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *rows,
+                              size_t *bytes);
+
+/* Eviction by accumulated weight.  Where a sequence has more than `keep` slots in use,
+ * each kv head keeps `keep` of them: the protected ones (pos < sinks, or among the newest
+ * `recent` positions: pos > newest pos - recent), then those of highest acc, ties to the
+ * lowest slot, NaN below every number.  sinks + recent is at most keep.  Kept slots below
+ * `keep` stay where they are; the i-th slot that leaves from below `keep` is replaced by
+ * the i-th kept slot from `keep` on.  K, V, acc and pos ([n_seq][kv_heads][slots], the
+ * position of each slot's token) move alike, and out->len receives min(len, keep).
+ * `out` holds at least `keep` slots per sequence; with out->k == kv->k and out->v ==
+ * kv->v (and equal strides) the eviction is in place and moves only what changes place;
+ * acc_out == acc and pos_out == pos likewise (with equal slots), len_out may be kv->len.
+ * Apart from that outputs and inputs are apart.  Output slots past the new length are
+ * left as they are. */
+int lfm_kv_evict(const lfm_kv *kv, const float *acc, const int32_t *pos, uint32_t keep,
+                 uint32_t sinks, uint32_t recent, const lfm_kv *out, float *acc_out,
+                 int32_t *pos_out, void *workspace, size_t workspace_bytes, void *stream);
+int lfm_kv_evict_workspace(const lfm_kv *kv, uint32_t keep, size_t *bytes);
+
 /* ---- synthetic model (seeded; identical bytes on every host) -------------- */
 typedef struct lfm_tensor_desc {
     char name[96];

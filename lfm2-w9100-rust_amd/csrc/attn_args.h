@@ -1,0 +1,56 @@
+// attn_args.h -- kernel arguments of the cache-attention operators, shared by the host
+// launcher (attn_ops.cpp) and the gfx950 kernels (lfm_attn.hip).  Every kernel takes one
+// of these structs by value.
+#pragma once
+#include <stdint.h>
+
+// K and V of n_seq sequences: element (b, h, slot, d) at b * ss + h * hs + slot * ts + d.
+struct KvView {
+    const uint16_t *k, *v;
+    const int32_t *len; // slots in use per sequence, clamped to [0, slots] by the kernels
+    int64_t ss, hs, ts;
+    uint32_t n_seq, kv_heads, slots;
+};
+
+// The rows of a call: q[row][head][d] and out alike.  start (n_seq + 1 entries) gives each
+// sequence's rows; null: row b is sequence b's.
+struct RowsView {
+    const void *q;
+    void *out;
+    float *lse; // nullable: [row][head], natural logarithm
+    const int32_t *start;
+    int64_t q_rs, q_hs, o_rs, o_hs;
+    uint32_t heads, n_rows;
+    float scale, cexp; // cexp = scale * log2(e)
+};
+
+struct AttnOpArgs {
+    KvView own;    // slots of the row's own sequence, causal
+    KvView prefix; // k null: none; else one sequence, visible to every row
+    RowsView r;
+    uint32_t window, sinks; // window 0: unlimited
+};
+
+struct ColsumArgs { // acc_out = acc_in + the rows' attention weights
+    KvView own;
+    RowsView r;       // lse set
+    const float *acc; // nullable
+    float *acc_out;   // [n_seq][kv_heads][slots]
+};
+
+// Eviction, first step: per (sequence, kv head) the source slot of each of the `keep`
+// slots that stay.
+struct EvictArgs {
+    KvView c;
+    void *k_out, *v_out; // may be c.k and c.v (then with its strides): in place
+    int64_t oss, ohs, ots;
+    const float *acc;    // [n_seq][kv_heads][slots]
+    const int32_t *pos;
+    float *acc_out;      // [n_seq][kv_heads][out_slots]
+    int32_t *pos_out, *len_out;
+    uint32_t keep, sinks, recent, out_slots, dim;
+    uint32_t in_place, acc_in_place, pos_in_place;
+    // workspace, per (sequence, kv head): map[n] (n < keep) is slot n itself, or ~i for
+    // the i-th hole, which movers[i] fills; head = {slots that remain, whether any leaves}
+    int32_t *map, *movers, *head;
+};

@@ -1,0 +1,430 @@
+// attn_ops.cpp -- C ABI of the cache-attention operators: argument checks, work splits and
+// launches of the kernels in lfm_attn.hip.
+#include <hip/hip_runtime_api.h>
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+
+#include <algorithm>
+#include <exception>
+#include <mutex>
+#include <unordered_map>
+
+#include "../../include/lfm_hip.h"
+#include "attn_args.h"
+#include "host_err.h"
+#include "launch_host.h"
+
+#define RC(call)                                                                              \
+    do {                                                                                      \
+        int _rc = (call);                                                                     \
+        if (_rc != LFM_OK)                                                                    \
+            return _rc;                                                                       \
+    } while (0)
+
+// ------------------------------------------------------------------ code object
+// Kernels by [type pair][head_dim 64, 128]; the pair is the rows' type.
+struct AttnKernels {
+    hipModule_t mod = nullptr;
+    hipFunction_t attn_simple[3][2], colsum_simple[3][2];
+    hipFunction_t kv_select, kv_move;
+};
+
+static std::mutex g_mu;
+static std::unordered_map<int, AttnKernels *> g_attn;
+
+static int load_attn(int dev)
+{
+    const std::string path = lfm_beside_code_object("lfm_attn.hsaco");
+    AttnKernels k;
+    hipError_t e = hipModuleLoad(&k.mod, path.c_str());
+    if (e != hipSuccess)
+        return fail(LFM_EDEVICE, "hipModuleLoad(%s): %s", path.c_str(), hipGetErrorString(e));
+    static const char *const types[3] = {"f32", "f16", "bf16"};
+    auto get = [&](hipFunction_t *f, const std::string &name) -> int {
+        const hipError_t r = hipModuleGetFunction(f, k.mod, name.c_str());
+        return r == hipSuccess ? LFM_OK
+                               : fail(LFM_EDEVICE, "hipModuleGetFunction(%s): %s", name.c_str(), hipGetErrorString(r));
+    };
+    int rc = LFM_OK;
+    for (int t = 0; t < 3 && rc == LFM_OK; ++t)
+        for (int d = 0; d < 2 && rc == LFM_OK; ++d) {
+            const std::string tag = std::string("_") + types[t] + (d ? "_128" : "_64");
+            rc = get(&k.attn_simple[t][d], "k_attn_simple" + tag);
+            if (rc == LFM_OK)
+                rc = get(&k.colsum_simple[t][d], "k_colsum_simple" + tag);
+        }
+    if (rc == LFM_OK)
+        rc = get(&k.kv_select, "k_kv_select");
+    if (rc == LFM_OK)
+        rc = get(&k.kv_move, "k_kv_move");
+    if (rc != LFM_OK) {
+        (void)hipModuleUnload(k.mod);
+        return rc;
+    }
+    g_attn[dev] = new AttnKernels(k);
+    return LFM_OK;
+}
+
+// The code object on the current device, loaded by the device's first call.
+static int attn_kernels(int dev, AttnKernels **out)
+{
+    try {
+        std::lock_guard<std::mutex> lk(g_mu);
+        auto it = g_attn.find(dev);
+        if (it == g_attn.end()) {
+            RC(load_attn(dev));
+            it = g_attn.find(dev);
+        }
+        *out = it->second;
+        return LFM_OK;
+    } catch (const std::exception &x) {
+        return fail(LFM_EINTERNAL, "loading the attention kernels: %s", x.what());
+    }
+}
+
+template <typename A> static int launch(hipFunction_t f, dim3 grid, uint32_t threads, hipStream_t s, const A &args)
+{
+    void *params[] = {(void *)&args};
+    const hipError_t e = hipModuleLaunchKernel(f, grid.x, grid.y, grid.z, threads, 1, 1, 0, s, params, nullptr);
+    return e == hipSuccess ? LFM_OK : fail(LFM_EDEVICE, "kernel launch failed: %s", hipGetErrorString(e));
+}
+
+// ------------------------------------------------------------------ argument checks
+// Sizes and strides; they decide the workspace and need no device.
+static int check_kv(const char *op, const char *name, const lfm_kv *c)
+{
+    if (!c)
+        return fail(LFM_EINVAL, "%s: %s is null", op, name);
+    if (c->type != LFM_TYPE_F16 && c->type != LFM_TYPE_BF16)
+        return fail(LFM_EINVAL, "%s: %s: type %u (a cache is F16 or BF16)", op, name, c->type);
+    if (c->head_dim != 64 && c->head_dim != 128)
+        return fail(LFM_EINVAL, "%s: %s: head_dim %u (64 or 128)", op, name, c->head_dim);
+    if (c->kv_heads == 0 || c->kv_heads > 65535 || c->n_seq > 65535)
+        return fail(LFM_EINVAL, "%s: %s: %u sequences of %u kv heads (at most 65535, 1..65535)", op, name, c->n_seq,
+                    c->kv_heads);
+    if (c->slots == 0 || c->slots > 0x7FFFFF00u)
+        return fail(LFM_EINVAL, "%s: %s: %u slots (1..%u)", op, name, c->slots, 0x7FFFFF00u);
+    for (int64_t s : {c->seq_stride, c->head_stride, c->slot_stride})
+        if (s < 0 || s % 8)
+            return fail(LFM_EINVAL, "%s: %s: stride %lld (multiples of 8 elements, not negative)", op, name,
+                        (long long)s);
+    return LFM_OK;
+}
+
+static int check_rows(const char *op, const lfm_kv *c, const lfm_rows *r)
+{
+    if (!r)
+        return fail(LFM_EINVAL, "%s: rows is null", op);
+    if (r->type > LFM_TYPE_BF16 || (r->type == LFM_TYPE_BF16) != (c->type == LFM_TYPE_BF16))
+        return fail(LFM_EINVAL, "%s: rows of type %u over a cache of type %u (F32 or F16 over F16, BF16 over BF16)",
+                    op, r->type, c->type);
+    if (r->heads == 0 || r->heads % c->kv_heads || r->heads > 65535)
+        return fail(LFM_EINVAL, "%s: %u heads over %u kv heads (a multiple, at most 65535)", op, r->heads,
+                    c->kv_heads);
+    if (r->n_rows > 0x7FFFFFFFu)
+        return fail(LFM_EINVAL, "%s: %u rows", op, r->n_rows);
+    if (!r->start && r->n_rows != c->n_seq)
+        return fail(LFM_EINVAL, "%s: %u rows for %u sequences without start (one row each)", op, r->n_rows, c->n_seq);
+    if (!(r->scale > 0.f) || !(r->scale < INFINITY))
+        return fail(LFM_EINVAL, "%s: scale %g (a positive number)", op, (double)r->scale);
+    const int64_t q = r->type == LFM_TYPE_F32 ? 4 : 8;
+    for (int64_t s : {r->q_row_stride, r->q_head_stride, r->out_row_stride, r->out_head_stride})
+        if (s < 0 || s % q)
+            return fail(LFM_EINVAL, "%s: row or head stride %lld (multiples of 16 bytes, not negative)", op,
+                        (long long)s);
+    if ((r->n_rows > 1 && r->out_row_stride == 0) || (r->heads > 1 && r->out_head_stride == 0))
+        return fail(LFM_EINVAL, "%s: an out stride of 0", op);
+    return LFM_OK;
+}
+
+// A device pointer of the current device (or managed memory), aligned.
+static int check_ptr(const char *op, const char *name, const void *p, size_t align, int dev)
+{
+    if (!p)
+        return fail(LFM_EINVAL, "%s: %s is null", op, name);
+    if ((uintptr_t)p % align)
+        return fail(LFM_EINVAL, "%s: %s is not %zu-byte aligned", op, name, align);
+    hipPointerAttribute_t at;
+    if (hipPointerGetAttributes(&at, p) != hipSuccess) {
+        (void)hipGetLastError();
+        return fail(LFM_EINVAL, "%s: %s is not device memory", op, name);
+    }
+    if (at.type != hipMemoryTypeDevice && at.type != hipMemoryTypeManaged)
+        return fail(LFM_EINVAL, "%s: %s is not device memory", op, name);
+    if (at.type == hipMemoryTypeDevice && at.device != dev)
+        return fail(LFM_EINVAL, "%s: %s lies on device %d, the current one is %d", op, name, at.device, dev);
+    return LFM_OK;
+}
+
+// The current device; `stream` has to be its own.
+static int current_device(const char *op, hipStream_t s, int *dev)
+{
+    if (hipGetDevice(dev) != hipSuccess) {
+        (void)hipGetLastError();
+        return fail(LFM_EDEVICE, "%s: no current device", op);
+    }
+    hipDevice_t of;
+    if (s && (hipStreamGetDevice(s, &of) != hipSuccess || of != *dev)) {
+        (void)hipGetLastError();
+        return fail(LFM_EINVAL, "%s: the stream is not one of the current device (%d)", op, *dev);
+    }
+    return LFM_OK;
+}
+
+static int check_kv_ptrs(const char *op, const char *const (&names)[3], const lfm_kv *c, int dev)
+{
+    RC(check_ptr(op, names[0], c->k, 16, dev));
+    RC(check_ptr(op, names[1], c->v, 16, dev));
+    return check_ptr(op, names[2], c->len, 4, dev);
+}
+static const char *const KV_NAMES[3] = {"kv->k", "kv->v", "kv->len"};
+static const char *const PREFIX_NAMES[3] = {"prefix->k", "prefix->v", "prefix->len"};
+static const char *const OUT_NAMES[3] = {"out->k", "out->v", "out->len"};
+
+static int check_rows_ptrs(const char *op, const lfm_rows *r, int dev)
+{
+    RC(check_ptr(op, "rows->q", r->q, 16, dev));
+    RC(check_ptr(op, "rows->out", r->out, 16, dev));
+    if (r->q == r->out)
+        return fail(LFM_EINVAL, "%s: out is q", op);
+    if (r->lse)
+        RC(check_ptr(op, "rows->lse", r->lse, 4, dev));
+    if (r->start)
+        RC(check_ptr(op, "rows->start", r->start, 4, dev));
+    return LFM_OK;
+}
+
+static int check_workspace(const char *op, void *p, size_t have, size_t need, int dev)
+{
+    if (have < need)
+        return fail(LFM_EINVAL, "%s: %zu bytes of workspace, %zu needed", op, have, need);
+    return need ? check_ptr(op, "workspace", p, 16, dev) : LFM_OK;
+}
+
+static KvView view(const lfm_kv *c)
+{
+    KvView v;
+    memset(&v, 0, sizeof(v));
+    v.k = (const uint16_t *)c->k;
+    v.v = (const uint16_t *)c->v;
+    v.len = c->len;
+    v.ss = c->seq_stride, v.hs = c->head_stride, v.ts = c->slot_stride;
+    v.n_seq = c->n_seq, v.kv_heads = c->kv_heads, v.slots = c->slots;
+    return v;
+}
+
+static RowsView view(const lfm_rows *r)
+{
+    RowsView v;
+    memset(&v, 0, sizeof(v));
+    v.q = r->q, v.out = r->out, v.lse = r->lse, v.start = r->start;
+    v.q_rs = r->q_row_stride, v.q_hs = r->q_head_stride;
+    v.o_rs = r->out_row_stride, v.o_hs = r->out_head_stride;
+    v.heads = r->heads, v.n_rows = r->n_rows;
+    v.scale = r->scale;
+    v.cexp = (float)((double)r->scale * 1.4426950408889634);
+    return v;
+}
+
+static int dim_index(const lfm_kv *c) { return c->head_dim == 128; }
+
+// ------------------------------------------------------------------ attention
+static int attend(const char *op, const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *rows, uint32_t window,
+                  uint32_t sinks, float *lse, hipStream_t s, int dev)
+{
+    AttnKernels *K;
+    RC(attn_kernels(dev, &K));
+    AttnOpArgs a;
+    memset(&a, 0, sizeof(a));
+    a.own = view(kv);
+    if (prefix)
+        a.prefix = view(prefix);
+    a.r = view(rows);
+    a.r.lse = lse;
+    a.window = window, a.sinks = sinks;
+    return launch(K->attn_simple[rows->type][dim_index(kv)], dim3(rows->n_rows, rows->heads), 64, s, a);
+}
+
+extern "C" int lfm_attn_window_workspace(const lfm_kv *kv, const lfm_rows *rows, uint32_t window, uint32_t sinks,
+                                         size_t *bytes)
+{
+    const char *op = "lfm_attn_window_workspace";
+    (void)window, (void)sinks;
+    RC(check_kv(op, "kv", kv));
+    RC(check_rows(op, kv, rows));
+    if (!bytes)
+        return fail(LFM_EINVAL, "%s: bytes is null", op);
+    *bytes = 0;
+    return LFM_OK;
+}
+
+extern "C" int lfm_attn_window(const lfm_kv *kv, const lfm_rows *rows, uint32_t window, uint32_t sinks,
+                               void *workspace, size_t workspace_bytes, void *stream)
+{
+    const char *op = "lfm_attn_window";
+    size_t need;
+    RC(lfm_attn_window_workspace(kv, rows, window, sinks, &need));
+    if (rows->n_rows == 0 || kv->n_seq == 0)
+        return LFM_OK;
+    int dev;
+    RC(current_device(op, (hipStream_t)stream, &dev));
+    RC(check_kv_ptrs(op, KV_NAMES, kv, dev));
+    RC(check_rows_ptrs(op, rows, dev));
+    RC(check_workspace(op, workspace, workspace_bytes, need, dev));
+    return attend(op, nullptr, kv, rows, window, sinks, rows->lse, (hipStream_t)stream, dev);
+}
+
+extern "C" int lfm_attn_scored_workspace(const lfm_kv *kv, const lfm_rows *rows, size_t *bytes)
+{
+    const char *op = "lfm_attn_scored_workspace";
+    RC(check_kv(op, "kv", kv));
+    RC(check_rows(op, kv, rows));
+    if (!bytes)
+        return fail(LFM_EINVAL, "%s: bytes is null", op);
+    *bytes = ((size_t)rows->n_rows * rows->heads * 4 + 255) / 256 * 256; // lse, where the caller wants none
+    return LFM_OK;
+}
+
+extern "C" int lfm_attn_scored(const lfm_kv *kv, const lfm_rows *rows, const float *acc_in, float *acc_out,
+                               void *workspace, size_t workspace_bytes, void *stream)
+{
+    const char *op = "lfm_attn_scored";
+    size_t need;
+    RC(lfm_attn_scored_workspace(kv, rows, &need));
+    if (kv->n_seq == 0)
+        return LFM_OK;
+    int dev;
+    RC(current_device(op, (hipStream_t)stream, &dev));
+    RC(check_kv_ptrs(op, KV_NAMES, kv, dev));
+    if (rows->n_rows)
+        RC(check_rows_ptrs(op, rows, dev));
+    if (acc_in)
+        RC(check_ptr(op, "acc_in", acc_in, 4, dev));
+    RC(check_ptr(op, "acc_out", acc_out, 4, dev));
+    RC(check_workspace(op, workspace, workspace_bytes, need, dev));
+    hipStream_t s = (hipStream_t)stream;
+    float *lse = rows->lse ? rows->lse : (float *)workspace;
+    if (rows->n_rows)
+        RC(attend(op, nullptr, kv, rows, 0, 0, lse, s, dev));
+    AttnKernels *K;
+    RC(attn_kernels(dev, &K));
+    ColsumArgs a;
+    memset(&a, 0, sizeof(a));
+    a.own = view(kv);
+    a.r = view(rows);
+    a.r.lse = lse;
+    a.acc = acc_in, a.acc_out = acc_out;
+    return launch(K->colsum_simple[rows->type][dim_index(kv)], dim3((kv->slots + 63) / 64, kv->kv_heads, kv->n_seq),
+                  64, s, a);
+}
+
+static int check_prefix(const char *op, const lfm_kv *prefix, const lfm_kv *kv)
+{
+    RC(check_kv(op, "prefix", prefix));
+    RC(check_kv(op, "kv", kv));
+    if (prefix->n_seq != 1)
+        return fail(LFM_EINVAL, "%s: a prefix of %u sequences (1)", op, prefix->n_seq);
+    if (prefix->kv_heads != kv->kv_heads || prefix->head_dim != kv->head_dim || prefix->type != kv->type)
+        return fail(LFM_EINVAL, "%s: prefix and kv differ in kv_heads, head_dim or type", op);
+    return LFM_OK;
+}
+
+extern "C" int lfm_attn_prefix_workspace(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *rows, size_t *bytes)
+{
+    const char *op = "lfm_attn_prefix_workspace";
+    RC(check_prefix(op, prefix, kv));
+    RC(check_rows(op, kv, rows));
+    if (!bytes)
+        return fail(LFM_EINVAL, "%s: bytes is null", op);
+    *bytes = 0;
+    return LFM_OK;
+}
+
+extern "C" int lfm_attn_prefix(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *rows, void *workspace,
+                               size_t workspace_bytes, void *stream)
+{
+    const char *op = "lfm_attn_prefix";
+    size_t need;
+    RC(lfm_attn_prefix_workspace(prefix, kv, rows, &need));
+    if (rows->n_rows == 0 || kv->n_seq == 0)
+        return LFM_OK;
+    int dev;
+    RC(current_device(op, (hipStream_t)stream, &dev));
+    RC(check_kv_ptrs(op, PREFIX_NAMES, prefix, dev));
+    RC(check_kv_ptrs(op, KV_NAMES, kv, dev));
+    RC(check_rows_ptrs(op, rows, dev));
+    RC(check_workspace(op, workspace, workspace_bytes, need, dev));
+    return attend(op, prefix, kv, rows, 0, 0, rows->lse, (hipStream_t)stream, dev);
+}
+
+// ------------------------------------------------------------------ eviction
+static size_t evict_list_bytes(const lfm_kv *kv, uint32_t keep)
+{
+    return ((size_t)kv->n_seq * kv->kv_heads * keep * 4 + 255) / 256 * 256;
+}
+
+extern "C" int lfm_kv_evict_workspace(const lfm_kv *kv, uint32_t keep, size_t *bytes)
+{
+    const char *op = "lfm_kv_evict_workspace";
+    RC(check_kv(op, "kv", kv));
+    if (keep == 0 || keep > 0x7FFFFF00u)
+        return fail(LFM_EINVAL, "%s: keep %u", op, keep);
+    if (!bytes)
+        return fail(LFM_EINVAL, "%s: bytes is null", op);
+    *bytes = 2 * evict_list_bytes(kv, keep) + (size_t)kv->n_seq * kv->kv_heads * 8;
+    return LFM_OK;
+}
+
+extern "C" int lfm_kv_evict(const lfm_kv *kv, const float *acc, const int32_t *pos, uint32_t keep, uint32_t sinks,
+                            uint32_t recent, const lfm_kv *out, float *acc_out, int32_t *pos_out, void *workspace,
+                            size_t workspace_bytes, void *stream)
+{
+    const char *op = "lfm_kv_evict";
+    size_t need;
+    RC(lfm_kv_evict_workspace(kv, keep, &need));
+    RC(check_kv(op, "out", out));
+    if (out->n_seq != kv->n_seq || out->kv_heads != kv->kv_heads || out->head_dim != kv->head_dim ||
+        out->type != kv->type)
+        return fail(LFM_EINVAL, "%s: out and kv differ in n_seq, kv_heads, head_dim or type", op);
+    if ((uint64_t)sinks + recent > keep)
+        return fail(LFM_EINVAL, "%s: sinks %u and recent %u do not fit into keep %u", op, sinks, recent, keep);
+    if (keep > out->slots)
+        return fail(LFM_EINVAL, "%s: keep %u, out holds %u slots", op, keep, out->slots);
+    const bool in_place = out->k == kv->k;
+    if (in_place != (out->v == kv->v) ||
+        (in_place && (out->seq_stride != kv->seq_stride || out->head_stride != kv->head_stride ||
+                      out->slot_stride != kv->slot_stride)))
+        return fail(LFM_EINVAL, "%s: in place needs both k and v, with the same strides", op);
+    if (((acc_out == acc && acc) || (pos_out == pos && pos)) && out->slots != kv->slots)
+        return fail(LFM_EINVAL, "%s: acc or pos in place needs out of %u slots", op, kv->slots);
+    if ((out->n_seq > 1 && out->seq_stride == 0) || (out->kv_heads > 1 && out->head_stride == 0) ||
+        (keep > 1 && out->slot_stride == 0))
+        return fail(LFM_EINVAL, "%s: out has a stride of 0", op);
+    if (kv->n_seq == 0)
+        return LFM_OK;
+    int dev;
+    RC(current_device(op, (hipStream_t)stream, &dev));
+    RC(check_kv_ptrs(op, KV_NAMES, kv, dev));
+    RC(check_kv_ptrs(op, OUT_NAMES, out, dev));
+    RC(check_ptr(op, "acc", acc, 4, dev));
+    RC(check_ptr(op, "pos", pos, 4, dev));
+    RC(check_ptr(op, "acc_out", acc_out, 4, dev));
+    RC(check_ptr(op, "pos_out", pos_out, 4, dev));
+    RC(check_workspace(op, workspace, workspace_bytes, need, dev));
+    AttnKernels *K;
+    RC(attn_kernels(dev, &K));
+    EvictArgs a;
+    memset(&a, 0, sizeof(a));
+    a.c = view(kv);
+    a.k_out = out->k, a.v_out = out->v;
+    a.oss = out->seq_stride, a.ohs = out->head_stride, a.ots = out->slot_stride;
+    a.acc = acc, a.pos = pos, a.acc_out = acc_out, a.pos_out = pos_out, a.len_out = out->len;
+    a.keep = keep, a.sinks = sinks, a.recent = recent, a.out_slots = out->slots, a.dim = kv->head_dim;
+    a.in_place = in_place, a.acc_in_place = acc == acc_out, a.pos_in_place = pos == pos_out;
+    a.map = (int32_t *)workspace;
+    a.movers = (int32_t *)((uint8_t *)workspace + evict_list_bytes(kv, keep));
+    a.head = (int32_t *)((uint8_t *)workspace + 2 * evict_list_bytes(kv, keep));
+    RC(launch(K->kv_select, dim3(kv->kv_heads, kv->n_seq), 1024, (hipStream_t)stream, a));
+    return launch(K->kv_move, dim3((keep + 31) / 32, kv->kv_heads, kv->n_seq), 256, (hipStream_t)stream, a);
+}

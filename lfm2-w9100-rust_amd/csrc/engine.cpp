@@ -175,13 +175,15 @@ static std::string code_object_path()
     return "lfm_kernels.hsaco";
 }
 
-// The prefill kernels live in a second code object next to the first.
-static std::string prefill_object_path()
+std::string lfm_beside_code_object(const char *file)
 {
     std::string p = code_object_path();
     const size_t slash = p.rfind('/');
-    return (slash == std::string::npos ? std::string(".") : p.substr(0, slash)) + "/lfm_prefill.hsaco";
+    return (slash == std::string::npos ? std::string(".") : p.substr(0, slash)) + "/" + file;
 }
+
+// The prefill kernels live in a second code object next to the first.
+static std::string prefill_object_path() { return lfm_beside_code_object("lfm_prefill.hsaco"); }
 
 // Loads the code object on the current device (once per device).
 static int get_kernels(Kernels **out)

@@ -1,11 +1,17 @@
 // launch_host.h -- host-side launch helpers shared by the library's sources
-// (engine.cpp, noalloc.hip); not part of the C ABI.
+// (engine.cpp, attn_ops.cpp, noalloc.hip); not part of the C ABI.
 #pragma once
 
 #include <hip/hip_runtime_api.h>
 #include <stdint.h>
 
+#include <string>
+
 #include "kargs.h"
+
+// Path of a code object that lies beside the first one (the directory of the library, or
+// of the file LFM_KERNELS names).
+__attribute__((visibility("hidden"))) std::string lfm_beside_code_object(const char *file);
 
 // Workgroups of the first argmax stage: one per 256 values, at most
 // NOALLOC_ARGMAX_WGS (the stage is grid-stride beyond that).

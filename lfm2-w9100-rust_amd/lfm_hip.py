@@ -74,6 +74,31 @@ class SynthOpts(C.Structure):
     ]
 
 
+TYPE_F32, TYPE_F16, TYPE_BF16 = range(3)
+
+
+class Kv(C.Structure):
+    """``lfm_kv``: K and V of a batch of sequences on the device."""
+
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("len", C.c_void_p), ("seq_stride", C.c_int64),
+        ("head_stride", C.c_int64), ("slot_stride", C.c_int64), ("type", C.c_uint32),
+        ("n_seq", C.c_uint32), ("kv_heads", C.c_uint32), ("slots", C.c_uint32),
+        ("head_dim", C.c_uint32),
+    ]
+
+
+class Rows(C.Structure):
+    """``lfm_rows``: query rows and their outputs."""
+
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("start", C.c_void_p),
+        ("q_row_stride", C.c_int64), ("q_head_stride", C.c_int64), ("out_row_stride", C.c_int64),
+        ("out_head_stride", C.c_int64), ("type", C.c_uint32), ("heads", C.c_uint32),
+        ("n_rows", C.c_uint32), ("scale", C.c_float),
+    ]
+
+
 (GGUF_U8, GGUF_I8, GGUF_U16, GGUF_I16, GGUF_U32, GGUF_I32, GGUF_F32, GGUF_BOOL, GGUF_STRING,
  GGUF_ARRAY, GGUF_U64, GGUF_I64, GGUF_F64) = range(13)
 GGUF_MAX_DIMS = 8
@@ -170,6 +195,14 @@ def lib():
         "lfm_q6k_matvec": (i32, [P, u64, u64, P, P, P]),
         "lfm_q6k_matvec_time": (i32, [P, u32, u64, u64, P, P, u32, pf32]),
         "lfm_q6k_gemm": (i32, [P, u64, u64, P, u32, P, P]),
+        "lfm_attn_window": (i32, [C.POINTER(Kv), C.POINTER(Rows), u32, u32, P, sz, P]),
+        "lfm_attn_window_workspace": (i32, [C.POINTER(Kv), C.POINTER(Rows), u32, u32, C.POINTER(sz)]),
+        "lfm_attn_scored": (i32, [C.POINTER(Kv), C.POINTER(Rows), P, P, P, sz, P]),
+        "lfm_attn_scored_workspace": (i32, [C.POINTER(Kv), C.POINTER(Rows), C.POINTER(sz)]),
+        "lfm_attn_prefix": (i32, [C.POINTER(Kv), C.POINTER(Kv), C.POINTER(Rows), P, sz, P]),
+        "lfm_attn_prefix_workspace": (i32, [C.POINTER(Kv), C.POINTER(Kv), C.POINTER(Rows), C.POINTER(sz)]),
+        "lfm_kv_evict": (i32, [C.POINTER(Kv), P, P, u32, u32, u32, C.POINTER(Kv), P, P, P, sz, P]),
+        "lfm_kv_evict_workspace": (i32, [C.POINTER(Kv), u32, C.POINTER(sz)]),
         "lfm_argmax": (i32, [P, u32, pu32, pf32]),
         "lfm_argmax_noalloc": (i32, [P, u32, pu32, pf32]),
         "lfm_synth_default_opts": (None, [C.POINTER(SynthOpts)]),
@@ -590,6 +623,194 @@ class DeviceBuffer:
             self.free()
         except Exception:
             pass
+
+
+# ------------------------------------------------------------------ attention over caches
+class DeviceTensor:
+    """A strided view of device memory for the cache-attention operators: what they take
+    beside torch tensors.  ``strides`` are in elements (default: row-major); dtype is a
+    numpy dtype or "bf16" (whose host arrays are the uint16 bit patterns)."""
+
+    def __init__(self, buf: DeviceBuffer, shape: Sequence[int], dtype, offset: int = 0,
+                 strides: Optional[Sequence[int]] = None):
+        self.buf, self.shape, self.offset = buf, tuple(int(n) for n in shape), int(offset)
+        self.dtype = "bf16" if isinstance(dtype, str) and dtype == "bf16" else np.dtype(dtype)
+        self.strides = tuple(strides) if strides is not None else _row_major(self.shape)
+        item = 2 if self.dtype == "bf16" else self.dtype.itemsize
+        last = sum((n - 1) * s for n, s in zip(self.shape, self.strides))
+        if all(self.shape) and (min(self.strides, default=0) < 0 or self.offset < 0
+                                or (self.offset + last + 1) * item > buf.nbytes):
+            raise LfmError(LFM_EINVAL, "the view reaches past its buffer")
+        self._ptr = buf.ptr + self.offset * item
+
+    @classmethod
+    def from_array(cls, a: np.ndarray, dtype=None) -> "DeviceTensor":
+        a = np.ascontiguousarray(a)
+        return cls(DeviceBuffer.from_array(a), a.shape, a.dtype if dtype is None else dtype)
+
+    def data_ptr(self) -> int:
+        return self._ptr
+
+    def stride(self):
+        return self.strides
+
+    def download(self) -> np.ndarray:
+        """The whole buffer's values, in its own order (bf16: bit patterns)."""
+        return self.buf.download(np.uint16 if self.dtype == "bf16" else self.dtype)
+
+
+def _row_major(shape):
+    out, n = [], 1
+    for d in reversed(shape):
+        out.append(n)
+        n *= d
+    return tuple(reversed(out))
+
+
+_DTYPES = {"float32": "f32", "torch.float32": "f32", "float16": "f16", "torch.float16": "f16",
+           "bf16": "bf16", "torch.bfloat16": "bf16", "int32": "i32", "torch.int32": "i32"}
+_TYPES = {"f32": TYPE_F32, "f16": TYPE_F16, "bf16": TYPE_BF16}
+
+
+def _dtype(t) -> str:
+    return _DTYPES.get(str(t.dtype), str(t.dtype))
+
+
+def _dense(t, what: str, dtype: str, shape) -> int:
+    """Address of a row-major device array of this type and shape."""
+    if _dtype(t) != dtype or tuple(t.shape) != tuple(shape) or \
+            any(n > 1 and s != r for n, s, r in zip(shape, t.stride(), _row_major(shape))):
+        raise LfmError(LFM_EINVAL, f"{what}: a row-major {dtype} array of {tuple(shape)} expected, got "
+                       f"{_dtype(t)} {tuple(t.shape)} with strides {tuple(t.stride())}")
+    return t.data_ptr()
+
+
+class KvCache:
+    """K and V of a batch of sequences: device tensors [n_seq][kv_heads][slots][head_dim]
+    (torch tensors or DeviceTensors; the last dimension contiguous, K and V with the same
+    strides) and the slots in use per sequence (int32 [n_seq], on the device too).  It
+    holds the tensors, not copies."""
+
+    def __init__(self, k, v, length):
+        if len(k.shape) != 4 or tuple(k.shape) != tuple(v.shape) or _dtype(k) != _dtype(v):
+            raise LfmError(LFM_EINVAL, "k and v: two arrays [n_seq][kv_heads][slots][head_dim] of one type expected")
+        kind = _TYPES.get(_dtype(k), TYPE_F32)
+        if kind == TYPE_F32:
+            raise LfmError(LFM_EINVAL, f"a cache of {_dtype(k)} (binary16 or bfloat16 expected)")
+        ks, vs = tuple(k.stride()), tuple(v.stride())
+        n, heads, slots, dim = (int(x) for x in k.shape)
+        if any(size > 1 and a != b for size, a, b in zip(k.shape, ks, vs)) or (dim > 1 and ks[3] != 1):
+            raise LfmError(LFM_EINVAL, f"k and v: equal strides with a contiguous last dimension expected: {ks}, {vs}")
+        self.k, self.v, self.length = k, v, length
+        self.n_seq, self.kv_heads, self.slots, self.head_dim, self.type = n, heads, slots, dim, kind
+        # a dimension of size one may have any stride in its tensor: it is never used
+        self._c = Kv(k.data_ptr(), v.data_ptr(), _dense(length, "length", "i32", (n,)),
+                     ks[0] if n > 1 else 0, ks[1] if heads > 1 else 0, ks[2] if slots > 1 else 0, kind, n,
+                     heads, slots, dim)
+        self._ref = C.byref(self._c)
+
+
+def _rows(q, cache: KvCache, out, start, scale, lse):
+    if len(q.shape) != 3 or q.shape[2] != cache.head_dim:
+        raise LfmError(LFM_EINVAL, f"q: [n_rows][heads][{cache.head_dim}] expected, got {tuple(q.shape)}")
+    n, heads, dim = q.shape
+    qs = q.stride()
+    kind = _TYPES.get(_dtype(q))
+    if kind is None or qs[2] != 1:
+        raise LfmError(LFM_EINVAL, f"q: {_dtype(q)} with strides {tuple(qs)} (float32, binary16 or bfloat16, the last "
+                       "dimension contiguous)")
+    os_, optr = qs, None
+    if out is not None:
+        os_ = out.stride()
+        if tuple(out.shape) != tuple(q.shape) or _dtype(out) != _dtype(q) or os_[2] != 1:
+            raise LfmError(LFM_EINVAL, "out: q's shape and type expected, the last dimension contiguous")
+        optr = out.data_ptr()
+    one, single = n > 1, heads > 1
+    return Rows(q.data_ptr(), optr, None if lse is None else _dense(lse, "lse", "f32", (n, heads)),
+                None if start is None else _dense(start, "start", "i32", (cache.n_seq + 1,)),
+                qs[0] if one else 0, qs[1] if single else 0, os_[0] if one else 0, os_[1] if single else 0,
+                kind, heads, n, dim ** -0.5 if scale is None else scale)
+
+
+def _space(workspace):
+    """Address and bytes of a workspace: a DeviceBuffer or a torch tensor of bytes."""
+    if isinstance(workspace, DeviceBuffer):
+        return workspace.ptr, workspace.nbytes
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def attn_window_workspace(q, cache: KvCache, *, window: int = 0, sinks: int = 0, start=None) -> int:
+    n = C.c_size_t()
+    _check(lib().lfm_attn_window_workspace(cache._ref, C.byref(_rows(q, cache, None, start, None, None)), window,
+                                           sinks, C.byref(n)))
+    return n.value
+
+
+def attn_window(q, cache: KvCache, out, workspace, *, window: int = 0, sinks: int = 0, start=None,
+                scale: Optional[float] = None, lse=None, stream: int = 0):
+    """out[row][head] = softmax(scale q K^T) V over the newest ``window`` positions up to the
+    row's own (0: all) and the first ``sinks`` (lfm_attn_window).  q and out are
+    [n_rows][heads][head_dim]; start (int32 [n_seq + 1], device) gives each sequence's rows,
+    None one row per sequence.  Enqueued on ``stream`` (a HIP stream's address); workspace:
+    attn_window_workspace(...) bytes for the same arguments."""
+    r = _rows(q, cache, out, start, scale, lse)
+    p, n = _space(workspace)
+    _check(lib().lfm_attn_window(cache._ref, C.byref(r), window, sinks, p, n, stream))
+
+
+def attn_scored_workspace(q, cache: KvCache, *, start=None) -> int:
+    n = C.c_size_t()
+    _check(lib().lfm_attn_scored_workspace(cache._ref, C.byref(_rows(q, cache, None, start, None, None)),
+                                           C.byref(n)))
+    return n.value
+
+
+def attn_scored(q, cache: KvCache, out, acc_in, acc_out, workspace, *, start=None,
+                scale: Optional[float] = None, lse=None, stream: int = 0):
+    """Attention over all positions, and acc_out = acc_in + the weights that every slot in
+    use receives from its kv head's query heads and the sequence's rows (lfm_attn_scored).
+    acc [n_seq][kv_heads][slots] float32; acc_in None counts as zeros, and may be acc_out."""
+    r = _rows(q, cache, out, start, scale, lse)
+    shape = (cache.n_seq, cache.kv_heads, cache.slots)
+    p, n = _space(workspace)
+    _check(lib().lfm_attn_scored(cache._ref, C.byref(r),
+                                 None if acc_in is None else _dense(acc_in, "acc_in", "f32", shape),
+                                 _dense(acc_out, "acc_out", "f32", shape), p, n, stream))
+
+
+def attn_prefix_workspace(q, prefix: KvCache, cache: KvCache, *, start=None) -> int:
+    n = C.c_size_t()
+    _check(lib().lfm_attn_prefix_workspace(prefix._ref, cache._ref,
+                                           C.byref(_rows(q, cache, None, start, None, None)), C.byref(n)))
+    return n.value
+
+
+def attn_prefix(q, prefix: KvCache, cache: KvCache, out, workspace, *, start=None,
+                scale: Optional[float] = None, lse=None, stream: int = 0):
+    """Attention of a batch that shares a prefix (a KvCache of one sequence): every row sees
+    the whole prefix, then its own sequence up to its position (lfm_attn_prefix)."""
+    r = _rows(q, cache, out, start, scale, lse)
+    p, n = _space(workspace)
+    _check(lib().lfm_attn_prefix(prefix._ref, cache._ref, C.byref(r), p, n, stream))
+
+
+def kv_evict_workspace(cache: KvCache, keep: int) -> int:
+    n = C.c_size_t()
+    _check(lib().lfm_kv_evict_workspace(cache._ref, keep, C.byref(n)))
+    return n.value
+
+
+def kv_evict(cache: KvCache, acc, pos, keep: int, out: KvCache, acc_out, pos_out, workspace, *,
+             sinks: int = 0, recent: int = 0, stream: int = 0):
+    """Keeps ``keep`` slots of every longer sequence, per kv head: the first ``sinks`` and the
+    newest ``recent`` positions, then the slots of highest acc (lfm_kv_evict).  In place
+    where out is cache, acc_out is acc and pos_out is pos."""
+    a = (cache.n_seq, cache.kv_heads, cache.slots)
+    b = (cache.n_seq, cache.kv_heads, out.slots)
+    p, n = _space(workspace)
+    _check(lib().lfm_kv_evict(cache._ref, _dense(acc, "acc", "f32", a), _dense(pos, "pos", "i32", a), keep, sinks,
+                              recent, out._ref, _dense(acc_out, "acc_out", "f32", b),
+                              _dense(pos_out, "pos_out", "i32", b), p, n, stream))
 
 
 # ------------------------------------------------------------------ Q6_K operator API
