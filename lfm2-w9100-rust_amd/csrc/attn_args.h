@@ -2,6 +2,7 @@
 // launcher (attn_ops.cpp) and the gfx950 kernels (lfm_attn.hip).  Every kernel takes one
 // of these structs by value.
 #pragma once
+#include <hip/hip_vector_types.h>
 #include <stdint.h>
 
 // K and V of n_seq sequences: element (b, h, slot, d) at b * ss + h * hs + slot * ts + d.
@@ -24,11 +25,25 @@ struct RowsView {
     float scale, cexp; // cexp = scale * log2(e)
 };
 
+#define MAX_GROUP 128 // query heads of a kv head
+
 struct AttnOpArgs {
     KvView own;    // slots of the row's own sequence, causal
     KvView prefix; // k null: none; else one sequence, visible to every row
     RowsView r;
     uint32_t window, sinks; // window 0: unlimited
+    // Key ranges: own_splits of the own slots, then prefix_splits of the prefix.  Where
+    // there is more than one in all, range s of row r, head h writes its softmax state to
+    // ml[(s * n_rows + r) * heads + h] = {log2 offset, sum} and its unnormalized output
+    // beside it in o, and k_attn_merge joins them.
+    uint32_t own_splits, prefix_splits;
+    uint32_t prefix_groups, own_groups; // row groups: of the whole batch, of one token
+    float2 *ml;
+    float *o;
+    // scored: scores[(b * heads + h) * slots + j], in units of q . k
+    float *scores;
+    const float *acc; // nullable
+    float *acc_out;   // [n_seq][kv_heads][slots]
 };
 
 struct ColsumArgs { // acc_out = acc_in + the rows' attention weights

@@ -27,6 +27,7 @@
 struct AttnKernels {
     hipModule_t mod = nullptr;
     hipFunction_t attn_simple[3][2], colsum_simple[3][2];
+    hipFunction_t step_1w4[3][2], step_wide[3][2], step_most[3][2], merge[3][2], scored_join[3][2];
     hipFunction_t kv_select, kv_move;
 };
 
@@ -50,9 +51,19 @@ static int load_attn(int dev)
     for (int t = 0; t < 3 && rc == LFM_OK; ++t)
         for (int d = 0; d < 2 && rc == LFM_OK; ++d) {
             const std::string tag = std::string("_") + types[t] + (d ? "_128" : "_64");
-            rc = get(&k.attn_simple[t][d], "k_attn_simple" + tag);
-            if (rc == LFM_OK)
-                rc = get(&k.colsum_simple[t][d], "k_colsum_simple" + tag);
+            struct {
+                hipFunction_t *f;
+                std::string name;
+            } fns[] = {{&k.attn_simple[t][d], "k_attn_simple" + tag},
+                       {&k.colsum_simple[t][d], "k_colsum_simple" + tag},
+                       {&k.step_1w4[t][d], "k_attn_step" + tag + "_r1w4"},
+                       {&k.step_wide[t][d], "k_attn_step" + tag + (d ? "_r1w8" : "_r1w16")},
+                       {&k.step_most[t][d], "k_attn_step" + tag + (d ? "_r2w4" : "_r4w4")},
+                       {&k.merge[t][d], "k_attn_merge" + tag},
+                       {&k.scored_join[t][d], "k_scored_join" + tag}};
+            for (auto &f : fns)
+                if (rc == LFM_OK)
+                    rc = get(f.f, f.name);
         }
     if (rc == LFM_OK)
         rc = get(&k.kv_select, "k_kv_select");
@@ -119,11 +130,11 @@ static int check_rows(const char *op, const lfm_kv *c, const lfm_rows *r)
     if (r->type > LFM_TYPE_BF16 || (r->type == LFM_TYPE_BF16) != (c->type == LFM_TYPE_BF16))
         return fail(LFM_EINVAL, "%s: rows of type %u over a cache of type %u (F32 or F16 over F16, BF16 over BF16)",
                     op, r->type, c->type);
-    if (r->heads == 0 || r->heads % c->kv_heads || r->heads > 65535)
-        return fail(LFM_EINVAL, "%s: %u heads over %u kv heads (a multiple, at most 65535)", op, r->heads,
-                    c->kv_heads);
-    if (r->n_rows > 0x7FFFFFFFu)
-        return fail(LFM_EINVAL, "%s: %u rows", op, r->n_rows);
+    if (r->heads == 0 || r->heads % c->kv_heads || r->heads / c->kv_heads > MAX_GROUP || r->heads > 65535)
+        return fail(LFM_EINVAL, "%s: %u heads over %u kv heads (a multiple, at most %u times)", op, r->heads,
+                    c->kv_heads, MAX_GROUP);
+    if ((uint64_t)r->n_rows * r->heads > 0x7FFFFFFFu)
+        return fail(LFM_EINVAL, "%s: %u rows of %u heads (2^31 - 1 of them at most)", op, r->n_rows, r->heads);
     if (!r->start && r->n_rows != c->n_seq)
         return fail(LFM_EINVAL, "%s: %u rows for %u sequences without start (one row each)", op, r->n_rows, c->n_seq);
     if (!(r->scale > 0.f) || !(r->scale < INFINITY))
@@ -230,19 +241,101 @@ static RowsView view(const lfm_rows *r)
 static int dim_index(const lfm_kv *c) { return c->head_dim == 128; }
 
 // ------------------------------------------------------------------ attention
-static int attend(const char *op, const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *rows, uint32_t window,
-                  uint32_t sinks, float *lse, hipStream_t s, int dev)
+// How a call's work is cut, from sizes alone.
+struct Plan {
+    uint32_t own_splits = 1, prefix_splits = 0, own_groups = 1, prefix_groups = 0;
+    bool many_waves = false, most = false; // the step kernel's form
+    bool join = false;                     // a second kernel joins the key ranges
+    size_t ml_bytes = 0, o_bytes = 0, score_bytes = 0;
+    size_t bytes() const { return ml_bytes + o_bytes + score_bytes; }
+};
+
+static size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+#define TARGET_WAVES 4096 // four to each of 1024 SIMDs
+
+static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint32_t window, uint32_t sinks, bool scored)
 {
-    AttnKernels *K;
-    RC(attn_kernels(dev, &K));
+    Plan p;
+    const uint32_t G = r->heads / kv->kv_heads, most = kv->head_dim == 64 ? 64 : 32;
+    const uint64_t span = window ? std::min<uint64_t>(kv->slots, (uint64_t)window + sinks + 63) : kv->slots;
+    const uint64_t blocks = (span + 31) / 32;
+    const uint64_t pairs = (uint64_t)r->n_rows * r->heads;
+    p.most = prefix ? (uint64_t)r->n_rows * G > 16 : G > 16;
+    const uint32_t per = p.most ? most : 16;
+    p.own_groups = (G + per - 1) / per;
+    const uint64_t items = (uint64_t)std::max(1u, r->n_rows) * p.own_groups * kv->kv_heads;
+    // a wave needs a few blocks for its loads to overlap; below that ranges only add joining
+    p.own_splits = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, TARGET_WAVES / 4 / items),
+                                                std::max<uint64_t>(1, blocks / 16));
+    if (!prefix && !p.most && blocks <= 64 && items < 1024) {
+        p.own_splits = 1;
+        p.many_waves = blocks > 4;
+    }
+    if (prefix) {
+        p.prefix_groups = (uint32_t)(((uint64_t)r->n_rows * G + per - 1) / per);
+        const uint64_t pitems = (uint64_t)std::max(1u, p.prefix_groups) * kv->kv_heads;
+        p.prefix_splits = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, TARGET_WAVES / 4 / pitems),
+                                                       std::max<uint64_t>(1, (prefix->slots + 511) / 512));
+    }
+    const uint32_t splits = p.own_splits + p.prefix_splits;
+    p.join = scored || splits > 1;
+    if (p.join) {
+        p.ml_bytes = round256((size_t)splits * pairs * 8);
+        p.o_bytes = round256((size_t)splits * pairs * kv->head_dim * 4);
+    }
+    if (scored)
+        p.score_bytes = round256((size_t)pairs * kv->slots * 4);
+    return p;
+}
+
+static AttnOpArgs op_args(const Plan &p, const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *rows, uint32_t window,
+                          uint32_t sinks, void *ws)
+{
     AttnOpArgs a;
     memset(&a, 0, sizeof(a));
     a.own = view(kv);
     if (prefix)
         a.prefix = view(prefix);
     a.r = view(rows);
-    a.r.lse = lse;
     a.window = window, a.sinks = sinks;
+    a.own_splits = p.own_splits, a.prefix_splits = p.prefix_splits;
+    a.own_groups = p.own_groups, a.prefix_groups = p.prefix_groups;
+    uint8_t *w = (uint8_t *)ws;
+    a.ml = (float2 *)w;
+    a.o = (float *)(w + p.ml_bytes);
+    a.scores = p.score_bytes ? (float *)(w + p.ml_bytes + p.o_bytes) : nullptr;
+    return a;
+}
+
+// Single rows: one launch over (kv head, row group and key range), one that joins.
+static int attend_step(AttnKernels *K, const Plan &p, const AttnOpArgs &a, const lfm_kv *kv, const lfm_rows *rows,
+                       hipStream_t s)
+{
+    const int t = rows->type, d = dim_index(kv);
+    const uint64_t items = (uint64_t)p.prefix_groups * p.prefix_splits +
+                           (uint64_t)rows->n_rows * p.own_groups * p.own_splits;
+    if (items * kv->kv_heads > 0x7FFFFFFFull)
+        return fail(LFM_EINVAL, "attention: %llu work items", (unsigned long long)items);
+    hipFunction_t f = p.most ? K->step_most[t][d] : p.many_waves ? K->step_wide[t][d] : K->step_1w4[t][d];
+    RC(launch(f, dim3((uint32_t)items * kv->kv_heads), p.many_waves ? (d ? 512 : 1024) : 256, s, a));
+    if (a.scores)
+        return launch(K->scored_join[t][d], dim3((kv->slots + 511) / 512, kv->kv_heads, kv->n_seq), 256, s, a);
+    if (p.join)
+        return launch(K->merge[t][d], dim3((rows->n_rows * rows->heads + 3) / 4), 256, s, a);
+    return LFM_OK;
+}
+
+static int attend(const char *op, const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *rows, uint32_t window,
+                  uint32_t sinks, float *lse, void *ws, hipStream_t s, int dev)
+{
+    AttnKernels *K;
+    RC(attn_kernels(dev, &K));
+    const Plan p = plan(prefix, kv, rows, window, sinks, false);
+    AttnOpArgs a = op_args(p, prefix, kv, rows, window, sinks, ws);
+    a.r.lse = lse;
+    if (!rows->start)
+        return attend_step(K, p, a, kv, rows, s);
     return launch(K->attn_simple[rows->type][dim_index(kv)], dim3(rows->n_rows, rows->heads), 64, s, a);
 }
 
@@ -250,12 +343,11 @@ extern "C" int lfm_attn_window_workspace(const lfm_kv *kv, const lfm_rows *rows,
                                          size_t *bytes)
 {
     const char *op = "lfm_attn_window_workspace";
-    (void)window, (void)sinks;
     RC(check_kv(op, "kv", kv));
     RC(check_rows(op, kv, rows));
     if (!bytes)
         return fail(LFM_EINVAL, "%s: bytes is null", op);
-    *bytes = 0;
+    *bytes = plan(nullptr, kv, rows, window, sinks, false).bytes();
     return LFM_OK;
 }
 
@@ -272,7 +364,7 @@ extern "C" int lfm_attn_window(const lfm_kv *kv, const lfm_rows *rows, uint32_t 
     RC(check_kv_ptrs(op, KV_NAMES, kv, dev));
     RC(check_rows_ptrs(op, rows, dev));
     RC(check_workspace(op, workspace, workspace_bytes, need, dev));
-    return attend(op, nullptr, kv, rows, window, sinks, rows->lse, (hipStream_t)stream, dev);
+    return attend(op, nullptr, kv, rows, window, sinks, rows->lse, workspace, (hipStream_t)stream, dev);
 }
 
 extern "C" int lfm_attn_scored_workspace(const lfm_kv *kv, const lfm_rows *rows, size_t *bytes)
@@ -282,7 +374,10 @@ extern "C" int lfm_attn_scored_workspace(const lfm_kv *kv, const lfm_rows *rows,
     RC(check_rows(op, kv, rows));
     if (!bytes)
         return fail(LFM_EINVAL, "%s: bytes is null", op);
-    *bytes = ((size_t)rows->n_rows * rows->heads * 4 + 255) / 256 * 256; // lse, where the caller wants none
+    if (!rows->start)
+        *bytes = plan(nullptr, kv, rows, 0, 0, true).bytes();
+    else // lse, where the caller wants none
+        *bytes = round256((size_t)rows->n_rows * rows->heads * 4) + plan(nullptr, kv, rows, 0, 0, false).bytes();
     return LFM_OK;
 }
 
@@ -304,11 +399,18 @@ extern "C" int lfm_attn_scored(const lfm_kv *kv, const lfm_rows *rows, const flo
     RC(check_ptr(op, "acc_out", acc_out, 4, dev));
     RC(check_workspace(op, workspace, workspace_bytes, need, dev));
     hipStream_t s = (hipStream_t)stream;
-    float *lse = rows->lse ? rows->lse : (float *)workspace;
-    if (rows->n_rows)
-        RC(attend(op, nullptr, kv, rows, 0, 0, lse, s, dev));
     AttnKernels *K;
     RC(attn_kernels(dev, &K));
+    if (!rows->start) {
+        const Plan p = plan(nullptr, kv, rows, 0, 0, true);
+        AttnOpArgs a = op_args(p, nullptr, kv, rows, 0, 0, workspace);
+        a.acc = acc_in, a.acc_out = acc_out;
+        return attend_step(K, p, a, kv, rows, s);
+    }
+    float *lse = rows->lse ? rows->lse : (float *)workspace;
+    if (rows->n_rows)
+        RC(attend(op, nullptr, kv, rows, 0, 0, lse,
+                  (uint8_t *)workspace + round256((size_t)rows->n_rows * rows->heads * 4), s, dev));
     ColsumArgs a;
     memset(&a, 0, sizeof(a));
     a.own = view(kv);
@@ -337,7 +439,7 @@ extern "C" int lfm_attn_prefix_workspace(const lfm_kv *prefix, const lfm_kv *kv,
     RC(check_rows(op, kv, rows));
     if (!bytes)
         return fail(LFM_EINVAL, "%s: bytes is null", op);
-    *bytes = 0;
+    *bytes = plan(prefix, kv, rows, 0, 0, false).bytes();
     return LFM_OK;
 }
 
@@ -355,7 +457,7 @@ extern "C" int lfm_attn_prefix(const lfm_kv *prefix, const lfm_kv *kv, const lfm
     RC(check_kv_ptrs(op, KV_NAMES, kv, dev));
     RC(check_rows_ptrs(op, rows, dev));
     RC(check_workspace(op, workspace, workspace_bytes, need, dev));
-    return attend(op, prefix, kv, rows, 0, 0, rows->lse, (hipStream_t)stream, dev);
+    return attend(op, prefix, kv, rows, 0, 0, rows->lse, workspace, (hipStream_t)stream, dev);
 }
 
 // ------------------------------------------------------------------ eviction

@@ -7,15 +7,70 @@
 #include "attn_args.h"
 #include "wave_ops.h"
 
-struct F32 {
-    typedef float type;
-};
+// ------------------------------------------------------------------ types
+// Queries and weights meet K and V on the 16x16x32 matrix instruction: lane l holds 8
+// numbers of row (A) or column (B) l % 16, at inner places 8 (l / 16) + i, and 4 results,
+// rows 4 (l / 16) + e of column l % 16.
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef short short8v __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) short4v lds_short4;
+
 struct F16 {
-    typedef _Float16 type;
+    typedef _Float16 type, kv;
+    typedef f16x8 vec;
+    static constexpr int parts = 1;
+    // Weights are 2^10 times their value relative to the largest, so that binary16's
+    // subnormals start 24 binary orders below it and not 14.
+    static constexpr float offset = 10.f;
+};
+struct F32 { // rows of 32 bits over a binary16 cache: two binary16 numbers each, 22 bits
+    typedef float type;
+    typedef _Float16 kv;
+    typedef f16x8 vec;
+    static constexpr int parts = 2;
+    static constexpr float offset = 10.f;
 };
 struct BF16 {
-    typedef __bf16 type;
+    typedef __bf16 type, kv;
+    typedef bf16x8 vec;
+    static constexpr int parts = 1;
+    static constexpr float offset = 0.f; // the exponent has 8 bits
 };
+
+__device__ __forceinline__ floatx4 mma(f16x8 a, f16x8 b, floatx4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx4 mma(bf16x8 a, bf16x8 b, floatx4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Largest and sum of a value over the lanes l, l ^ 16, l ^ 32, l ^ 48 (one query row).
+__device__ __forceinline__ float quarter_other(float v)
+{
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    return (threadIdx.x & 16) ? __builtin_bit_cast(float, lo) : __builtin_bit_cast(float, hi);
+}
+__device__ __forceinline__ float row_max(float v)
+{
+    v = fmaxf(v, quarter_other(v));
+    const float2v h = wave_halves(v);
+    return fmaxf(h[0], h[1]);
+}
+__device__ __forceinline__ float row_sum(float v)
+{
+    v += quarter_other(v);
+    const float2v h = wave_halves(v);
+    return h[0] + h[1];
+}
 
 __device__ __forceinline__ int32_t clamp_len(const KvView &c, uint32_t b)
 {
@@ -54,12 +109,487 @@ __device__ __forceinline__ bool find_row(const AttnOpArgs &a, uint32_t row, uint
     return false;
 }
 
+// Four outputs of a row and head, rounded to the rows' type.
+template <typename TQ>
+__device__ __forceinline__ void store_out(const RowsView &r, uint32_t row, uint32_t h, uint32_t d, floatx4 v)
+{
+    typedef typename TQ::type tq;
+    typedef tq tq4 __attribute__((ext_vector_type(4)));
+    *(tq4 *)((tq *)r.out + (int64_t)row * r.o_rs + (int64_t)h * r.o_hs + d) = __builtin_convertvector(v, tq4);
+}
+
+// ------------------------------------------------------------------ rows in matrix form
+// Query rows of one lane (its row of RT tiles of 16) as B operands, and cexp / the power of
+// two that an F32 row was multiplied by so that its largest value lies in binary16's range.
+template <typename TQ, int D, int RT> struct Queries {
+    typename TQ::vec q[RT][TQ::parts][D / 32];
+    float c[TQ::parts == 2 ? RT : 1];
+    float back[TQ::parts == 2 ? RT : 1]; // the inverse of that power
+};
+
+template <typename TQ, int D, int RT>
+__device__ __forceinline__ void load_row(Queries<TQ, D, RT> &Q, int t, const RowsView &r, bool valid, uint32_t row,
+                                         uint32_t h)
+{
+    typedef typename TQ::type tq;
+    const uint32_t g = (threadIdx.x & 63) >> 4;
+    const tq *p = (const tq *)r.q + (int64_t)row * r.q_rs + (int64_t)h * r.q_hs + 8 * g;
+    if constexpr (TQ::parts == 1) {
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+            typename TQ::vec v = {};
+            if (valid)
+                v = *(const typename TQ::vec *)(p + 32 * j);
+            Q.q[t][0][j] = v;
+        }
+        Q.c[0] = r.cexp;
+    } else {
+        float x[D / 32][8], top = 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+            floatx4 a = {}, b = {};
+            if (valid) {
+                a = *(const floatx4 *)(p + 32 * j);
+                b = *(const floatx4 *)(p + 32 * j + 4);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[j][i] = a[i], x[j][4 + i] = b[i];
+                top = fmaxf(top, fmaxf(fabsf(a[i]), fabsf(b[i])));
+            }
+        }
+        top = row_max(top);
+        int ex = 14;
+        if (top > 0.f && top < INFINITY)
+            frexpf(top, &ex);
+        const int up = min(14 - ex, 126);
+        const float s = ldexpf(1.f, up);
+        Q.back[t] = ldexpf(1.f, -up);
+        Q.c[t] = r.cexp * Q.back[t];
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = x[j][i] * s;
+                const _Float16 hi = (_Float16)y;
+                Q.q[t][0][j][i] = hi;
+                Q.q[t][1][j][i] = (_Float16)(y - (float)hi);
+            }
+    }
+}
+
+// ------------------------------------------------------------------ softmax state
+// Of RT tiles of 16 rows: o[t][n] are dims 16 n + 4 (lane / 16) + e of row lane % 16.  m is
+// the largest score so far (units of q . k), mc = m c - offset; l the lane's own part of the
+// sum of the weights 2^(s c - mc), whose four parts are added at the end.
+template <typename TQ, int D, int RT> struct State {
+    floatx4 o[RT][D / 16];
+    float m[RT], mc[RT], l[RT];
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n)
+                o[t][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+            m[t] = -INFINITY, mc[t] = 0.f, l[t] = 0.f;
+        }
+    }
+};
+
+// Scores of 32 keys (s[0]: keys 4 (lane / 16) + e, s[1]: the same + 16) -> weights as a B
+// operand: inner place 8 (lane / 16) + i is key 16 (i / 4) + 4 (lane / 16) + i % 4.  The
+// rescaling of o is skipped where no row's maximum rose.
+template <typename TQ, int D, int RT>
+__device__ __forceinline__ void weigh(State<TQ, D, RT> &S, int t, const floatx4 (&s)[2], float c,
+                                      typename TQ::vec (&p)[TQ::parts])
+{
+    float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+    top = fmaxf(top, fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    if (__ballot(top > S.m[t])) {
+        const float mn = fmaxf(S.m[t], row_max(top));
+        // a row of -inf alone keeps offset 0: its weights are 2^-inf = 0
+        const float mcn = mn > -INFINITY ? mn * c - TQ::offset : 0.f;
+        const float r = S.m[t] > -INFINITY ? exp2_hw(S.mc[t] - mcn) : 0.f;
+        S.m[t] = mn, S.mc[t] = mcn, S.l[t] *= r;
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n)
+            S.o[t][n] *= r;
+    }
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        w[i] = exp2_hw(fmaf(s[i / 4][i % 4], c, -S.mc[t]));
+    }
+    S.l[t] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const auto hi = (typename TQ::kv)w[i];
+        p[0][i] = hi;
+        if constexpr (TQ::parts == 2)
+            p[1][i] = (_Float16)(w[i] - (float)hi);
+    }
+}
+
+// ------------------------------------------------------------------ V in shared memory
+// 32 rows of D, each row's 16-byte pieces in the order piece ^ (row % pieces), so that the
+// 16 rows that a transposed read touches lie in different banks.
+template <int D> __device__ __forceinline__ uint32_t v_piece(uint32_t row, uint32_t piece)
+{
+    return row * (D / 8) + (piece ^ (row & (D / 8 - 1)));
+}
+
+// The lane's address for transposed_read: row 4 (lane / 16) + (lane % 16) / 4, dims 4 (lane % 4).
+template <int D> __device__ __forceinline__ uint32_t v_lane(uint32_t lane)
+{
+    const uint32_t row = 4 * (lane >> 4) + ((lane & 15) >> 2);
+    return v_piece<D>(row, (lane & 3) >> 1) * 16 + (lane & 1) * 8;
+}
+
+// V^T of dims 16 n .. 16 n + 15 as an A operand in the order of weigh(): two transposed
+// reads, each giving the lane dim 16 n + lane % 16 of four rows.
+template <typename TQ, int D>
+__device__ __forceinline__ typename TQ::vec v_operand(const uint8_t *tile, uint32_t at, int n)
+{
+    const uint8_t *p = tile + (at ^ (uint32_t)(n << 5));
+    const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)p);
+    const short4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(p + 16 * D * 2));
+    const short8v v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    return __builtin_bit_cast(typename TQ::vec, v);
+}
+
+// ------------------------------------------------------------------ visible blocks
+// Blocks of 32 slots that a row at hi - 1 sees: those of the first tokens, then those of
+// the window (all in one run where the two meet).
+struct Blocks {
+    uint32_t hi, wlo, sinks; // slot j is seen: j < hi and (j < sinks or j >= wlo)
+    uint32_t first, skip, count;
+    __device__ __forceinline__ void set(int32_t pos, uint32_t window, uint32_t s)
+    {
+        hi = (uint32_t)max(pos + 1, 0);
+        wlo = window && window < hi ? hi - window : 0;
+        if (s >= wlo)
+            wlo = 0;
+        sinks = wlo ? s : 0;
+        first = (sinks + 31) / 32;
+        const uint32_t from = max(wlo / 32, first);
+        skip = from - first;
+        count = (hi + 31) / 32 - skip;
+    }
+    __device__ __forceinline__ uint32_t block(uint32_t i) const { return i < first ? i : i + skip; }
+    __device__ __forceinline__ bool whole(uint32_t blk) const
+    {
+        const uint32_t j = blk * 32;
+        return j + 32 <= hi && (j + 32 <= sinks || j >= wlo);
+    }
+    __device__ __forceinline__ bool seen(uint32_t j) const { return j < hi && (j < sinks || j >= wlo); }
+};
+
+// A key range's share [lo, hi) of n blocks.
+__device__ __forceinline__ void share(uint32_t n, uint32_t part, uint32_t parts, uint32_t *lo, uint32_t *hi)
+{
+    *lo = (uint32_t)((uint64_t)n * part / parts);
+    *hi = (uint32_t)((uint64_t)n * (part + 1) / parts);
+}
+
+// ------------------------------------------------------------------ rows that see the same slots
+// One workgroup: up to 16 RT (row, head) pairs of one kv head that see the same slots (a
+// token's query heads, or any rows over the prefix), over one key range.  Its waves take
+// blocks of 32 slots in turn, each with a softmax state of its own, joined at the end: a
+// wave streams K straight into A operands and V through a piece of shared memory of its own
+// (the transposed read), the next block's loads in flight, and no wave waits for another.
+template <typename TQ, int D, int RT, int NW> __device__ __forceinline__ void attn_step(const AttnOpArgs &a)
+{
+    typedef typename TQ::vec vec;
+    constexpr int VL = D / 16;                   // 16-byte loads of V a lane and block
+    constexpr uint32_t ROWS = 16 * RT, PIECES = D / 8;
+    constexpr uint32_t V_BYTES = 32 * D * 2, O_BYTES = ROWS * D * 4;
+    constexpr uint32_t SMEM = NW * (V_BYTES > O_BYTES ? V_BYTES : O_BYTES);
+    __shared__ __attribute__((aligned(16))) uint8_t smem[SMEM];
+    __shared__ float2 sml[NW][ROWS];
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4;
+    const uint32_t kh = blockIdx.x % a.own.kv_heads, G = a.r.heads / a.own.kv_heads;
+    uint32_t item = blockIdx.x / a.own.kv_heads;
+    const uint32_t prefix_items = a.prefix_groups * a.prefix_splits;
+    const bool pre = item < prefix_items;
+    // rows: pair i of the group is (row0 + (i0 + i) / G, head kh G + (i0 + i) % G)
+    uint32_t group, part, parts, row0, total;
+    const uint16_t *kp, *vp;
+    int64_t ts;
+    Blocks bl;
+    if (pre) {
+        group = item % a.prefix_groups, part = item / a.prefix_groups, parts = a.prefix_splits;
+        row0 = 0, total = a.r.n_rows * G;
+        bl.set(clamp_len(a.prefix, 0) - 1, 0, 0);
+        const int64_t at = (int64_t)kh * a.prefix.hs;
+        kp = a.prefix.k + at, vp = a.prefix.v + at, ts = a.prefix.ts;
+    } else {
+        item -= prefix_items;
+        group = item % a.own_groups, item /= a.own_groups;
+        part = item % a.own_splits, parts = a.own_splits;
+        row0 = item / a.own_splits, total = G;
+        bl.set(clamp_len(a.own, row0) - 1, a.window, a.sinks);
+        const int64_t at = (int64_t)row0 * a.own.ss + (int64_t)kh * a.own.hs;
+        kp = a.own.k + at, vp = a.own.v + at, ts = a.own.ts;
+    }
+    const uint32_t i0 = group * ROWS;
+    uint32_t b0, b1;
+    share(bl.count, part, parts, &b0, &b1);
+    const uint32_t tiles = (min(ROWS, total - i0) + 15) / 16;
+
+    Queries<TQ, D, RT> Q;
+    State<TQ, D, RT> S;
+    S.clear();
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const uint32_t i = i0 + 16 * t + (lane & 15);
+        load_row<TQ, D, RT>(Q, t, a.r, i < total, row0 + i / G, kh * G + i % G);
+    }
+    uint8_t *const vt = smem + wave * V_BYTES;
+    const uint32_t at = v_lane<D>(lane);
+    vec kr[2][D / 32];
+    uint4 vr[VL];
+    auto load = [&](uint32_t blk) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const uint32_t j = min(blk * 32 + 16 * u + (lane & 15), bl.hi - 1);
+            const uint16_t *p = kp + (int64_t)j * ts + 8 * g;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+                kr[u][i] = *(const vec *)(p + 32 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < VL; ++i) {
+            const uint32_t j = min(blk * 32 + (i * 64 + lane) / PIECES, bl.hi - 1);
+            vr[i] = *(const uint4 *)(vp + (int64_t)j * ts + (lane % PIECES) * 8);
+        }
+    };
+    uint32_t b = b0 + wave;
+    if (b < b1)
+        load(bl.block(b));
+    for (; b < b1; b += NW) {
+        const uint32_t blk = bl.block(b);
+        const bool whole = bl.whole(blk);
+        // V to shared memory; slots that are not seen become zeros, whatever they hold
+#pragma unroll
+        for (int i = 0; i < VL; ++i) {
+            const uint32_t row = (i * 64 + lane) / PIECES;
+            if (!whole && !bl.seen(blk * 32 + row))
+                vr[i] = make_uint4(0, 0, 0, 0);
+            *(uint4 *)(vt + v_piece<D>(row, lane % PIECES) * 16) = vr[i];
+        }
+        floatx4 s[RT][2];
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+            if (t < (int)tiles) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    s[t][u] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                        for (int x = 0; x < TQ::parts; ++x)
+                            s[t][u] = mma(kr[u][i], Q.q[t][x][i], s[t][u]);
+                }
+            }
+        if (b + NW < b1)
+            load(bl.block(b + NW));
+        if (a.scores && !pre) { // uniform
+            const uint32_t i = i0 + (lane & 15);
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+                if (i + 16 * t < total)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t j = blk * 32 + 16 * u + 4 * g;
+                        float *to = a.scores + ((size_t)row0 * a.r.heads + kh * G + i + 16 * t) * a.own.slots + j;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (j + e < bl.hi) {
+                                if constexpr (TQ::parts == 2)
+                                    to[e] = s[t][u][e] * Q.back[t];
+                                else
+                                    to[e] = s[t][u][e];
+                            }
+                    }
+        }
+        if (!whole) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (!bl.seen(blk * 32 + 16 * u + 4 * g + e))
+#pragma unroll
+                        for (int t = 0; t < RT; ++t)
+                            s[t][u][e] = -INFINITY;
+        }
+        vec p[RT][TQ::parts];
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+            if (t < (int)tiles)
+                weigh<TQ, D, RT>(S, t, s[t], Q.c[TQ::parts == 2 ? t : 0], p[t]);
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+            const vec v = v_operand<TQ, D>(vt, at, n);
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+                if (t < (int)tiles)
+#pragma unroll
+                    for (int x = 0; x < TQ::parts; ++x)
+                        S.o[t][n] = mma(v, p[t][x], S.o[t][n]);
+        }
+    }
+    // join the waves: offsets and sums first, then the outputs at the common offset
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        S.l[t] = row_sum(S.l[t]);
+        if (lane < 16)
+            sml[wave][16 * t + lane] = make_float2(S.m[t] > -INFINITY ? S.mc[t] : -INFINITY, S.l[t]);
+    }
+    __syncthreads();
+    float *const so = (float *)smem; // [wave][row][D]
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        float top = -INFINITY;
+        for (int w = 0; w < NW; ++w)
+            top = fmaxf(top, sml[w][16 * t + (lane & 15)].x);
+        const float f = S.m[t] > -INFINITY ? exp2_hw(S.mc[t] - top) : 0.f;
+        float *to = so + ((size_t)wave * ROWS + 16 * t + (lane & 15)) * D + 4 * g;
+        if (i0 + 16 * t + (lane & 15) < total)
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n)
+                *(floatx4 *)(to + 16 * n) = S.o[t][n] * f;
+    }
+    __syncthreads();
+    const bool final = !a.scores && a.own_splits + a.prefix_splits == 1;
+    constexpr uint32_t QD = D / 4;
+    for (uint32_t x = tid; x < min(ROWS, total - i0) * QD; x += NW * 64) {
+        const uint32_t i = x / QD, d = (x % QD) * 4;
+        float top = -INFINITY, l = 0.f;
+        for (int w = 0; w < NW; ++w)
+            top = fmaxf(top, sml[w][i].x);
+        floatx4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < NW; ++w) {
+            const float2 e = sml[w][i];
+            l += e.x > -INFINITY ? e.y * exp2_hw(e.x - top) : e.y;
+            o += *(const floatx4 *)(so + ((size_t)w * ROWS + i) * D + d);
+        }
+        const uint32_t row = row0 + (i0 + i) / G, h = kh * G + (i0 + i) % G;
+        if (final) {
+            const bool empty = bl.hi == 0;
+            store_out<TQ>(a.r, row, h, d, empty ? o : o / l);
+            if (d == 0 && a.r.lse)
+                a.r.lse[(size_t)row * a.r.heads + h] = empty ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+        } else {
+            const size_t at2 = ((size_t)(pre ? a.own_splits + part : part) * a.r.n_rows + row) * a.r.heads + h;
+            *(floatx4 *)(a.o + at2 * D + d) = o;
+            if (d == 0)
+                a.ml[at2] = make_float2(top, l);
+        }
+    }
+}
+
+// Joins the key ranges of a row and head: a wave each.
+template <typename TQ, int D> __device__ __forceinline__ void attn_merge(const AttnOpArgs &a)
+{
+    const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t pairs = a.r.n_rows * a.r.heads;
+    if (id >= pairs)
+        return;
+    const uint32_t row = id / a.r.heads, h = id % a.r.heads, n = a.own_splits + a.prefix_splits;
+    uint32_t b;
+    int32_t pos;
+    if (!find_row(a, row, &b, &pos))
+        return;
+    float top = -INFINITY;
+    for (uint32_t s = lane; s < n; s += 64)
+        top = fmaxf(top, a.ml[(size_t)s * pairs + id].x);
+    top = wave_max(top);
+    constexpr int E = D / 64;
+    float l = 0.f, o[E] = {};
+    for (uint32_t s = 0; s < n; ++s) {
+        const float2 e = a.ml[(size_t)s * pairs + id];
+        const float f = e.x > -INFINITY ? exp2_hw(e.x - top) : 0.f;
+        // a range without a number adds its sum (0, or NaN from its scores) as it is
+        l += e.x > -INFINITY ? e.y * f : e.y;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float x = a.o[((size_t)s * pairs + id) * D + lane * E + i];
+            o[i] += e.x > -INFINITY ? x * f : 0.f;
+        }
+    }
+    const bool empty = pos < 0 && (!a.prefix.k || clamp_len(a.prefix, 0) == 0);
+    typedef typename TQ::type tq;
+    tq *to = (tq *)a.r.out + (int64_t)row * a.r.o_rs + (int64_t)h * a.r.o_hs + lane * E;
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        to[i] = (tq)(empty ? 0.f : o[i] / l);
+    if (a.r.lse && lane == 0)
+        a.r.lse[id] = empty ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+}
+
+#define SCORED_SLOTS 512
+// After a scored step: joins the key ranges of one (sequence, kv head) and adds every
+// slot's weights, SCORED_SLOTS slots a workgroup.  Scores were kept as they left the
+// matrix cores, so a weight is one exponential here: 16 bytes a slot and kv head at four
+// query heads, where reading K again would be 128 or 256.
+template <typename TQ, int D> __device__ __forceinline__ void scored_join(const AttnOpArgs &a)
+{
+    const uint32_t chunk = blockIdx.x, kh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, wave = tid >> 6,
+                   lane = tid & 63;
+    const uint32_t G = a.r.heads / a.own.kv_heads, n = (uint32_t)clamp_len(a.own, b), pairs = a.r.n_rows * a.r.heads;
+    if (chunk && chunk * SCORED_SLOTS >= n)
+        return;
+    __shared__ float2 st[MAX_GROUP]; // offset and 1 / sum
+    for (uint32_t g = wave; g < G; g += 4) {
+        const uint32_t id = b * a.r.heads + kh * G + g;
+        float top = -INFINITY;
+        for (uint32_t s = lane; s < a.own_splits; s += 64)
+            top = fmaxf(top, a.ml[(size_t)s * pairs + id].x);
+        top = wave_max(top);
+        float l = 0.f;
+        for (uint32_t s = 0; s < a.own_splits; ++s) { // in order: the sum every other form of it has
+            const float2 e = a.ml[(size_t)s * pairs + id];
+            l += e.x > -INFINITY ? e.y * exp2_hw(e.x - top) : e.y;
+        }
+        if (lane == 0)
+            st[g] = make_float2(top, 1.0f / l);
+        if (chunk == 0) {
+            constexpr int E = D / 64;
+            float o[E] = {};
+            for (uint32_t s = 0; s < a.own_splits; ++s) {
+                const float x = a.ml[(size_t)s * pairs + id].x;
+                const float f = x > -INFINITY ? exp2_hw(x - top) : 0.f;
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    o[i] += x > -INFINITY ? f * a.o[((size_t)s * pairs + id) * D + lane * E + i] : 0.f;
+            }
+            typedef typename TQ::type tq;
+            tq *to = (tq *)a.r.out + (int64_t)b * a.r.o_rs + (int64_t)(kh * G + g) * a.r.o_hs + lane * E;
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                to[i] = (tq)(n == 0 ? 0.f : o[i] / l);
+            if (a.r.lse && lane == 0)
+                a.r.lse[id] = n == 0 ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+        }
+    }
+    __syncthreads();
+    for (uint32_t j = chunk * SCORED_SLOTS + tid; j < min(n, (chunk + 1) * SCORED_SLOTS); j += 256) {
+        const float *s = a.scores + ((size_t)b * a.r.heads + kh * G) * a.own.slots + j;
+        float sum = 0.f;
+        for (uint32_t g = 0; g < G; ++g)
+            sum += exp2_hw(fmaf(s[(size_t)g * a.own.slots], a.r.cexp, -st[g].x)) * st[g].y;
+        const size_t at = ((size_t)b * a.own.kv_heads + kh) * a.own.slots + j;
+        a.acc_out[at] = (a.acc ? a.acc[at] : 0.f) + sum;
+    }
+}
+
 // One wave per row and head: 64 slots at a time, a lane's score each, then every lane its
 // dims of the weighted sum.
 template <typename TQ, typename TK, int D> __device__ void attn_simple(const AttnOpArgs &a)
 {
     typedef typename TQ::type tq;
-    typedef typename TK::type tk;
+    typedef typename TK::kv tk;
     const uint32_t row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, kh = h / (a.r.heads / a.own.kv_heads);
     uint32_t b;
     int32_t pos;
@@ -122,7 +652,7 @@ template <typename TQ, typename TK, int D> __device__ void attn_simple(const Att
 template <typename TQ, typename TK, int D> __device__ void colsum_simple(const ColsumArgs &a)
 {
     typedef typename TQ::type tq;
-    typedef typename TK::type tk;
+    typedef typename TK::kv tk;
     const uint32_t kh = blockIdx.y, b = blockIdx.z, G = a.r.heads / a.own.kv_heads;
     const int32_t n = clamp_len(a.own, b), j = (int32_t)(blockIdx.x * 64 + threadIdx.x);
     if (j >= n)
@@ -146,6 +676,33 @@ template <typename TQ, typename TK, int D> __device__ void colsum_simple(const C
     const size_t at = ((size_t)b * a.own.kv_heads + kh) * a.own.slots + j;
     a.acc_out[at] = (a.acc ? a.acc[at] : 0.f) + sum;
 }
+
+// RT: row tiles of a workgroup of rows that see the same slots, as many as the registers
+// hold beside the next block's K and V.
+#define STEP(TQ, tag, D, RT, NW)                                                                               \
+    extern "C" __global__ __launch_bounds__(NW * 64) void k_attn_step_##tag##_##D##_r##RT##w##NW(              \
+        const AttnOpArgs a)                                                                                    \
+    {                                                                                                          \
+        attn_step<TQ, D, RT, NW>(a);                                                                           \
+    }
+#define STEPS(TQ, tag, D, MOST, WAVES)                                                                         \
+    STEP(TQ, tag, D, 1, 4)                                                                                     \
+    STEP(TQ, tag, D, 1, WAVES)                                                                                    \
+    STEP(TQ, tag, D, MOST, 4)                                                                                  \
+    extern "C" __global__ __launch_bounds__(256) void k_attn_merge_##tag##_##D(const AttnOpArgs a)             \
+    {                                                                                                          \
+        attn_merge<TQ, D>(a);                                                                                  \
+    }                                                                                                          \
+    extern "C" __global__ __launch_bounds__(256) void k_scored_join_##tag##_##D(const AttnOpArgs a)            \
+    {                                                                                                          \
+        scored_join<TQ, D>(a);                                                                                 \
+    }
+STEPS(F32, f32, 64, 4, 16)
+STEPS(F32, f32, 128, 2, 8)
+STEPS(F16, f16, 64, 4, 16)
+STEPS(F16, f16, 128, 2, 8)
+STEPS(BF16, bf16, 64, 4, 16)
+STEPS(BF16, bf16, 128, 2, 8)
 
 #define INSTANCES(TQ, TK, tag, D)                                                                              \
     extern "C" __global__ __launch_bounds__(64) void k_attn_simple_##tag##_##D(const AttnOpArgs a)             \
