@@ -42,13 +42,7 @@ struct AttnOpArgs {
     float *o;
     // scored: scores[(b * heads + h) * slots + j], in units of q . k
     float *scores;
-    const float *acc; // nullable
-    float *acc_out;   // [n_seq][kv_heads][slots]
-};
-
-struct ColsumArgs { // acc_out = acc_in + the rows' attention weights
-    KvView own;
-    RowsView r;       // lse set
+    float2 *stats; // nullable: per row and head {log2 offset, 1 / sum} of its weights
     const float *acc; // nullable
     float *acc_out;   // [n_seq][kv_heads][slots]
 };

@@ -23,10 +23,14 @@
     } while (0)
 
 // ------------------------------------------------------------------ code object
+// Row tiles of 16 of the larger forms, as many as the registers hold.
+static uint32_t step_tiles(uint32_t dim) { return dim == 64 ? 4 : 2; }
+static uint32_t tile_tiles(uint32_t type, uint32_t dim) { return dim == 64 && type != LFM_TYPE_F32 ? 4 : 2; }
+
 // Kernels by [type pair][head_dim 64, 128]; the pair is the rows' type.
 struct AttnKernels {
     hipModule_t mod = nullptr;
-    hipFunction_t attn_simple[3][2], colsum_simple[3][2];
+    hipFunction_t tile_1[3][2], tile_most[3][2], weights[3][2];
     hipFunction_t step_1w4[3][2], step_wide[3][2], step_most[3][2], merge[3][2], scored_join[3][2];
     hipFunction_t kv_select, kv_move;
 };
@@ -54,11 +58,12 @@ static int load_attn(int dev)
             struct {
                 hipFunction_t *f;
                 std::string name;
-            } fns[] = {{&k.attn_simple[t][d], "k_attn_simple" + tag},
-                       {&k.colsum_simple[t][d], "k_colsum_simple" + tag},
+            } fns[] = {{&k.tile_1[t][d], "k_attn_tile" + tag + "_r1"},
+                       {&k.tile_most[t][d], "k_attn_tile" + tag + "_r" + std::to_string(tile_tiles(t, d ? 128 : 64))},
+                       {&k.weights[t][d], "k_attn_weights" + tag},
                        {&k.step_1w4[t][d], "k_attn_step" + tag + "_r1w4"},
                        {&k.step_wide[t][d], "k_attn_step" + tag + (d ? "_r1w8" : "_r1w16")},
-                       {&k.step_most[t][d], "k_attn_step" + tag + (d ? "_r2w4" : "_r4w4")},
+                       {&k.step_most[t][d], "k_attn_step" + tag + "_r" + std::to_string(step_tiles(d ? 128 : 64)) + "w4"},
                        {&k.merge[t][d], "k_attn_merge" + tag},
                        {&k.scored_join[t][d], "k_scored_join" + tag}};
             for (auto &f : fns)
@@ -238,6 +243,8 @@ static RowsView view(const lfm_rows *r)
     return v;
 }
 
+static size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
 static int dim_index(const lfm_kv *c) { return c->head_dim == 128; }
 
 // ------------------------------------------------------------------ attention
@@ -245,32 +252,47 @@ static int dim_index(const lfm_kv *c) { return c->head_dim == 128; }
 struct Plan {
     uint32_t own_splits = 1, prefix_splits = 0, own_groups = 1, prefix_groups = 0;
     bool many_waves = false, most = false; // the step kernel's form
-    bool join = false;                     // a second kernel joins the key ranges
-    size_t ml_bytes = 0, o_bytes = 0, score_bytes = 0;
-    size_t bytes() const { return ml_bytes + o_bytes + score_bytes; }
+    bool tile_most = false;                // the tile kernel's
+    uint64_t tile_items = 0;
+    bool join = false; // a second kernel joins the key ranges
+    size_t ml_bytes = 0, o_bytes = 0, score_bytes = 0, stat_bytes = 0;
+    size_t bytes() const { return ml_bytes + o_bytes + score_bytes + stat_bytes; }
 };
 
-static size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 #define TARGET_WAVES 4096 // four to each of 1024 SIMDs
 
 static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint32_t window, uint32_t sinks, bool scored)
 {
     Plan p;
-    const uint32_t G = r->heads / kv->kv_heads, most = kv->head_dim == 64 ? 64 : 32;
-    const uint64_t span = window ? std::min<uint64_t>(kv->slots, (uint64_t)window + sinks + 63) : kv->slots;
-    const uint64_t blocks = (span + 31) / 32;
+    const uint32_t G = r->heads / kv->kv_heads;
     const uint64_t pairs = (uint64_t)r->n_rows * r->heads;
     p.most = prefix ? (uint64_t)r->n_rows * G > 16 : G > 16;
-    const uint32_t per = p.most ? most : 16;
-    p.own_groups = (G + per - 1) / per;
-    const uint64_t items = (uint64_t)std::max(1u, r->n_rows) * p.own_groups * kv->kv_heads;
-    // a wave needs a few blocks for its loads to overlap; below that ranges only add joining
-    p.own_splits = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, TARGET_WAVES / 4 / items),
-                                                std::max<uint64_t>(1, blocks / 16));
-    if (!prefix && !p.most && blocks <= 64 && items < 1024) {
-        p.own_splits = 1;
-        p.many_waves = blocks > 4;
+    const uint32_t per = p.most ? 16 * step_tiles(kv->head_dim) : 16;
+    if (!r->start) {
+        const uint64_t span = window ? std::min<uint64_t>(kv->slots, (uint64_t)window + sinks + 63) : kv->slots;
+        const uint64_t blocks = (span + 31) / 32;
+        p.own_groups = (G + per - 1) / per;
+        const uint64_t items = (uint64_t)std::max(1u, r->n_rows) * p.own_groups * kv->kv_heads;
+        // a wave needs a few blocks for its loads to overlap; below that ranges only add joining
+        p.own_splits = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, TARGET_WAVES / 4 / items),
+                                                    std::max<uint64_t>(1, blocks / 16));
+        if (!prefix && !p.most && blocks <= 64 && items < 1024) {
+            p.own_splits = 1;
+            p.many_waves = blocks > 4;
+        }
+    } else {
+        // sequences end inside tiles: at most one more tile each
+        const uint64_t cut = (uint64_t)r->n_rows * G;
+        const uint32_t most = 64 * tile_tiles(r->type, kv->head_dim);
+        p.tile_most = cut / most * kv->kv_heads >= 512;
+        const uint64_t rows = p.tile_most ? most : 64;
+        p.tile_items = cut / rows + std::min<uint64_t>(kv->n_seq, r->n_rows);
+        const uint64_t span = window ? std::min<uint64_t>(kv->slots, (uint64_t)window + sinks + rows / G + 128)
+                                     : kv->slots;
+        p.own_splits = (uint32_t)std::min<uint64_t>(
+            std::max<uint64_t>(1, 512 / std::max<uint64_t>(1, p.tile_items * kv->kv_heads)),
+            std::max<uint64_t>(1, span / 512));
     }
     if (prefix) {
         p.prefix_groups = (uint32_t)(((uint64_t)r->n_rows * G + per - 1) / per);
@@ -279,13 +301,16 @@ static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint
                                                        std::max<uint64_t>(1, (prefix->slots + 511) / 512));
     }
     const uint32_t splits = p.own_splits + p.prefix_splits;
-    p.join = scored || splits > 1;
+    const bool steps = scored && !r->start; // scores are kept from the step to the join
+    p.join = steps || splits > 1;
     if (p.join) {
         p.ml_bytes = round256((size_t)splits * pairs * 8);
         p.o_bytes = round256((size_t)splits * pairs * kv->head_dim * 4);
     }
-    if (scored)
+    if (steps)
         p.score_bytes = round256((size_t)pairs * kv->slots * 4);
+    else if (scored)
+        p.stat_bytes = round256((size_t)pairs * 8);
     return p;
 }
 
@@ -303,40 +328,43 @@ static AttnOpArgs op_args(const Plan &p, const lfm_kv *prefix, const lfm_kv *kv,
     a.own_groups = p.own_groups, a.prefix_groups = p.prefix_groups;
     uint8_t *w = (uint8_t *)ws;
     a.ml = (float2 *)w;
-    a.o = (float *)(w + p.ml_bytes);
-    a.scores = p.score_bytes ? (float *)(w + p.ml_bytes + p.o_bytes) : nullptr;
+    a.o = (float *)(w += p.ml_bytes);
+    w += p.o_bytes;
+    a.scores = p.score_bytes ? (float *)w : nullptr;
+    w += p.score_bytes;
+    a.stats = p.stat_bytes ? (float2 *)w : nullptr;
     return a;
 }
 
-// Single rows: one launch over (kv head, row group and key range), one that joins.
-static int attend_step(AttnKernels *K, const Plan &p, const AttnOpArgs &a, const lfm_kv *kv, const lfm_rows *rows,
-                       hipStream_t s)
+// Grids are flat, kv heads fastest: with 8 of them each XCD's cache serves one.
+static int launch_items(hipFunction_t f, uint64_t items, uint32_t kv_heads, uint32_t threads, hipStream_t s,
+                        const AttnOpArgs &a)
+{
+    if (items * kv_heads > 0x7FFFFFFFull)
+        return fail(LFM_EINVAL, "attention: %llu work items of %u kv heads", (unsigned long long)items, kv_heads);
+    return launch(f, dim3((uint32_t)items * kv_heads), threads, s, a);
+}
+
+// One launch over (kv head, rows, key range), the prefix's items before the own ones; rows
+// of many tokens take theirs in a second launch; then the ranges are joined.
+static int attend(AttnKernels *K, const Plan &p, const AttnOpArgs &a, const lfm_kv *kv, const lfm_rows *rows,
+                  hipStream_t s)
 {
     const int t = rows->type, d = dim_index(kv);
-    const uint64_t items = (uint64_t)p.prefix_groups * p.prefix_splits +
-                           (uint64_t)rows->n_rows * p.own_groups * p.own_splits;
-    if (items * kv->kv_heads > 0x7FFFFFFFull)
-        return fail(LFM_EINVAL, "attention: %llu work items", (unsigned long long)items);
-    hipFunction_t f = p.most ? K->step_most[t][d] : p.many_waves ? K->step_wide[t][d] : K->step_1w4[t][d];
-    RC(launch(f, dim3((uint32_t)items * kv->kv_heads), p.many_waves ? (d ? 512 : 1024) : 256, s, a));
+    const uint64_t steps = (uint64_t)p.prefix_groups * p.prefix_splits +
+                           (rows->start ? 0 : (uint64_t)rows->n_rows * p.own_groups * p.own_splits);
+    if (steps) {
+        hipFunction_t f = p.most ? K->step_most[t][d] : p.many_waves ? K->step_wide[t][d] : K->step_1w4[t][d];
+        RC(launch_items(f, steps, kv->kv_heads, p.many_waves ? (d ? 512 : 1024) : 256, s, a));
+    }
+    if (rows->start)
+        RC(launch_items(p.tile_most ? K->tile_most[t][d] : K->tile_1[t][d], p.tile_items * p.own_splits, kv->kv_heads,
+                        256, s, a));
     if (a.scores)
         return launch(K->scored_join[t][d], dim3((kv->slots + 511) / 512, kv->kv_heads, kv->n_seq), 256, s, a);
     if (p.join)
         return launch(K->merge[t][d], dim3((rows->n_rows * rows->heads + 3) / 4), 256, s, a);
     return LFM_OK;
-}
-
-static int attend(const char *op, const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *rows, uint32_t window,
-                  uint32_t sinks, float *lse, void *ws, hipStream_t s, int dev)
-{
-    AttnKernels *K;
-    RC(attn_kernels(dev, &K));
-    const Plan p = plan(prefix, kv, rows, window, sinks, false);
-    AttnOpArgs a = op_args(p, prefix, kv, rows, window, sinks, ws);
-    a.r.lse = lse;
-    if (!rows->start)
-        return attend_step(K, p, a, kv, rows, s);
-    return launch(K->attn_simple[rows->type][dim_index(kv)], dim3(rows->n_rows, rows->heads), 64, s, a);
 }
 
 extern "C" int lfm_attn_window_workspace(const lfm_kv *kv, const lfm_rows *rows, uint32_t window, uint32_t sinks,
@@ -364,7 +392,10 @@ extern "C" int lfm_attn_window(const lfm_kv *kv, const lfm_rows *rows, uint32_t 
     RC(check_kv_ptrs(op, KV_NAMES, kv, dev));
     RC(check_rows_ptrs(op, rows, dev));
     RC(check_workspace(op, workspace, workspace_bytes, need, dev));
-    return attend(op, nullptr, kv, rows, window, sinks, rows->lse, workspace, (hipStream_t)stream, dev);
+    AttnKernels *K;
+    RC(attn_kernels(dev, &K));
+    const Plan p = plan(nullptr, kv, rows, window, sinks, false);
+    return attend(K, p, op_args(p, nullptr, kv, rows, window, sinks, workspace), kv, rows, (hipStream_t)stream);
 }
 
 extern "C" int lfm_attn_scored_workspace(const lfm_kv *kv, const lfm_rows *rows, size_t *bytes)
@@ -374,10 +405,7 @@ extern "C" int lfm_attn_scored_workspace(const lfm_kv *kv, const lfm_rows *rows,
     RC(check_rows(op, kv, rows));
     if (!bytes)
         return fail(LFM_EINVAL, "%s: bytes is null", op);
-    if (!rows->start)
-        *bytes = plan(nullptr, kv, rows, 0, 0, true).bytes();
-    else // lse, where the caller wants none
-        *bytes = round256((size_t)rows->n_rows * rows->heads * 4) + plan(nullptr, kv, rows, 0, 0, false).bytes();
+    *bytes = plan(nullptr, kv, rows, 0, 0, true).bytes();
     return LFM_OK;
 }
 
@@ -401,24 +429,15 @@ extern "C" int lfm_attn_scored(const lfm_kv *kv, const lfm_rows *rows, const flo
     hipStream_t s = (hipStream_t)stream;
     AttnKernels *K;
     RC(attn_kernels(dev, &K));
-    if (!rows->start) {
-        const Plan p = plan(nullptr, kv, rows, 0, 0, true);
-        AttnOpArgs a = op_args(p, nullptr, kv, rows, 0, 0, workspace);
-        a.acc = acc_in, a.acc_out = acc_out;
-        return attend_step(K, p, a, kv, rows, s);
-    }
-    float *lse = rows->lse ? rows->lse : (float *)workspace;
-    if (rows->n_rows)
-        RC(attend(op, nullptr, kv, rows, 0, 0, lse,
-                  (uint8_t *)workspace + round256((size_t)rows->n_rows * rows->heads * 4), s, dev));
-    ColsumArgs a;
-    memset(&a, 0, sizeof(a));
-    a.own = view(kv);
-    a.r = view(rows);
-    a.r.lse = lse;
+    const Plan p = plan(nullptr, kv, rows, 0, 0, true);
+    AttnOpArgs a = op_args(p, nullptr, kv, rows, 0, 0, workspace);
     a.acc = acc_in, a.acc_out = acc_out;
-    return launch(K->colsum_simple[rows->type][dim_index(kv)], dim3((kv->slots + 63) / 64, kv->kv_heads, kv->n_seq),
-                  64, s, a);
+    if (rows->n_rows)
+        RC(attend(K, p, a, kv, rows, s));
+    if (!rows->start)
+        return LFM_OK;
+    return launch(K->weights[rows->type][dim_index(kv)], dim3((kv->slots + 63) / 64, kv->kv_heads, kv->n_seq), 512, s,
+                  a);
 }
 
 static int check_prefix(const char *op, const lfm_kv *prefix, const lfm_kv *kv)
@@ -457,7 +476,10 @@ extern "C" int lfm_attn_prefix(const lfm_kv *prefix, const lfm_kv *kv, const lfm
     RC(check_kv_ptrs(op, KV_NAMES, kv, dev));
     RC(check_rows_ptrs(op, rows, dev));
     RC(check_workspace(op, workspace, workspace_bytes, need, dev));
-    return attend(op, prefix, kv, rows, 0, 0, rows->lse, workspace, (hipStream_t)stream, dev);
+    AttnKernels *K;
+    RC(attn_kernels(dev, &K));
+    const Plan p = plan(prefix, kv, rows, 0, 0, false);
+    return attend(K, p, op_args(p, prefix, kv, rows, 0, 0, workspace), kv, rows, (hipStream_t)stream);
 }
 
 // ------------------------------------------------------------------ eviction

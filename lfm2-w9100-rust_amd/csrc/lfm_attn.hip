@@ -89,7 +89,8 @@ __device__ __forceinline__ void seq_rows(const RowsView &r, uint32_t b, int32_t 
     *hi = max(*lo, min(r.start[b + 1], (int32_t)r.n_rows));
 }
 
-// Sequence and position of a row; false where the row belongs to none.
+// Sequence and position of a row, the same for a whole wave; false where the row belongs to
+// no sequence.
 __device__ __forceinline__ bool find_row(const AttnOpArgs &a, uint32_t row, uint32_t *b, int32_t *pos)
 {
     if (!a.r.start) {
@@ -97,12 +98,16 @@ __device__ __forceinline__ bool find_row(const AttnOpArgs &a, uint32_t row, uint
         *pos = clamp_len(a.own, row) - 1;
         return true;
     }
-    for (uint32_t s = 0; s < a.own.n_seq; ++s) {
-        int32_t lo, hi;
-        seq_rows(a.r, s, &lo, &hi);
-        if ((int32_t)row >= lo && (int32_t)row < hi) {
-            *b = s;
-            *pos = clamp_len(a.own, s) - hi + (int32_t)row;
+    const uint32_t lane = threadIdx.x & 63;
+    for (uint32_t s0 = 0; s0 < a.own.n_seq; s0 += 64) {
+        int32_t lo = 0, hi = 0;
+        if (s0 + lane < a.own.n_seq)
+            seq_rows(a.r, s0 + lane, &lo, &hi);
+        const uint64_t in = __ballot((int32_t)row >= lo && (int32_t)row < hi);
+        if (in) {
+            const uint32_t at = (uint32_t)__ffsll((unsigned long long)in) - 1;
+            *b = s0 + at;
+            *pos = clamp_len(a.own, *b) - __builtin_amdgcn_readlane(hi, at) + (int32_t)row;
             return true;
         }
     }
@@ -259,30 +264,37 @@ __device__ __forceinline__ typename TQ::vec v_operand(const uint8_t *tile, uint3
 }
 
 // ------------------------------------------------------------------ visible blocks
-// Blocks of 32 slots that a row at hi - 1 sees: those of the first tokens, then those of
-// the window (all in one run where the two meet).
-struct Blocks {
-    uint32_t hi, wlo, sinks; // slot j is seen: j < hi and (j < sinks or j >= wlo)
+// Blocks of N slots that rows at positions lo .. hi see: those of the first tokens, then
+// those of the window (all in one run where the two meet).  A slot is taken to be seen where
+// the earliest row's window and the latest row's position allow it; with lo and hi exchanged,
+// where every row does.
+template <int N> struct Blocks {
+    uint32_t hi, wlo, sinks; // slot j: j < hi and (j < sinks or j >= wlo)
     uint32_t first, skip, count;
-    __device__ __forceinline__ void set(int32_t pos, uint32_t window, uint32_t s)
+    __device__ __forceinline__ void set(int32_t pos_lo, int32_t pos_hi, uint32_t window, uint32_t s)
     {
-        hi = (uint32_t)max(pos + 1, 0);
-        wlo = window && window < hi ? hi - window : 0;
+        hi = (uint32_t)max(pos_hi + 1, 0);
+        const uint32_t end = (uint32_t)max(pos_lo + 1, 0);
+        wlo = window && window < end ? end - window : 0;
         if (s >= wlo)
             wlo = 0;
         sinks = wlo ? s : 0;
-        first = (sinks + 31) / 32;
-        const uint32_t from = max(wlo / 32, first);
+        first = (min(sinks, hi) + N - 1) / N;
+        const uint32_t from = max(wlo / N, first);
         skip = from - first;
-        count = (hi + 31) / 32 - skip;
+        count = max((hi + N - 1) / N, from) - skip;
     }
     __device__ __forceinline__ uint32_t block(uint32_t i) const { return i < first ? i : i + skip; }
-    __device__ __forceinline__ bool whole(uint32_t blk) const
-    {
-        const uint32_t j = blk * 32;
-        return j + 32 <= hi && (j + 32 <= sinks || j >= wlo);
-    }
     __device__ __forceinline__ bool seen(uint32_t j) const { return j < hi && (j < sinks || j >= wlo); }
+    __device__ __forceinline__ bool covers(uint32_t j, uint32_t n) const
+    {
+        return j + n <= hi && (j + n <= sinks || j >= wlo);
+    }
+    __device__ __forceinline__ bool touches(uint32_t j, uint32_t n) const
+    {
+        return j < hi && (j < sinks || j + n > wlo);
+    }
+    __device__ __forceinline__ bool whole(uint32_t blk) const { return covers(blk * N, N); }
 };
 
 // A key range's share [lo, hi) of n blocks.
@@ -290,6 +302,15 @@ __device__ __forceinline__ void share(uint32_t n, uint32_t part, uint32_t parts,
 {
     *lo = (uint32_t)((uint64_t)n * part / parts);
     *hi = (uint32_t)((uint64_t)n * (part + 1) / parts);
+}
+
+// A row's state once it is whole: its lse, and what attn_weights needs of it.
+__device__ __forceinline__ void finish_row(const AttnOpArgs &a, size_t id, bool empty, float offset, float l)
+{
+    if (a.r.lse)
+        a.r.lse[id] = empty ? -INFINITY : (offset + log2f(l)) * 0.6931471805599453f;
+    if (a.stats)
+        a.stats[id] = empty ? make_float2(0.f, 0.f) : make_float2(offset, 1.0f / l);
 }
 
 // ------------------------------------------------------------------ rows that see the same slots
@@ -316,11 +337,11 @@ template <typename TQ, int D, int RT, int NW> __device__ __forceinline__ void at
     uint32_t group, part, parts, row0, total;
     const uint16_t *kp, *vp;
     int64_t ts;
-    Blocks bl;
+    Blocks<32> bl;
     if (pre) {
         group = item % a.prefix_groups, part = item / a.prefix_groups, parts = a.prefix_splits;
         row0 = 0, total = a.r.n_rows * G;
-        bl.set(clamp_len(a.prefix, 0) - 1, 0, 0);
+        bl.set(0, clamp_len(a.prefix, 0) - 1, 0, 0);
         const int64_t at = (int64_t)kh * a.prefix.hs;
         kp = a.prefix.k + at, vp = a.prefix.v + at, ts = a.prefix.ts;
     } else {
@@ -328,7 +349,8 @@ template <typename TQ, int D, int RT, int NW> __device__ __forceinline__ void at
         group = item % a.own_groups, item /= a.own_groups;
         part = item % a.own_splits, parts = a.own_splits;
         row0 = item / a.own_splits, total = G;
-        bl.set(clamp_len(a.own, row0) - 1, a.window, a.sinks);
+        const int32_t pos = clamp_len(a.own, row0) - 1;
+        bl.set(pos, pos, a.window, a.sinks);
         const int64_t at = (int64_t)row0 * a.own.ss + (int64_t)kh * a.own.hs;
         kp = a.own.k + at, vp = a.own.v + at, ts = a.own.ts;
     }
@@ -478,8 +500,8 @@ template <typename TQ, int D, int RT, int NW> __device__ __forceinline__ void at
         if (final) {
             const bool empty = bl.hi == 0;
             store_out<TQ>(a.r, row, h, d, empty ? o : o / l);
-            if (d == 0 && a.r.lse)
-                a.r.lse[(size_t)row * a.r.heads + h] = empty ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+            if (d == 0)
+                finish_row(a, (size_t)row * a.r.heads + h, empty, top, l);
         } else {
             const size_t at2 = ((size_t)(pre ? a.own_splits + part : part) * a.r.n_rows + row) * a.r.heads + h;
             *(floatx4 *)(a.o + at2 * D + d) = o;
@@ -524,8 +546,8 @@ template <typename TQ, int D> __device__ __forceinline__ void attn_merge(const A
 #pragma unroll
     for (int i = 0; i < E; ++i)
         to[i] = (tq)(empty ? 0.f : o[i] / l);
-    if (a.r.lse && lane == 0)
-        a.r.lse[id] = empty ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+    if (lane == 0)
+        finish_row(a, id, empty, top, l);
 }
 
 #define SCORED_SLOTS 512
@@ -569,8 +591,8 @@ template <typename TQ, int D> __device__ __forceinline__ void scored_join(const 
 #pragma unroll
             for (int i = 0; i < E; ++i)
                 to[i] = (tq)(n == 0 ? 0.f : o[i] / l);
-            if (a.r.lse && lane == 0)
-                a.r.lse[id] = n == 0 ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+            if (lane == 0)
+                finish_row(a, id, n == 0, top, l);
         }
     }
     __syncthreads();
@@ -584,97 +606,347 @@ template <typename TQ, int D> __device__ __forceinline__ void scored_join(const 
     }
 }
 
-// One wave per row and head: 64 slots at a time, a lane's score each, then every lane its
-// dims of the weighted sum.
-template <typename TQ, typename TK, int D> __device__ void attn_simple(const AttnOpArgs &a)
+// ------------------------------------------------------------------ rows of many tokens
+// The (sequence, part) of a flat item where sequence b has ceil(rows_b * per / of) of them;
+// false past the last.  64 sequences at a time, the same in every wave.
+__device__ __forceinline__ bool find_item(const RowsView &r, uint32_t n_seq, uint32_t item, uint32_t per, uint32_t of,
+                                          uint32_t *b, uint32_t *part, uint32_t *parts)
 {
-    typedef typename TQ::type tq;
-    typedef typename TK::kv tk;
-    const uint32_t row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, kh = h / (a.r.heads / a.own.kv_heads);
-    uint32_t b;
-    int32_t pos;
-    if (!find_row(a, row, &b, &pos))
-        return;
-    __shared__ float qs[D], ps[64];
-    for (int d = lane; d < D; d += 64)
-        qs[d] = (float)((const tq *)a.r.q)[(int64_t)row * a.r.q_rs + (int64_t)h * a.r.q_hs + d];
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, o[D / 64];
-    for (int i = 0; i < D / 64; ++i)
-        o[i] = 0.f;
-    for (int part = 0; part < 2; ++part) {
-        if (part == 0 && !a.prefix.k)
-            continue;
-        const KvView &c = part ? a.own : a.prefix;
-        const int32_t n = part ? pos + 1 : clamp_len(c, 0);
-        const int64_t base = (part ? (int64_t)b * c.ss : 0) + (int64_t)kh * c.hs;
-        const tk *k = (const tk *)c.k + base, *v = (const tk *)c.v + base;
-        for (int32_t j0 = 0; j0 < n; j0 += 64) {
-            const int32_t j = j0 + (int32_t)lane;
-            bool seen = j < n;
-            if (part && a.window)
-                seen = seen && (j < (int64_t)a.sinks || j > (int64_t)pos - a.window);
-            float s = -INFINITY;
-            if (seen) {
-                s = 0.f;
-                for (int d = 0; d < D; ++d)
-                    s += qs[d] * (float)k[(int64_t)j * c.ts + d];
-            }
-            const uint64_t any = __ballot(seen);
-            if (!any)
-                continue;
-            const float mn = fmaxf(m, wave_max(s));
-            const float r = m > -INFINITY ? exp2f((m - mn) * a.r.cexp) : 0.f;
-            const float p = seen ? exp2f((s - mn) * a.r.cexp) : 0.f;
-            l = l * r + wave_sum(p);
-            m = mn;
-            __syncthreads();
-            ps[lane] = p;
-            __syncthreads();
-            for (int i = 0; i < D / 64; ++i)
-                o[i] *= r;
-            for (int jj = 0; jj < 64; ++jj)
-                if ((any >> jj) & 1)
-                    for (int i = 0; i < D / 64; ++i)
-                        o[i] += ps[jj] * (float)v[(int64_t)(j0 + jj) * c.ts + lane + 64 * i];
+    const uint32_t lane = threadIdx.x & 63;
+    for (uint32_t s0 = 0; s0 < n_seq; s0 += 64) {
+        uint32_t n = 0;
+        if (s0 + lane < n_seq) {
+            int32_t lo, hi;
+            seq_rows(r, s0 + lane, &lo, &hi);
+            n = (uint32_t)(((uint64_t)(hi - lo) * per + of - 1) / of);
         }
+        uint32_t upto = n; // inclusive sums over the lanes
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = __shfl_up(upto, d);
+            upto += lane >= (uint32_t)d ? o : 0;
+        }
+        const uint32_t all = __builtin_amdgcn_readlane(upto, 63);
+        if (item < all) {
+            const uint32_t at = (uint32_t)__ffsll((unsigned long long)__ballot(upto > item)) - 1;
+            *b = s0 + at;
+            *parts = __builtin_amdgcn_readlane(n, at);
+            *part = item - (__builtin_amdgcn_readlane(upto, at) - *parts);
+            return true;
+        }
+        item -= all;
     }
-    const bool empty = pos < 0 && (!a.prefix.k || clamp_len(a.prefix, 0) == 0);
-    for (int i = 0; i < D / 64; ++i)
-        ((tq *)a.r.out)[(int64_t)row * a.r.o_rs + (int64_t)h * a.r.o_hs + lane + 64 * i] =
-            (tq)(empty ? 0.f : o[i] / l);
-    if (a.r.lse && lane == 0)
-        a.r.lse[(size_t)row * a.r.heads + h] = empty ? -INFINITY : m * a.r.scale + logf(l);
+    return false;
 }
 
-// One wave per 64 slots of a (sequence, kv head): a lane adds the weights its slot gets
-// from every row and head, in order.
-template <typename TQ, typename TK, int D> __device__ void colsum_simple(const ColsumArgs &a)
+template <typename TQ> __device__ __forceinline__ bool has_nonfinite(uint4 v)
 {
-    typedef typename TQ::type tq;
-    typedef typename TK::kv tk;
+    constexpr uint32_t E = TQ::offset == 0.f ? 0x7F807F80u : 0x7C007C00u; // exponents of two numbers
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        bad = bad || (w[i] & E & 0xFFFF0000u) == (E & 0xFFFF0000u) || (w[i] & E & 0xFFFFu) == (E & 0xFFFFu);
+    return bad;
+}
+
+#define TILE_KEYS 64
+// One workgroup: 64 RT (token, head) pairs of one sequence and kv head, 16 RT a wave, over
+// one key range.  Blocks of 64 slots pass through two buffers of shared memory, K and V as
+// they lie in the cache with their 16-byte pieces exchanged (v_piece); every wave reads K as
+// A operands and V through the transposed read.  The next block's loads are in flight while
+// a block is used.  Blocks that no row of a wave sees are passed over by it, those that all
+// its rows see whole are used without masks.
+//
+// A slot that some rows of a wave see and others do not may hold an infinity or NaN in V,
+// which times a weight of 0 would reach all of them: where a masked block holds such
+// numbers, the products leave them out and they are added row by row.
+template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(const AttnOpArgs &a)
+{
+    typedef typename TQ::vec vec;
+    constexpr uint32_t ROWS = 64 * RT, PIECES = D / 8, BYTES = TILE_KEYS * D * 2;
+    constexpr int LD = TILE_KEYS * PIECES / 256; // 16-byte loads of K, and of V, a thread and block
+    __shared__ __attribute__((aligned(16))) uint8_t ks[2][BYTES], vs[2][BYTES];
+    __shared__ float pw[4][16][33]; // one row tile's weights of 32 slots, a wave each
+    __shared__ uint64_t odd[4];     // slots of a block whose V is not all finite
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4;
+    const uint32_t kh = blockIdx.x % a.own.kv_heads, G = a.r.heads / a.own.kv_heads;
+    const uint32_t flat = blockIdx.x / a.own.kv_heads, split = flat % a.own_splits;
+    uint32_t b, tile, tiles;
+    if (!find_item(a.r, a.own.n_seq, flat / a.own_splits, G, ROWS, &b, &tile, &tiles))
+        return;
+    tile = tiles - 1 - tile; // the longest first
+    int32_t lo, hi;
+    seq_rows(a.r, b, &lo, &hi);
+    const uint32_t total = (uint32_t)(hi - lo) * G, p0 = tile * ROWS;
+    const int32_t first = clamp_len(a.own, b) - (hi - lo); // position of the sequence's first row
+    const int32_t pos_lo = first + (int32_t)(p0 / G), pos_hi = first + (int32_t)((min(p0 + ROWS, total) - 1) / G);
+    Blocks<TILE_KEYS> bl;
+    bl.set(pos_lo, pos_hi, a.window, a.sinks);
+    uint32_t b0, b1;
+    share(bl.count, split, a.own_splits, &b0, &b1);
+
+    Queries<TQ, D, RT> Q;
+    State<TQ, D, RT> S;
+    S.clear();
+    int32_t pos[RT];
+    const uint32_t w0 = p0 + wave * 16 * RT;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const uint32_t i = w0 + 16 * t + (lane & 15);
+        load_row<TQ, D, RT>(Q, t, a.r, i < total, (uint32_t)lo + i / G, kh * G + i % G);
+        pos[t] = i < total ? first + (int32_t)(i / G) : -1;
+    }
+    // what this wave's rows see: some row of it, every row of it
+    const bool any_row = w0 < total;
+    const int32_t wpos_lo = first + (int32_t)(w0 / G), wpos_hi = first + (int32_t)((min(w0 + 16 * RT, total) - 1) / G);
+    Blocks<32> some, each;
+    some.set(wpos_lo, wpos_hi, a.window, a.sinks);
+    each.set(wpos_hi, wpos_lo, a.window, a.sinks);
+    Blocks<TILE_KEYS> all; // every row of the workgroup
+    all.set(pos_hi, pos_lo, a.window, a.sinks);
+
+    const int64_t at0 = (int64_t)b * a.own.ss + (int64_t)kh * a.own.hs;
+    const uint16_t *kp = a.own.k + at0, *vp = a.own.v + at0;
+    uint4 kr[LD], vr[LD];
+    auto load = [&](uint32_t blk) {
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const uint32_t j = min(blk * TILE_KEYS + (i * 256 + tid) / PIECES, bl.hi - 1);
+            const int64_t o = (int64_t)j * a.own.ts + (tid % PIECES) * 8;
+            kr[i] = *(const uint4 *)(kp + o);
+            vr[i] = *(const uint4 *)(vp + o);
+        }
+    };
+    // slots past the last visible one repeat it in K and are zeros in V
+    auto store = [&](uint32_t i0, uint32_t blk, uint32_t buf) {
+        const bool whole = all.whole(blk);
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const uint32_t row = (i * 256 + tid) / PIECES, to = v_piece<D>(row, tid % PIECES) * 16;
+            *(uint4 *)(ks[buf] + to) = kr[i];
+            if (!whole) {
+                if (!bl.seen(blk * TILE_KEYS + row))
+                    vr[i] = make_uint4(0, 0, 0, 0);
+                else if (has_nonfinite<TQ>(vr[i]))
+                    atomicOr((unsigned long long *)&odd[i0 & 3], 1ull << row);
+            }
+            *(uint4 *)(vs[buf] + to) = vr[i];
+        }
+    };
+    if (tid < 4)
+        odd[tid] = 0;
+    __syncthreads();
+    if (b0 < b1) {
+        load(bl.block(b0));
+        store(b0, bl.block(b0), 0);
+    }
+    if (b0 + 1 < b1)
+        load(bl.block(b0 + 1));
+    const uint32_t at = v_lane<D>(lane);
+    for (uint32_t i = b0; i < b1; ++i) {
+        const uint32_t blk = bl.block(i), buf = (i - b0) & 1;
+        __syncthreads();
+        if (tid == 0)
+            odd[(i + 2) & 3] = 0; // used last at i - 2, filled next at i + 1
+#pragma unroll
+        for (uint32_t sub = 0; sub < 2; ++sub) {
+            const uint32_t j0 = blk * TILE_KEYS + 32 * sub;
+            if (!any_row || !some.touches(j0, 32))
+                continue;
+            const bool whole = each.covers(j0, 32);
+            const uint8_t *kb = ks[buf] + sub * 32 * D * 2, *vb = vs[buf] + sub * 32 * D * 2;
+            vec k[2][D / 32];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x)
+                    k[u][x] = *(const vec *)(kb + v_piece<D>(16 * u + (lane & 15), g + 4 * x) * 16);
+            vec p[RT][TQ::parts];
+            uint32_t wrong = 0;
+            if (!whole)
+                wrong = __builtin_amdgcn_readfirstlane((uint32_t)(odd[i & 3] >> (32 * sub)));
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                floatx4 s[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    s[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+                        for (int y = 0; y < TQ::parts; ++y)
+                            s[u] = mma(k[u][x], Q.q[t][y][x], s[u]);
+                }
+                if (!whole) {
+                    // row at pos sees j <= pos, and j < sinks or j > pos - window
+                    const int32_t from = a.window && (uint32_t)max(pos[t], 0) >= a.window ? pos[t] - (int32_t)a.window : -1;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int32_t j = (int32_t)j0 + 16 * u + 4 * g + e;
+                            if (j > pos[t] || (j <= from && (uint32_t)j >= a.sinks))
+                                s[u][e] = -INFINITY;
+                        }
+                }
+                weigh<TQ, D, RT>(S, t, s, Q.c[TQ::parts == 2 ? t : 0], p[t]);
+            }
+            if (wrong) { // uniform; rare
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        float w = (float)p[t][0][x];
+                        if constexpr (TQ::parts == 2)
+                            w += (float)p[t][1][x];
+                        pw[wave][lane & 15][16 * (x / 4) + 4 * g + x % 4] = w;
+                    }
+                    __builtin_amdgcn_wave_barrier();
+                    for (uint32_t m = wrong; m; m &= m - 1) {
+                        const uint32_t j = (uint32_t)__ffs((int)m) - 1;
+                        const float w = pw[wave][lane & 15][j];
+#pragma unroll
+                        for (int n = 0; n < D / 16; ++n) {
+                            const typename TQ::kv *v =
+                                (const typename TQ::kv *)(vb + v_piece<D>(j, 2 * n + g / 2) * 16 + (g & 1) * 8);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float x = (float)v[e];
+                                if (w != 0.f && !(fabsf(x) < INFINITY))
+                                    S.o[t][n][e] += w * x;
+                            }
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) {
+                vec v = v_operand<TQ, D>(vb, at, n);
+                if (wrong)
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)
+                        if (!(fabsf((float)v[x]) < INFINITY))
+                            v[x] = (typename TQ::kv)0.f;
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+#pragma unroll
+                    for (int y = 0; y < TQ::parts; ++y)
+                        S.o[t][n] = mma(v, p[t][y], S.o[t][n]);
+            }
+        }
+        if (i + 1 < b1)
+            store(i + 1, bl.block(i + 1), buf ^ 1);
+        if (i + 2 < b1)
+            load(bl.block(i + 2));
+    }
+    const bool final = a.own_splits + a.prefix_splits == 1;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const float l = row_sum(S.l[t]);
+        const uint32_t i = w0 + 16 * t + (lane & 15);
+        if (i >= total)
+            continue;
+        const uint32_t row = (uint32_t)lo + i / G, h = kh * G + i % G;
+        const float off = S.m[t] > -INFINITY ? S.mc[t] : -INFINITY;
+        if (final) {
+            const bool empty = pos[t] < 0;
+            const float f = empty ? 0.f : 1.0f / l;
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n)
+                store_out<TQ>(a.r, row, h, 16 * n + 4 * g, S.o[t][n] * f);
+            if (g == 0)
+                finish_row(a, row * a.r.heads + h, empty, off, l);
+        } else {
+            const size_t to = ((size_t)split * a.r.n_rows + row) * a.r.heads + h;
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n)
+                *(floatx4 *)(a.o + to * D + 16 * n + 4 * g) = S.o[t][n];
+            if (g == 0)
+                a.ml[to] = make_float2(off, l);
+        }
+    }
+}
+
+#define SUM_KEYS 64
+#define SUM_WAVES 8
+// The weights that SUM_KEYS slots of one (sequence, kv head) receive from all rows: scores
+// once more, with the slots as B operands in registers and 16 (token, head) pairs at a time
+// as A operands, a wave every SUM_WAVES-th; a weight is 2^(s c - offset) / sum with its row's
+// softmax state.  A lane adds its slots' weights over its rows; the lanes' and the waves' sums
+// are joined in a fixed order.
+template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const AttnOpArgs &a)
+{
+    typedef typename TQ::vec vec;
+    constexpr int KT = SUM_KEYS / 16;
+    __shared__ float part[SUM_WAVES][SUM_KEYS];
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4;
     const uint32_t kh = blockIdx.y, b = blockIdx.z, G = a.r.heads / a.own.kv_heads;
-    const int32_t n = clamp_len(a.own, b), j = (int32_t)(blockIdx.x * 64 + threadIdx.x);
-    if (j >= n)
+    const uint32_t n = (uint32_t)clamp_len(a.own, b), j0 = blockIdx.x * SUM_KEYS;
+    if (j0 >= n)
         return;
     int32_t lo, hi;
     seq_rows(a.r, b, &lo, &hi);
-    const tk *k = (const tk *)a.own.k + (int64_t)b * a.own.ss + (int64_t)kh * a.own.hs + (int64_t)j * a.own.ts;
-    float sum = 0.f;
-    for (int32_t row = lo; row < hi; ++row) {
-        if (j > n - hi + row)
-            continue;
-        for (uint32_t g = 0; g < G; ++g) {
-            const uint32_t h = kh * G + g;
-            const tq *q = (const tq *)a.r.q + (int64_t)row * a.r.q_rs + (int64_t)h * a.r.q_hs;
-            float s = 0.f;
-            for (int d = 0; d < D; ++d)
-                s += (float)q[d] * (float)k[d];
-            sum += expf(s * a.r.scale - a.r.lse[(size_t)row * a.r.heads + h]);
+    const uint32_t total = (uint32_t)(hi - lo) * G;
+    const int32_t first = (int32_t)n - (hi - lo);
+    vec k[KT][D / 32];
+    const uint16_t *kp = a.own.k + (int64_t)b * a.own.ss + (int64_t)kh * a.own.hs + 8 * g;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        const uint16_t *p = kp + (int64_t)min(j0 + 16 * t + (lane & 15), n - 1) * a.own.ts;
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x)
+            k[t][x] = *(const vec *)(p + 32 * x);
+    }
+    float sum[KT] = {};
+    // pairs before the first that sees slot j0 add nothing
+    const uint32_t from = (int32_t)j0 > first ? ((j0 - first) * G) / 16 : 0;
+    for (uint32_t i0 = from + wave; i0 * 16 < total; i0 += SUM_WAVES) {
+        Queries<TQ, D, 1> Q;
+        const uint32_t i = i0 * 16 + (lane & 15);
+        load_row<TQ, D, 1>(Q, 0, a.r, i < total, (uint32_t)lo + i / G, kh * G + i % G);
+        // the lane's four rows of the result: 4 g + e
+        float off[4], inv[4], c[4];
+        int32_t pos[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t r = i0 * 16 + 4 * g + e;
+            const bool in = r < total;
+            const float2 st = in ? a.stats[((size_t)lo + r / G) * a.r.heads + kh * G + r % G] : make_float2(0.f, 0.f);
+            off[e] = st.x, inv[e] = st.y;
+            pos[e] = in ? first + (int32_t)(r / G) : -1;
+            c[e] = TQ::parts == 2 ? __shfl(Q.c[0], 4 * g + e) : Q.c[0];
+        }
+        const bool whole = first + (int32_t)(i0 * 16 / G) >= (int32_t)(j0 + SUM_KEYS - 1) && i0 * 16 + 16 <= total;
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            floatx4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+                for (int y = 0; y < TQ::parts; ++y)
+                    s = mma(Q.q[0][y][x], k[t][x], s);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float w = exp2_hw(fmaf(s[e], c[e], -off[e])) * inv[e];
+                sum[t] += whole || (int32_t)(j0 + 16 * t + (lane & 15)) <= pos[e] ? w : 0.f;
+            }
         }
     }
-    const size_t at = ((size_t)b * a.own.kv_heads + kh) * a.own.slots + j;
-    a.acc_out[at] = (a.acc ? a.acc[at] : 0.f) + sum;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        const float v = row_sum(sum[t]);
+        if (lane < 16)
+            part[wave][16 * t + lane] = v;
+    }
+    __syncthreads();
+    if (tid < SUM_KEYS && j0 + tid < n) {
+        float v = 0.f;
+        for (int w = 0; w < SUM_WAVES; ++w)
+            v += part[w][tid];
+        const size_t at = ((size_t)b * a.own.kv_heads + kh) * a.own.slots + j0 + tid;
+        a.acc_out[at] = (a.acc ? a.acc[at] : 0.f) + v;
+    }
 }
 
 // RT: row tiles of a workgroup of rows that see the same slots, as many as the registers
@@ -704,21 +976,24 @@ STEPS(F16, f16, 128, 2, 8)
 STEPS(BF16, bf16, 64, 4, 16)
 STEPS(BF16, bf16, 128, 2, 8)
 
-#define INSTANCES(TQ, TK, tag, D)                                                                              \
-    extern "C" __global__ __launch_bounds__(64) void k_attn_simple_##tag##_##D(const AttnOpArgs a)             \
+#define TILE(TQ, tag, D, RT)                                                                                   \
+    extern "C" __global__ __launch_bounds__(256, 2) void k_attn_tile_##tag##_##D##_r##RT(const AttnOpArgs a)   \
     {                                                                                                          \
-        attn_simple<TQ, TK, D>(a);                                                                             \
-    }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(64) void k_colsum_simple_##tag##_##D(const ColsumArgs a)           \
-    {                                                                                                          \
-        colsum_simple<TQ, TK, D>(a);                                                                           \
+        attn_tile<TQ, D, RT>(a);                                                                               \
     }
-INSTANCES(F32, F16, f32, 64)
-INSTANCES(F32, F16, f32, 128)
-INSTANCES(F16, F16, f16, 64)
-INSTANCES(F16, F16, f16, 128)
-INSTANCES(BF16, BF16, bf16, 64)
-INSTANCES(BF16, BF16, bf16, 128)
+#define TILES(TQ, tag, D, MOST)                                                                                \
+    TILE(TQ, tag, D, 1)                                                                                        \
+    TILE(TQ, tag, D, MOST)                                                                                     \
+    extern "C" __global__ __launch_bounds__(SUM_WAVES * 64) void k_attn_weights_##tag##_##D(const AttnOpArgs a)\
+    {                                                                                                          \
+        attn_weights<TQ, D>(a);                                                                                \
+    }
+TILES(F32, f32, 64, 2)
+TILES(F32, f32, 128, 2)
+TILES(F16, f16, 64, 4)
+TILES(F16, f16, 128, 2)
+TILES(BF16, bf16, 64, 4)
+TILES(BF16, bf16, 128, 2)
 
 // ------------------------------------------------------------------ eviction
 // Rank of a slot as an integer: NaN below every number, the protected slots above all.
