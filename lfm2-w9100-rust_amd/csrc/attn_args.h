@@ -32,7 +32,8 @@ struct AttnOpArgs {
     KvView prefix; // k null: none; else one sequence, visible to every row
     RowsView r;
     uint32_t window, sinks; // window 0: unlimited
-    // Key ranges: own_splits of the own slots, then prefix_splits of the prefix.  Where
+    uint32_t group;         // query heads of a kv head
+    // Key ranges, 64 at most: own_splits of the own slots, then prefix_splits of the prefix.  Where
     // there is more than one in all, range s of row r, head h writes its softmax state to
     // ml[(s * n_rows + r) * heads + h] = {log2 offset, sum} and its unnormalized output
     // beside it in o, and k_attn_merge joins them.

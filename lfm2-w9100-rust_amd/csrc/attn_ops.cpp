@@ -261,6 +261,12 @@ struct Plan {
 
 
 #define TARGET_WAVES 4096 // four to each of 1024 SIMDs
+#define MOST_RANGES 32    // key ranges of one kind: 64 lanes join a row's
+
+static uint32_t ranges(uint64_t wanted, uint64_t worth)
+{
+    return (uint32_t)std::min<uint64_t>({std::max<uint64_t>(1, wanted), std::max<uint64_t>(1, worth), MOST_RANGES});
+}
 
 static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint32_t window, uint32_t sinks, bool scored)
 {
@@ -275,8 +281,7 @@ static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint
         p.own_groups = (G + per - 1) / per;
         const uint64_t items = (uint64_t)std::max(1u, r->n_rows) * p.own_groups * kv->kv_heads;
         // a wave needs a few blocks for its loads to overlap; below that ranges only add joining
-        p.own_splits = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, TARGET_WAVES / 4 / items),
-                                                    std::max<uint64_t>(1, blocks / 16));
+        p.own_splits = ranges(TARGET_WAVES / 4 / items, blocks / 16);
         if (!prefix && !p.most && blocks <= 64 && items < 1024) {
             p.own_splits = 1;
             p.many_waves = blocks > 4;
@@ -290,15 +295,12 @@ static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint
         p.tile_items = cut / rows + std::min<uint64_t>(kv->n_seq, r->n_rows);
         const uint64_t span = window ? std::min<uint64_t>(kv->slots, (uint64_t)window + sinks + rows / G + 128)
                                      : kv->slots;
-        p.own_splits = (uint32_t)std::min<uint64_t>(
-            std::max<uint64_t>(1, 512 / std::max<uint64_t>(1, p.tile_items * kv->kv_heads)),
-            std::max<uint64_t>(1, span / 512));
+        p.own_splits = ranges(512 / std::max<uint64_t>(1, p.tile_items * kv->kv_heads), span / 512);
     }
     if (prefix) {
         p.prefix_groups = (uint32_t)(((uint64_t)r->n_rows * G + per - 1) / per);
         const uint64_t pitems = (uint64_t)std::max(1u, p.prefix_groups) * kv->kv_heads;
-        p.prefix_splits = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, TARGET_WAVES / 4 / pitems),
-                                                       std::max<uint64_t>(1, (prefix->slots + 511) / 512));
+        p.prefix_splits = ranges(TARGET_WAVES / 4 / pitems, (prefix->slots + 511) / 512);
     }
     const uint32_t splits = p.own_splits + p.prefix_splits;
     const bool steps = scored && !r->start; // scores are kept from the step to the join
@@ -324,6 +326,7 @@ static AttnOpArgs op_args(const Plan &p, const lfm_kv *prefix, const lfm_kv *kv,
         a.prefix = view(prefix);
     a.r = view(rows);
     a.window = window, a.sinks = sinks;
+    a.group = rows->heads / kv->kv_heads;
     a.own_splits = p.own_splits, a.prefix_splits = p.prefix_splits;
     a.own_groups = p.own_groups, a.prefix_groups = p.prefix_groups;
     uint8_t *w = (uint8_t *)ws;

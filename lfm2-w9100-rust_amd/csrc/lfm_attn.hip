@@ -7,6 +7,10 @@
 #include "attn_args.h"
 #include "wave_ops.h"
 
+template <int N> struct Const {
+    static constexpr int value = N;
+};
+
 // ------------------------------------------------------------------ types
 // Queries and weights meet K and V on the 16x16x32 matrix instruction: lane l holds 8
 // numbers of row (A) or column (B) l % 16, at inner places 8 (l / 16) + i, and 4 results,
@@ -22,16 +26,16 @@ struct F16 {
     typedef _Float16 type, kv;
     typedef f16x8 vec;
     static constexpr int parts = 1;
-    // Weights are 2^10 times their value relative to the largest, so that binary16's
-    // subnormals start 24 binary orders below it and not 14.
-    static constexpr float offset = 10.f;
+    // A weight is 2^7 or more times its value relative to the largest (see Weights), so that
+    // binary16's subnormals start 21 binary orders below it and not 14.
+    static constexpr float offset = 7.f;
 };
 struct F32 { // rows of 32 bits over a binary16 cache: two binary16 numbers each, 22 bits
     typedef float type;
     typedef _Float16 kv;
     typedef f16x8 vec;
     static constexpr int parts = 2;
-    static constexpr float offset = 10.f;
+    static constexpr float offset = 7.f;
 };
 struct BF16 {
     typedef __bf16 type, kv;
@@ -124,12 +128,36 @@ __device__ __forceinline__ void store_out(const RowsView &r, uint32_t row, uint3
 }
 
 // ------------------------------------------------------------------ rows in matrix form
-// Query rows of one lane (its row of RT tiles of 16) as B operands, and cexp / the power of
-// two that an F32 row was multiplied by so that its largest value lies in binary16's range.
+// Pairs of a row and one of a kv head's G query heads, counted through: pair x after
+// (row, rem) is row + (rem + x) / G, head (rem + x) % G.  rem + x stays below 384, where the
+// product with ceil(2^16 / G) gives the quotient exactly (G <= 128).
+struct Pairs {
+    uint32_t row, rem, G, inv;
+    __device__ __forceinline__ Pairs(uint32_t first_row, uint32_t pair, uint32_t group)
+    {
+        G = group;
+        inv = (65535 + G) / G;
+        const uint32_t q = G == 1 ? pair : pair / G;
+        row = first_row + q;
+        rem = pair - q * G;
+    }
+    __device__ __forceinline__ uint32_t row_of(uint32_t x) const { return row + (((rem + x) * inv) >> 16); }
+    __device__ __forceinline__ uint32_t head_of(uint32_t x) const
+    {
+        const uint32_t y = rem + x;
+        return y - ((y * inv) >> 16) * G;
+    }
+};
+
+// RT tiles of 16 query rows as B operands (the lane's row: lane % 16).  An F32 row is scaled
+// by the power of two that brings its largest value into binary16's range, and its scores
+// back by c.
 template <typename TQ, int D, int RT> struct Queries {
+    static constexpr int N = TQ::parts == 2 ? RT : 1;
     typename TQ::vec q[RT][TQ::parts][D / 32];
-    float c[TQ::parts == 2 ? RT : 1];
-    float back[TQ::parts == 2 ? RT : 1]; // the inverse of that power
+    float c[N], slack[N], back[N]; // cexp / power; 8 / c; 1 / power
+    __device__ __forceinline__ float c_of(int t) const { return c[N == 1 ? 0 : t]; }
+    __device__ __forceinline__ float slack_of(int t) const { return slack[N == 1 ? 0 : t]; }
 };
 
 template <typename TQ, int D, int RT>
@@ -148,6 +176,7 @@ __device__ __forceinline__ void load_row(Queries<TQ, D, RT> &Q, int t, const Row
             Q.q[t][0][j] = v;
         }
         Q.c[0] = r.cexp;
+        Q.slack[0] = fminf(8.f / r.cexp, 3.0e38f);
     } else {
         float x[D / 32][8], top = 0.f;
 #pragma unroll
@@ -171,6 +200,7 @@ __device__ __forceinline__ void load_row(Queries<TQ, D, RT> &Q, int t, const Row
         const float s = ldexpf(1.f, up);
         Q.back[t] = ldexpf(1.f, -up);
         Q.c[t] = r.cexp * Q.back[t];
+        Q.slack[t] = fminf(8.f * __builtin_amdgcn_rcpf(Q.c[t]), 3.0e38f);
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
 #pragma unroll
@@ -185,8 +215,9 @@ __device__ __forceinline__ void load_row(Queries<TQ, D, RT> &Q, int t, const Row
 
 // ------------------------------------------------------------------ softmax state
 // Of RT tiles of 16 rows: o[t][n] are dims 16 n + 4 (lane / 16) + e of row lane % 16.  m is
-// the largest score so far (units of q . k), mc = m c - offset; l the lane's own part of the
-// sum of the weights 2^(s c - mc), whose four parts are added at the end.
+// the score that weights are taken relative to (units of q . k), mc = m c - offset; l the
+// lane's own part of the sum of the weights 2^(s c - mc), whose four parts are added at the
+// end.
 template <typename TQ, int D, int RT> struct State {
     floatx4 o[RT][D / 16];
     float m[RT], mc[RT], l[RT];
@@ -202,37 +233,53 @@ template <typename TQ, int D, int RT> struct State {
     }
 };
 
-// Scores of 32 keys (s[0]: keys 4 (lane / 16) + e, s[1]: the same + 16) -> weights as a B
-// operand: inner place 8 (lane / 16) + i is key 16 (i / 4) + 4 (lane / 16) + i % 4.  The
-// rescaling of o is skipped where no row's maximum rose.
-template <typename TQ, int D, int RT>
-__device__ __forceinline__ void weigh(State<TQ, D, RT> &S, int t, const floatx4 (&s)[2], float c,
-                                      typename TQ::vec (&p)[TQ::parts])
+// Scores of 32 slots and NT row tiles (s[t][0]: slots 4 (lane / 16) + e, s[t][1]: the same +
+// 16) -> weights as B operands: inner place 8 (lane / 16) + i is slot 16 (i / 4) + 4 (lane /
+// 16) + i % 4.  m follows the largest score only when that is 8 binary orders above it, for
+// all the tiles at once: after the first block hardly ever, and a weight stays below 2^15.
+template <int NT, typename TQ, int D, int RT>
+__device__ __forceinline__ void weigh(State<TQ, D, RT> &S, const floatx4 (&s)[RT][2], const Queries<TQ, D, RT> &Q,
+                                      typename TQ::vec (&p)[RT][TQ::parts])
 {
-    float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
-    top = fmaxf(top, fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    if (__ballot(top > S.m[t])) {
-        const float mn = fmaxf(S.m[t], row_max(top));
-        // a row of -inf alone keeps offset 0: its weights are 2^-inf = 0
-        const float mcn = mn > -INFINITY ? mn * c - TQ::offset : 0.f;
-        const float r = S.m[t] > -INFINITY ? exp2_hw(S.mc[t] - mcn) : 0.f;
-        S.m[t] = mn, S.mc[t] = mcn, S.l[t] *= r;
+    float top[NT];
+    bool rises = false;
 #pragma unroll
-        for (int n = 0; n < D / 16; ++n)
-            S.o[t][n] *= r;
+    for (int t = 0; t < NT; ++t) {
+        const floatx4 &x = s[t][0], &y = s[t][1];
+        top[t] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+        rises |= top[t] > S.m[t] + Q.slack_of(t);
     }
-    float w[8];
+    if (__ballot(rises)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        w[i] = exp2_hw(fmaf(s[i / 4][i % 4], c, -S.mc[t]));
+        for (int t = 0; t < NT; ++t) {
+            const float mn = fmaxf(S.m[t], row_max(top[t]));
+            // a row of -inf alone keeps mc 0: its weights are 2^-inf = 0
+            const float mcn = mn > -INFINITY ? mn * Q.c_of(t) - TQ::offset : 0.f;
+            const float r = S.m[t] > -INFINITY ? exp2_hw(S.mc[t] - mcn) : 0.f;
+            S.m[t] = mn, S.mc[t] = mcn, S.l[t] *= r;
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n)
+                S.o[t][n] *= r;
+        }
     }
-    S.l[t] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+    typedef typename TQ::kv kv2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const auto hi = (typename TQ::kv)w[i];
-        p[0][i] = hi;
-        if constexpr (TQ::parts == 2)
-            p[1][i] = (_Float16)(w[i] - (float)hi);
+    for (int t = 0; t < NT; ++t) {
+        float w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            w[i] = exp2_hw(fmaf(s[t][i / 4][i % 4], Q.c_of(t), -S.mc[t]));
+        S.l[t] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const kv2 hi = __builtin_convertvector((float2v){w[i], w[i + 1]}, kv2);
+            p[t][0][i] = hi[0], p[t][0][i + 1] = hi[1];
+            if constexpr (TQ::parts == 2) {
+                const float2v back = __builtin_convertvector(hi, float2v);
+                const kv2 lo = __builtin_convertvector((float2v){w[i] - back[0], w[i + 1] - back[1]}, kv2);
+                p[t][1][i] = lo[0], p[t][1][i + 1] = lo[1];
+            }
+        }
     }
 }
 
@@ -300,9 +347,17 @@ template <int N> struct Blocks {
 // A key range's share [lo, hi) of n blocks.
 __device__ __forceinline__ void share(uint32_t n, uint32_t part, uint32_t parts, uint32_t *lo, uint32_t *hi)
 {
-    *lo = (uint32_t)((uint64_t)n * part / parts);
-    *hi = (uint32_t)((uint64_t)n * (part + 1) / parts);
+    if (parts == 1) {
+        *lo = 0, *hi = n;
+        return;
+    }
+    const uint32_t each = n / parts, more = n - each * parts;
+    *lo = each * part + min(part, more);
+    *hi = *lo + each + (part < more);
 }
+
+// 1 / l by the hardware (one unit in the last place of 32 bits).
+__device__ __forceinline__ float inverse(float l) { return __builtin_amdgcn_rcpf(l); }
 
 // A row's state once it is whole: its lse, and what attn_weights needs of it.
 __device__ __forceinline__ void finish_row(const AttnOpArgs &a, size_t id, bool empty, float offset, float l)
@@ -310,7 +365,7 @@ __device__ __forceinline__ void finish_row(const AttnOpArgs &a, size_t id, bool 
     if (a.r.lse)
         a.r.lse[id] = empty ? -INFINITY : (offset + log2f(l)) * 0.6931471805599453f;
     if (a.stats)
-        a.stats[id] = empty ? make_float2(0.f, 0.f) : make_float2(offset, 1.0f / l);
+        a.stats[id] = empty ? make_float2(0.f, 0.f) : make_float2(offset, inverse(l));
 }
 
 // ------------------------------------------------------------------ rows that see the same slots
@@ -329,26 +384,37 @@ template <typename TQ, int D, int RT, int NW> __device__ __forceinline__ void at
     __shared__ __attribute__((aligned(16))) uint8_t smem[SMEM];
     __shared__ float2 sml[NW][ROWS];
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4;
-    const uint32_t kh = blockIdx.x % a.own.kv_heads, G = a.r.heads / a.own.kv_heads;
+    const uint32_t kh = blockIdx.x % a.own.kv_heads, G = a.group;
     uint32_t item = blockIdx.x / a.own.kv_heads;
     const uint32_t prefix_items = a.prefix_groups * a.prefix_splits;
     const bool pre = item < prefix_items;
-    // rows: pair i of the group is (row0 + (i0 + i) / G, head kh G + (i0 + i) % G)
-    uint32_t group, part, parts, row0, total;
+    uint32_t group = 0, part, parts, row0, total;
     const uint16_t *kp, *vp;
     int64_t ts;
     Blocks<32> bl;
     if (pre) {
-        group = item % a.prefix_groups, part = item / a.prefix_groups, parts = a.prefix_splits;
+        part = item;
+        if (a.prefix_groups > 1) {
+            part = item / a.prefix_groups;
+            group = item - part * a.prefix_groups;
+        }
+        parts = a.prefix_splits;
         row0 = 0, total = a.r.n_rows * G;
         bl.set(0, clamp_len(a.prefix, 0) - 1, 0, 0);
         const int64_t at = (int64_t)kh * a.prefix.hs;
         kp = a.prefix.k + at, vp = a.prefix.v + at, ts = a.prefix.ts;
     } else {
         item -= prefix_items;
-        group = item % a.own_groups, item /= a.own_groups;
-        part = item % a.own_splits, parts = a.own_splits;
-        row0 = item / a.own_splits, total = G;
+        if (a.own_groups > 1) {
+            const uint32_t q = item / a.own_groups;
+            group = item - q * a.own_groups, item = q;
+        }
+        row0 = item, part = 0, parts = a.own_splits;
+        if (parts > 1) {
+            row0 = item / parts;
+            part = item - row0 * parts;
+        }
+        total = G;
         const int32_t pos = clamp_len(a.own, row0) - 1;
         bl.set(pos, pos, a.window, a.sinks);
         const int64_t at = (int64_t)row0 * a.own.ss + (int64_t)kh * a.own.hs;
@@ -357,16 +423,9 @@ template <typename TQ, int D, int RT, int NW> __device__ __forceinline__ void at
     const uint32_t i0 = group * ROWS;
     uint32_t b0, b1;
     share(bl.count, part, parts, &b0, &b1);
-    const uint32_t tiles = (min(ROWS, total - i0) + 15) / 16;
+    const uint32_t rows = min(ROWS, total - i0);
+    const Pairs pairs(row0, i0, G);
 
-    Queries<TQ, D, RT> Q;
-    State<TQ, D, RT> S;
-    S.clear();
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const uint32_t i = i0 + 16 * t + (lane & 15);
-        load_row<TQ, D, RT>(Q, t, a.r, i < total, row0 + i / G, kh * G + i % G);
-    }
     uint8_t *const vt = smem + wave * V_BYTES;
     const uint32_t at = v_lane<D>(lane);
     vec kr[2][D / 32];
@@ -389,21 +448,31 @@ template <typename TQ, int D, int RT, int NW> __device__ __forceinline__ void at
     uint32_t b = b0 + wave;
     if (b < b1)
         load(bl.block(b));
-    for (; b < b1; b += NW) {
-        const uint32_t blk = bl.block(b);
-        const bool whole = bl.whole(blk);
-        // V to shared memory; slots that are not seen become zeros, whatever they hold
+    Queries<TQ, D, RT> Q;
+    State<TQ, D, RT> S;
+    S.clear();
 #pragma unroll
-        for (int i = 0; i < VL; ++i) {
-            const uint32_t row = (i * 64 + lane) / PIECES;
-            if (!whole && !bl.seen(blk * 32 + row))
-                vr[i] = make_uint4(0, 0, 0, 0);
-            *(uint4 *)(vt + v_piece<D>(row, lane % PIECES) * 16) = vr[i];
-        }
-        floatx4 s[RT][2];
+    for (int t = 0; t < RT; ++t) {
+        const uint32_t x = 16 * t + (lane & 15);
+        load_row<TQ, D, RT>(Q, t, a.r, x < rows, pairs.row_of(x), kh * G + pairs.head_of(x));
+    }
+    // NT: the row tiles in use (all, or the first)
+    auto stream = [&](auto nt) {
+        constexpr int NT = decltype(nt)::value;
+        for (; b < b1; b += NW) {
+            const uint32_t blk = bl.block(b);
+            const bool whole = bl.whole(blk);
+            // V to shared memory; slots that are not seen become zeros, whatever they hold
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
-            if (t < (int)tiles) {
+            for (int i = 0; i < VL; ++i) {
+                const uint32_t row = (i * 64 + lane) / PIECES;
+                if (!whole && !bl.seen(blk * 32 + row))
+                    vr[i] = make_uint4(0, 0, 0, 0);
+                *(uint4 *)(vt + v_piece<D>(row, lane % PIECES) * 16) = vr[i];
+            }
+            floatx4 s[RT][2];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     s[t][u] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -413,54 +482,55 @@ template <typename TQ, int D, int RT, int NW> __device__ __forceinline__ void at
                         for (int x = 0; x < TQ::parts; ++x)
                             s[t][u] = mma(kr[u][i], Q.q[t][x][i], s[t][u]);
                 }
+            if (b + NW < b1)
+                load(bl.block(b + NW));
+            if (a.scores && !pre) { // uniform
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    if (16 * t + (lane & 15) < rows)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const uint32_t j = blk * 32 + 16 * u + 4 * g;
+                            float *to = a.scores +
+                                        ((size_t)row0 * a.r.heads + kh * G + i0 + 16 * t + (lane & 15)) * a.own.slots + j;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (j + e < bl.hi) {
+                                    if constexpr (TQ::parts == 2)
+                                        to[e] = s[t][u][e] * Q.back[t];
+                                    else
+                                        to[e] = s[t][u][e];
+                                }
+                        }
             }
-        if (b + NW < b1)
-            load(bl.block(b + NW));
-        if (a.scores && !pre) { // uniform
-            const uint32_t i = i0 + (lane & 15);
+            if (!whole) {
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
-                if (i + 16 * t < total)
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t j = blk * 32 + 16 * u + 4 * g;
-                        float *to = a.scores + ((size_t)row0 * a.r.heads + kh * G + i + 16 * t) * a.own.slots + j;
+                    for (int e = 0; e < 4; ++e) {
+                        const bool seen = bl.seen(blk * 32 + 16 * u + 4 * g + e);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (j + e < bl.hi) {
-                                if constexpr (TQ::parts == 2)
-                                    to[e] = s[t][u][e] * Q.back[t];
-                                else
-                                    to[e] = s[t][u][e];
-                            }
+                        for (int t = 0; t < NT; ++t)
+                            s[t][u][e] = seen ? s[t][u][e] : -INFINITY;
                     }
-        }
-        if (!whole) {
+            }
+            vec p[RT][TQ::parts];
+            weigh<NT>(S, s, Q, p);
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int n = 0; n < D / 16; ++n) {
+                const vec v = v_operand<TQ, D>(vt, at, n);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (!bl.seen(blk * 32 + 16 * u + 4 * g + e))
-#pragma unroll
-                        for (int t = 0; t < RT; ++t)
-                            s[t][u][e] = -INFINITY;
-        }
-        vec p[RT][TQ::parts];
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-            if (t < (int)tiles)
-                weigh<TQ, D, RT>(S, t, s[t], Q.c[TQ::parts == 2 ? t : 0], p[t]);
-#pragma unroll
-        for (int n = 0; n < D / 16; ++n) {
-            const vec v = v_operand<TQ, D>(vt, at, n);
-#pragma unroll
-            for (int t = 0; t < RT; ++t)
-                if (t < (int)tiles)
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int x = 0; x < TQ::parts; ++x)
                         S.o[t][n] = mma(v, p[t][x], S.o[t][n]);
+            }
         }
-    }
+    };
+    if (RT == 1 || rows <= 16)
+        stream(Const<1>());
+    else
+        stream(Const<RT>());
     // join the waves: offsets and sums first, then the outputs at the common offset
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -473,11 +543,12 @@ template <typename TQ, int D, int RT, int NW> __device__ __forceinline__ void at
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         float top = -INFINITY;
+#pragma unroll
         for (int w = 0; w < NW; ++w)
             top = fmaxf(top, sml[w][16 * t + (lane & 15)].x);
         const float f = S.m[t] > -INFINITY ? exp2_hw(S.mc[t] - top) : 0.f;
         float *to = so + ((size_t)wave * ROWS + 16 * t + (lane & 15)) * D + 4 * g;
-        if (i0 + 16 * t + (lane & 15) < total)
+        if (16 * t + (lane & 15) < rows)
 #pragma unroll
             for (int n = 0; n < D / 16; ++n)
                 *(floatx4 *)(to + 16 * n) = S.o[t][n] * f;
@@ -485,69 +556,104 @@ template <typename TQ, int D, int RT, int NW> __device__ __forceinline__ void at
     __syncthreads();
     const bool final = !a.scores && a.own_splits + a.prefix_splits == 1;
     constexpr uint32_t QD = D / 4;
-    for (uint32_t x = tid; x < min(ROWS, total - i0) * QD; x += NW * 64) {
+    for (uint32_t x = tid; x < rows * QD; x += NW * 64) {
         const uint32_t i = x / QD, d = (x % QD) * 4;
         float top = -INFINITY, l = 0.f;
+#pragma unroll
         for (int w = 0; w < NW; ++w)
             top = fmaxf(top, sml[w][i].x);
         floatx4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
         for (int w = 0; w < NW; ++w) {
             const float2 e = sml[w][i];
             l += e.x > -INFINITY ? e.y * exp2_hw(e.x - top) : e.y;
             o += *(const floatx4 *)(so + ((size_t)w * ROWS + i) * D + d);
         }
-        const uint32_t row = row0 + (i0 + i) / G, h = kh * G + (i0 + i) % G;
+        const uint32_t row = pairs.row_of(i), h = kh * G + pairs.head_of(i);
         if (final) {
             const bool empty = bl.hi == 0;
-            store_out<TQ>(a.r, row, h, d, empty ? o : o / l);
+            store_out<TQ>(a.r, row, h, d, empty ? o : o * inverse(l));
             if (d == 0)
                 finish_row(a, (size_t)row * a.r.heads + h, empty, top, l);
         } else {
-            const size_t at2 = ((size_t)(pre ? a.own_splits + part : part) * a.r.n_rows + row) * a.r.heads + h;
-            *(floatx4 *)(a.o + at2 * D + d) = o;
+            const size_t to = ((size_t)(pre ? a.own_splits + part : part) * a.r.n_rows + row) * a.r.heads + h;
+            *(floatx4 *)(a.o + to * D + d) = o;
             if (d == 0)
-                a.ml[at2] = make_float2(top, l);
+                a.ml[to] = make_float2(top, l);
         }
     }
+}
+
+// The key ranges (64 at most) of one row and head, joined by a wave: the common offset and
+// the sum, the same in every lane, and the lane's D / 64 dims of the output before its
+// division by the sum.  Lane s holds range s's state; eight ranges' outputs are loaded
+// before the first is used.
+template <int D>
+__device__ __forceinline__ void join(const AttnOpArgs &a, uint32_t id, uint32_t n, bool outputs, float *top, float *sum,
+                                     float (&o)[D / 64])
+{
+    constexpr int E = D / 64;
+    const uint32_t lane = threadIdx.x & 63, pairs = a.r.n_rows * a.r.heads;
+    float2 e = make_float2(-INFINITY, 0.f);
+    if (lane < n)
+        e = a.ml[(size_t)lane * pairs + id];
+    *top = wave_max(e.x);
+    const float f = e.x > -INFINITY ? exp2_hw(e.x - *top) : 0.f;
+    // a range without a number adds its sum (0, or NaN from its scores) as it is
+    *sum = wave_sum(e.x > -INFINITY ? e.y * f : e.y);
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        o[i] = 0.f;
+    if (!outputs)
+        return;
+    for (uint32_t s0 = 0; s0 < n; s0 += 8) {
+        float x[8][E];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                x[j][i] = a.o[((size_t)min(s0 + j, n - 1) * pairs + id) * D + lane * E + i];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float w = lane_f32(f, min(s0 + j, 63u));
+            if (s0 + j < n && w > 0.f)
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    o[i] += w * x[j][i];
+        }
+    }
+}
+
+template <typename TQ, int D>
+__device__ __forceinline__ void store_row(const AttnOpArgs &a, uint32_t row, uint32_t h, bool empty, float top, float sum,
+                                          const float (&o)[D / 64])
+{
+    constexpr int E = D / 64;
+    const uint32_t lane = threadIdx.x & 63;
+    typedef typename TQ::type tq;
+    tq *to = (tq *)a.r.out + (int64_t)row * a.r.o_rs + (int64_t)h * a.r.o_hs + lane * E;
+    const float f = inverse(sum);
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        to[i] = (tq)(empty ? 0.f : o[i] * f);
+    if (lane == 0)
+        finish_row(a, (size_t)row * a.r.heads + h, empty, top, sum);
 }
 
 // Joins the key ranges of a row and head: a wave each.
 template <typename TQ, int D> __device__ __forceinline__ void attn_merge(const AttnOpArgs &a)
 {
-    const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const uint32_t pairs = a.r.n_rows * a.r.heads;
-    if (id >= pairs)
+    const uint32_t id = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (id >= a.r.n_rows * a.r.heads)
         return;
-    const uint32_t row = id / a.r.heads, h = id % a.r.heads, n = a.own_splits + a.prefix_splits;
+    const uint32_t row = id / a.r.heads, h = id - row * a.r.heads;
     uint32_t b;
     int32_t pos;
     if (!find_row(a, row, &b, &pos))
         return;
-    float top = -INFINITY;
-    for (uint32_t s = lane; s < n; s += 64)
-        top = fmaxf(top, a.ml[(size_t)s * pairs + id].x);
-    top = wave_max(top);
-    constexpr int E = D / 64;
-    float l = 0.f, o[E] = {};
-    for (uint32_t s = 0; s < n; ++s) {
-        const float2 e = a.ml[(size_t)s * pairs + id];
-        const float f = e.x > -INFINITY ? exp2_hw(e.x - top) : 0.f;
-        // a range without a number adds its sum (0, or NaN from its scores) as it is
-        l += e.x > -INFINITY ? e.y * f : e.y;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float x = a.o[((size_t)s * pairs + id) * D + lane * E + i];
-            o[i] += e.x > -INFINITY ? x * f : 0.f;
-        }
-    }
-    const bool empty = pos < 0 && (!a.prefix.k || clamp_len(a.prefix, 0) == 0);
-    typedef typename TQ::type tq;
-    tq *to = (tq *)a.r.out + (int64_t)row * a.r.o_rs + (int64_t)h * a.r.o_hs + lane * E;
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-        to[i] = (tq)(empty ? 0.f : o[i] / l);
-    if (lane == 0)
-        finish_row(a, id, empty, top, l);
+    float top, sum, o[D / 64];
+    join<D>(a, id, a.own_splits + a.prefix_splits, true, &top, &sum, o);
+    store_row<TQ, D>(a, row, h, pos < 0 && (!a.prefix.k || clamp_len(a.prefix, 0) == 0), top, sum, o);
 }
 
 #define SCORED_SLOTS 512
@@ -557,52 +663,33 @@ template <typename TQ, int D> __device__ __forceinline__ void attn_merge(const A
 // query heads, where reading K again would be 128 or 256.
 template <typename TQ, int D> __device__ __forceinline__ void scored_join(const AttnOpArgs &a)
 {
-    const uint32_t chunk = blockIdx.x, kh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, wave = tid >> 6,
-                   lane = tid & 63;
-    const uint32_t G = a.r.heads / a.own.kv_heads, n = (uint32_t)clamp_len(a.own, b), pairs = a.r.n_rows * a.r.heads;
+    const uint32_t chunk = blockIdx.x, kh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x,
+                   wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const uint32_t G = a.group, n = (uint32_t)clamp_len(a.own, b);
     if (chunk && chunk * SCORED_SLOTS >= n)
         return;
     __shared__ float2 st[MAX_GROUP]; // offset and 1 / sum
+    // the outputs of the G heads are spread over the workgroups in use
+    const uint32_t chunks = max(1u, (n + SCORED_SLOTS - 1) / SCORED_SLOTS);
     for (uint32_t g = wave; g < G; g += 4) {
-        const uint32_t id = b * a.r.heads + kh * G + g;
-        float top = -INFINITY;
-        for (uint32_t s = lane; s < a.own_splits; s += 64)
-            top = fmaxf(top, a.ml[(size_t)s * pairs + id].x);
-        top = wave_max(top);
-        float l = 0.f;
-        for (uint32_t s = 0; s < a.own_splits; ++s) { // in order: the sum every other form of it has
-            const float2 e = a.ml[(size_t)s * pairs + id];
-            l += e.x > -INFINITY ? e.y * exp2_hw(e.x - top) : e.y;
-        }
+        const bool mine = chunk == g % chunks;
+        float top, sum, o[D / 64];
+        join<D>(a, b * a.r.heads + kh * G + g, a.own_splits, mine, &top, &sum, o);
         if (lane == 0)
-            st[g] = make_float2(top, 1.0f / l);
-        if (chunk == 0) {
-            constexpr int E = D / 64;
-            float o[E] = {};
-            for (uint32_t s = 0; s < a.own_splits; ++s) {
-                const float x = a.ml[(size_t)s * pairs + id].x;
-                const float f = x > -INFINITY ? exp2_hw(x - top) : 0.f;
-#pragma unroll
-                for (int i = 0; i < E; ++i)
-                    o[i] += x > -INFINITY ? f * a.o[((size_t)s * pairs + id) * D + lane * E + i] : 0.f;
-            }
-            typedef typename TQ::type tq;
-            tq *to = (tq *)a.r.out + (int64_t)b * a.r.o_rs + (int64_t)(kh * G + g) * a.r.o_hs + lane * E;
-#pragma unroll
-            for (int i = 0; i < E; ++i)
-                to[i] = (tq)(n == 0 ? 0.f : o[i] / l);
-            if (lane == 0)
-                finish_row(a, id, n == 0, top, l);
-        }
+            st[g] = make_float2(top, inverse(sum));
+        if (mine)
+            store_row<TQ, D>(a, b, kh * G + g, n == 0, top, sum, o);
     }
     __syncthreads();
     for (uint32_t j = chunk * SCORED_SLOTS + tid; j < min(n, (chunk + 1) * SCORED_SLOTS); j += 256) {
         const float *s = a.scores + ((size_t)b * a.r.heads + kh * G) * a.own.slots + j;
+        const size_t at = ((size_t)b * a.own.kv_heads + kh) * a.own.slots + j;
+        const float had = a.acc ? a.acc[at] : 0.f;
         float sum = 0.f;
+#pragma unroll 4
         for (uint32_t g = 0; g < G; ++g)
             sum += exp2_hw(fmaf(s[(size_t)g * a.own.slots], a.r.cexp, -st[g].x)) * st[g].y;
-        const size_t at = ((size_t)b * a.own.kv_heads + kh) * a.own.slots + j;
-        a.acc_out[at] = (a.acc ? a.acc[at] : 0.f) + sum;
+        a.acc_out[at] = had + sum;
     }
 }
 
@@ -670,10 +757,10 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
     __shared__ float pw[4][16][33]; // one row tile's weights of 32 slots, a wave each
     __shared__ uint64_t odd[4];     // slots of a block whose V is not all finite
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4;
-    const uint32_t kh = blockIdx.x % a.own.kv_heads, G = a.r.heads / a.own.kv_heads;
-    const uint32_t flat = blockIdx.x / a.own.kv_heads, split = flat % a.own_splits;
+    const uint32_t kh = blockIdx.x % a.own.kv_heads, G = a.group;
+    const uint32_t flat = blockIdx.x / a.own.kv_heads, split = a.own_splits == 1 ? 0 : flat % a.own_splits;
     uint32_t b, tile, tiles;
-    if (!find_item(a.r, a.own.n_seq, flat / a.own_splits, G, ROWS, &b, &tile, &tiles))
+    if (!find_item(a.r, a.own.n_seq, a.own_splits == 1 ? flat : flat / a.own_splits, G, ROWS, &b, &tile, &tiles))
         return;
     tile = tiles - 1 - tile; // the longest first
     int32_t lo, hi;
@@ -691,11 +778,13 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
     S.clear();
     int32_t pos[RT];
     const uint32_t w0 = p0 + wave * 16 * RT;
+    const Pairs pairs((uint32_t)lo, w0, G);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        const uint32_t i = w0 + 16 * t + (lane & 15);
-        load_row<TQ, D, RT>(Q, t, a.r, i < total, (uint32_t)lo + i / G, kh * G + i % G);
-        pos[t] = i < total ? first + (int32_t)(i / G) : -1;
+        const uint32_t x = 16 * t + (lane & 15), row = pairs.row_of(x);
+        const bool in = w0 + x < total;
+        load_row<TQ, D, RT>(Q, t, a.r, in, row, kh * G + pairs.head_of(x));
+        pos[t] = in ? first + (int32_t)row - lo : -1;
     }
     // what this wave's rows see: some row of it, every row of it
     const bool any_row = w0 < total;
@@ -766,32 +855,35 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
             uint32_t wrong = 0;
             if (!whole)
                 wrong = __builtin_amdgcn_readfirstlane((uint32_t)(odd[i & 3] >> (32 * sub)));
+            floatx4 s[RT][2];
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                floatx4 s[2];
+            for (int t = 0; t < RT; ++t)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    s[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+                    s[t][u] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int x = 0; x < D / 32; ++x)
 #pragma unroll
                         for (int y = 0; y < TQ::parts; ++y)
-                            s[u] = mma(k[u][x], Q.q[t][y][x], s[u]);
+                            s[t][u] = mma(k[u][x], Q.q[t][y][x], s[t][u]);
                 }
-                if (!whole) {
-                    // row at pos sees j <= pos, and j < sinks or j > pos - window
-                    const int32_t from = a.window && (uint32_t)max(pos[t], 0) >= a.window ? pos[t] - (int32_t)a.window : -1;
+            if (!whole) {
+                // row at pos sees j <= pos, and j < sinks or j > pos - window
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    const int32_t from =
+                        a.window && (uint32_t)max(pos[t], 0) >= a.window ? pos[t] - (int32_t)a.window : -1;
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int32_t j = (int32_t)j0 + 16 * u + 4 * g + e;
-                            if (j > pos[t] || (j <= from && (uint32_t)j >= a.sinks))
-                                s[u][e] = -INFINITY;
+                            const bool hidden = (j > pos[t]) | ((j <= from) & ((uint32_t)j >= a.sinks));
+                            s[t][u][e] = hidden ? -INFINITY : s[t][u][e];
                         }
                 }
-                weigh<TQ, D, RT>(S, t, s, Q.c[TQ::parts == 2 ? t : 0], p[t]);
             }
+            weigh<RT>(S, s, Q, p);
             if (wrong) { // uniform; rare
 #pragma unroll
                 for (int t = 0; t < RT; ++t) {
@@ -844,14 +936,14 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const float l = row_sum(S.l[t]);
-        const uint32_t i = w0 + 16 * t + (lane & 15);
-        if (i >= total)
+        const uint32_t x = 16 * t + (lane & 15);
+        if (w0 + x >= total)
             continue;
-        const uint32_t row = (uint32_t)lo + i / G, h = kh * G + i % G;
+        const uint32_t row = pairs.row_of(x), h = kh * G + pairs.head_of(x);
         const float off = S.m[t] > -INFINITY ? S.mc[t] : -INFINITY;
         if (final) {
             const bool empty = pos[t] < 0;
-            const float f = empty ? 0.f : 1.0f / l;
+            const float f = empty ? 0.f : inverse(l);
 #pragma unroll
             for (int n = 0; n < D / 16; ++n)
                 store_out<TQ>(a.r, row, h, 16 * n + 4 * g, S.o[t][n] * f);
@@ -871,17 +963,18 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
 #define SUM_KEYS 64
 #define SUM_WAVES 8
 // The weights that SUM_KEYS slots of one (sequence, kv head) receive from all rows: scores
-// once more, with the slots as B operands in registers and 16 (token, head) pairs at a time
-// as A operands, a wave every SUM_WAVES-th; a weight is 2^(s c - offset) / sum with its row's
-// softmax state.  A lane adds its slots' weights over its rows; the lanes' and the waves' sums
-// are joined in a fixed order.
+// once more, with the slots as A operands in registers and 16 (token, head) pairs at a time
+// as B operands, a wave every SUM_WAVES-th, the next pairs' loads in flight.  A lane's scores
+// are of one row (its softmax state: offset and 1 / sum) and four slots a tile; it adds its
+// slots' weights 2^(s c - offset) / sum over its rows.  The lanes' and the waves' sums are
+// joined in a fixed order.
 template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const AttnOpArgs &a)
 {
     typedef typename TQ::vec vec;
     constexpr int KT = SUM_KEYS / 16;
     __shared__ float part[SUM_WAVES][SUM_KEYS];
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4;
-    const uint32_t kh = blockIdx.y, b = blockIdx.z, G = a.r.heads / a.own.kv_heads;
+    const uint32_t kh = blockIdx.y, b = blockIdx.z, G = a.group;
     const uint32_t n = (uint32_t)clamp_len(a.own, b), j0 = blockIdx.x * SUM_KEYS;
     if (j0 >= n)
         return;
@@ -898,26 +991,31 @@ template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const
         for (int x = 0; x < D / 32; ++x)
             k[t][x] = *(const vec *)(p + 32 * x);
     }
-    float sum[KT] = {};
+    floatx4 sum[KT] = {};
+    struct Next {
+        Queries<TQ, D, 1> q;
+        float2 st;
+        int32_t pos;
+    };
+    auto load = [&](uint32_t i0, Next &x) {
+        const Pairs pairs((uint32_t)lo, i0 * 16, G);
+        const bool in = i0 * 16 + (lane & 15) < total;
+        const uint32_t row = pairs.row_of(lane & 15), h = kh * G + pairs.head_of(lane & 15);
+        load_row<TQ, D, 1>(x.q, 0, a.r, in, row, h);
+        x.st = in ? a.stats[(size_t)row * a.r.heads + h] : make_float2(0.f, 0.f);
+        x.pos = in ? first + (int32_t)row - lo : -1;
+    };
     // pairs before the first that sees slot j0 add nothing
-    const uint32_t from = (int32_t)j0 > first ? ((j0 - first) * G) / 16 : 0;
-    for (uint32_t i0 = from + wave; i0 * 16 < total; i0 += SUM_WAVES) {
-        Queries<TQ, D, 1> Q;
-        const uint32_t i = i0 * 16 + (lane & 15);
-        load_row<TQ, D, 1>(Q, 0, a.r, i < total, (uint32_t)lo + i / G, kh * G + i % G);
-        // the lane's four rows of the result: 4 g + e
-        float off[4], inv[4], c[4];
-        int32_t pos[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t r = i0 * 16 + 4 * g + e;
-            const bool in = r < total;
-            const float2 st = in ? a.stats[((size_t)lo + r / G) * a.r.heads + kh * G + r % G] : make_float2(0.f, 0.f);
-            off[e] = st.x, inv[e] = st.y;
-            pos[e] = in ? first + (int32_t)(r / G) : -1;
-            c[e] = TQ::parts == 2 ? __shfl(Q.c[0], 4 * g + e) : Q.c[0];
-        }
-        const bool whole = first + (int32_t)(i0 * 16 / G) >= (int32_t)(j0 + SUM_KEYS - 1) && i0 * 16 + 16 <= total;
+    const uint32_t from = (int32_t)j0 > first ? ((j0 - first) * G) / 16 : 0, end = (total + 15) / 16;
+    Next cur, nxt;
+    uint32_t i0 = from + wave;
+    if (i0 < end)
+        load(i0, nxt);
+    for (; i0 < end; i0 += SUM_WAVES) {
+        cur = nxt;
+        if (i0 + SUM_WAVES < end)
+            load(i0 + SUM_WAVES, nxt);
+        const bool whole = __ballot(cur.pos < (int32_t)(j0 + SUM_KEYS - 1)) == 0;
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
             floatx4 s = {0.f, 0.f, 0.f, 0.f};
@@ -925,20 +1023,31 @@ template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const
             for (int x = 0; x < D / 32; ++x)
 #pragma unroll
                 for (int y = 0; y < TQ::parts; ++y)
-                    s = mma(Q.q[0][y][x], k[t][x], s);
+                    s = mma(k[t][x], cur.q.q[0][y][x], s);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float w = exp2_hw(fmaf(s[e], c[e], -off[e])) * inv[e];
-                sum[t] += whole || (int32_t)(j0 + 16 * t + (lane & 15)) <= pos[e] ? w : 0.f;
+                const float w = exp2_hw(fmaf(s[e], cur.q.c[0], -cur.st.x));
+                const float to = fmaf(w, cur.st.y, sum[t][e]);
+                if (whole)
+                    sum[t][e] = to;
+                else // a row's NaN stays with the slots it sees
+                    sum[t][e] = (int32_t)(j0 + 16 * t + 4 * g + e) <= cur.pos ? to : sum[t][e];
             }
         }
     }
+    // the 16 lanes of a slot's row are its rows' sums
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-        const float v = row_sum(sum[t]);
-        if (lane < 16)
-            part[wave][16 * t + lane] = v;
-    }
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float v = sum[t][e];
+            v += dpp_mov<0xb1>(v, 0.f);  // quad_perm [1,0,3,2]
+            v += dpp_mov<0x4e>(v, 0.f);  // quad_perm [2,3,0,1]
+            v += dpp_mov<0x114>(v, 0.f); // row_shr:4
+            v += dpp_mov<0x118>(v, 0.f); // row_shr:8: the row's sum in lane 15 of 16
+            if ((lane & 15) == 15)
+                part[wave][16 * t + 4 * g + e] = v;
+        }
     __syncthreads();
     if (tid < SUM_KEYS && j0 + tid < n) {
         float v = 0.f;
@@ -952,7 +1061,7 @@ template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const
 // RT: row tiles of a workgroup of rows that see the same slots, as many as the registers
 // hold beside the next block's K and V.
 #define STEP(TQ, tag, D, RT, NW)                                                                               \
-    extern "C" __global__ __launch_bounds__(NW * 64) void k_attn_step_##tag##_##D##_r##RT##w##NW(              \
+    extern "C" __global__ __launch_bounds__(NW * 64, RT == 1 ? NW / 4 : 2) void k_attn_step_##tag##_##D##_r##RT##w##NW( \
         const AttnOpArgs a)                                                                                    \
     {                                                                                                          \
         attn_step<TQ, D, RT, NW>(a);                                                                           \
@@ -1008,9 +1117,11 @@ __device__ __forceinline__ uint32_t evict_key(const EvictArgs &a, float acc, int
 }
 
 #define SEL_THREADS 1024
-// The `keep` slots of highest rank of one (sequence, kv head), ties to the lowest slot:
-// the rank of the last one by four 8-bit histograms from the top, then each wave counts
-// and places its own run of slots.
+#define SEL_HELD 32768 // slots whose ranks are held in shared memory; further ones are made again
+#define SEL_COPIES 16  // of each histogram, by lane: ranks share their upper bits
+// The `keep` slots of highest rank of one (sequence, kv head), ties to the lowest slot: the
+// rank of the last one by 8-bit histograms from the top (as many as it takes until a bin is
+// taken whole), then each wave counts and places its own run of slots.
 extern "C" __global__ __launch_bounds__(SEL_THREADS) void k_kv_select(const EvictArgs a)
 {
     const uint32_t kh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -1025,65 +1136,112 @@ extern "C" __global__ __launch_bounds__(SEL_THREADS) void k_kv_select(const Evic
     const float *acc = a.acc + bh * a.c.slots;
     const int32_t *pos = a.pos + bh * a.c.slots;
     int32_t *map = a.map + bh * keep, *movers = a.movers + bh * keep;
-    __shared__ uint32_t hist[256];
+    __shared__ uint32_t held[SEL_HELD];
+    __shared__ __attribute__((aligned(16))) uint32_t hist[256 * SEL_COPIES], bins[256];
     __shared__ int32_t wmax[16];
-    __shared__ uint32_t sh_prefix, sh_need, cnt_eq[16], cnt_hole[16], cnt_move[16];
+    __shared__ uint32_t cnt_eq[16], cnt_hole[16], cnt_move[16];
+    // positions first (their maximum), the first ranks' weights loaded beside them
+    constexpr int EARLY = 8;
+    float early[EARLY];
     int32_t newest = INT32_MIN;
-    for (uint32_t j = tid; j < n; j += SEL_THREADS)
-        newest = max(newest, pos[j]);
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i) {
+        const uint32_t j = min(tid + i * SEL_THREADS, n - 1);
+        early[i] = acc[j];
+        const int32_t p = pos[j];
+        newest = max(newest, p);
+        held[tid + i * SEL_THREADS] = (uint32_t)p;
+    }
+    for (uint32_t j = tid + EARLY * SEL_THREADS; j < n; j += SEL_THREADS) {
+        const int32_t p = pos[j];
+        newest = max(newest, p);
+        if (j < SEL_HELD)
+            held[j] = (uint32_t)p;
+    }
     newest = wave_max_i(newest);
     if (lane == 0)
         wmax[wave] = newest;
-    if (tid == 0)
-        sh_prefix = 0, sh_need = keep;
     __syncthreads();
+#pragma unroll
     for (int w = 0; w < 16; ++w)
         newest = max(newest, wmax[w]);
-    for (int pass = 3; pass >= 0; --pass) {
-        if (tid < 256)
-            hist[tid] = 0;
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i) // each thread its own slots: no barrier between
+        held[tid + i * SEL_THREADS] = evict_key(a, early[i], (int32_t)held[tid + i * SEL_THREADS], newest);
+    for (uint32_t j = tid + EARLY * SEL_THREADS; j < min(n, (uint32_t)SEL_HELD); j += SEL_THREADS)
+        held[j] = evict_key(a, acc[j], (int32_t)held[j], newest);
+    auto rank = [&](uint32_t j) { return j < SEL_HELD ? held[j] : evict_key(a, acc[j], pos[j], newest); };
+    uint32_t last = 0, mask = 0, need = keep; // kept: rank & mask above `last`, and `need` of those at it
+    bool exact = false;
+    for (int pass = 3; pass >= 0 && !exact; --pass) {
+        for (uint32_t i = tid; i < 256 * SEL_COPIES / 4; i += SEL_THREADS)
+            ((uint4 *)hist)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        const uint32_t prefix = sh_prefix, mask = pass == 3 ? 0u : 0xFFFFFFFFu << (8 * (pass + 1));
         for (uint32_t j = tid; j < n; j += SEL_THREADS) {
-            const uint32_t k = evict_key(a, acc[j], pos[j], newest);
-            if ((k & mask) == prefix)
-                atomicAdd(&hist[(k >> (8 * pass)) & 255], 1u);
+            const uint32_t k = rank(j);
+            if ((k & mask) == last)
+                atomicAdd(&hist[((k >> (8 * pass)) & 255) * SEL_COPIES + (lane & (SEL_COPIES - 1))], 1u);
         }
         __syncthreads();
-        if (tid == 0) {
-            uint32_t need = sh_need;
-            int d = 255;
-            for (; d > 0 && hist[d] < need; --d)
-                need -= hist[d];
-            sh_prefix = prefix | (uint32_t)d << (8 * pass);
-            sh_need = need;
+        if (tid < 256) {
+            uint32_t v = 0;
+#pragma unroll
+            for (int i = 0; i < SEL_COPIES / 4; ++i) {
+                const uint4 x = ((const uint4 *)hist)[tid * (SEL_COPIES / 4) + i];
+                v += x.x + x.y + x.z + x.w;
+            }
+            bins[tid] = v;
         }
         __syncthreads();
+        // every wave: lane l holds bins 255 - 4 l downwards; the bin where the count from the
+        // top reaches `need`
+        const uint4 x = ((const uint4 *)bins)[63 - lane];
+        const uint32_t four = x.x + x.y + x.z + x.w;
+        uint32_t upto = four;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = __shfl_up(upto, d);
+            upto += lane >= (uint32_t)d ? o : 0;
+        }
+        const uint32_t at = (uint32_t)__ffsll((unsigned long long)__ballot(upto >= need)) - 1;
+        uint32_t left = need - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(four, at));
+        const uint32_t c[4] = {(uint32_t)__builtin_amdgcn_readlane(x.w, at), (uint32_t)__builtin_amdgcn_readlane(x.z, at),
+                               (uint32_t)__builtin_amdgcn_readlane(x.y, at), (uint32_t)__builtin_amdgcn_readlane(x.x, at)};
+        uint32_t bin = 255 - 4 * at, count = c[0];
+#pragma unroll
+        for (int i = 1; i < 4; ++i)
+            if (left > count && bin + i == 256 - 4 * at) { // still passing bins
+                left -= count;
+                count = c[i];
+                --bin;
+            }
+        last |= bin << (8 * pass);
+        mask |= 255u << (8 * pass);
+        need = left;
+        exact = left == count;
     }
-    const uint32_t last = sh_prefix, need = sh_need; // the need lowest slots of rank `last` stay
     const uint32_t run = ((n + 15) / 16 + 63) / 64 * 64, j0 = wave * run, j1 = min(n, j0 + run);
     const uint64_t below = (1ull << lane) - 1;
-    uint32_t eq = 0;
-    for (uint32_t j = j0; j < j1; j += 64) {
-        const bool in = j + lane < j1;
-        const uint32_t k = in ? evict_key(a, acc[j + lane], pos[j + lane], newest) : 0;
-        eq += __popcll(__ballot(in && k == last));
-    }
-    if (lane == 0)
-        cnt_eq[wave] = eq;
-    __syncthreads();
     uint32_t eq0 = 0;
-    for (uint32_t w = 0; w < wave; ++w)
-        eq0 += cnt_eq[w];
+    if (!exact) { // uniform: only some of the slots at the last rank stay, the lowest
+        uint32_t eq = 0;
+        for (uint32_t j = j0; j < j1; j += 64)
+            eq += __popcll(__ballot(j + lane < j1 && (rank(min(j + lane, n - 1)) & mask) == last));
+        if (lane == 0)
+            cnt_eq[wave] = eq;
+        __syncthreads();
+        for (uint32_t w = 0; w < wave; ++w)
+            eq0 += cnt_eq[w];
+    }
     uint32_t holes = 0, moves = 0, hole0 = 0, move0 = 0;
     for (int place = 0; place < 2; ++place) {
         uint32_t e = eq0;
         for (uint32_t j = j0; j < j1; j += 64) {
             const uint32_t s = j + lane;
             const bool in = s < j1;
-            const uint32_t k = in ? evict_key(a, acc[s], pos[s], newest) : 0;
+            const uint32_t k = in ? rank(s) & mask : 0;
             const uint64_t meq = __ballot(in && k == last);
-            const bool kept = in && (k > last || (k == last && e + __popcll(meq & below) < need));
+            const bool kept = in && (k > last || (k == last && (exact || e + __popcll(meq & below) < need)));
             e += __popcll(meq);
             const uint64_t mh = __ballot(in && s < keep && !kept), mm = __ballot(s >= keep && kept);
             if (place) {
