@@ -31,7 +31,7 @@ static uint32_t tile_tiles(uint32_t type, uint32_t dim) { return dim == 64 && ty
 struct AttnKernels {
     hipModule_t mod = nullptr;
     hipFunction_t tile_1[3][2], tile_most[3][2], weights[3][2];
-    hipFunction_t step_1w4[3][2], step_wide[3][2], step_most[3][2], merge[3][2], scored_join[3][2];
+    hipFunction_t step_1[3][2], step_most[3][2], merge[3][2], scored_join[3][2];
     hipFunction_t kv_select, kv_move;
 };
 
@@ -61,9 +61,8 @@ static int load_attn(int dev)
             } fns[] = {{&k.tile_1[t][d], "k_attn_tile" + tag + "_r1"},
                        {&k.tile_most[t][d], "k_attn_tile" + tag + "_r" + std::to_string(tile_tiles(t, d ? 128 : 64))},
                        {&k.weights[t][d], "k_attn_weights" + tag},
-                       {&k.step_1w4[t][d], "k_attn_step" + tag + "_r1w4"},
-                       {&k.step_wide[t][d], "k_attn_step" + tag + (d ? "_r1w8" : "_r1w16")},
-                       {&k.step_most[t][d], "k_attn_step" + tag + "_r" + std::to_string(step_tiles(d ? 128 : 64)) + "w4"},
+                       {&k.step_1[t][d], "k_attn_step" + tag + "_r1"},
+                       {&k.step_most[t][d], "k_attn_step" + tag + "_r" + std::to_string(step_tiles(d ? 128 : 64))},
                        {&k.merge[t][d], "k_attn_merge" + tag},
                        {&k.scored_join[t][d], "k_scored_join" + tag}};
             for (auto &f : fns)
@@ -251,8 +250,8 @@ static int dim_index(const lfm_kv *c) { return c->head_dim == 128; }
 // How a call's work is cut, from sizes alone.
 struct Plan {
     uint32_t own_splits = 1, prefix_splits = 0, own_groups = 1, prefix_groups = 0;
-    bool many_waves = false, most = false; // the step kernel's form
-    bool tile_most = false;                // the tile kernel's
+    bool most = false;      // the step kernel's larger form
+    bool tile_most = false; // the tile kernel's
     uint64_t tile_items = 0;
     bool join = false; // a second kernel joins the key ranges
     size_t ml_bytes = 0, o_bytes = 0, score_bytes = 0, stat_bytes = 0;
@@ -260,7 +259,7 @@ struct Plan {
 };
 
 
-#define TARGET_WAVES 4096 // four to each of 1024 SIMDs
+#define TARGET_GROUPS 512 // workgroups of four waves: two to a CU
 #define MOST_RANGES 32    // key ranges of one kind: 64 lanes join a row's
 
 static uint32_t ranges(uint64_t wanted, uint64_t worth)
@@ -280,12 +279,13 @@ static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint
         const uint64_t blocks = (span + 31) / 32;
         p.own_groups = (G + per - 1) / per;
         const uint64_t items = (uint64_t)std::max(1u, r->n_rows) * p.own_groups * kv->kv_heads;
-        // a wave needs a few blocks for its loads to overlap; below that ranges only add joining
-        p.own_splits = ranges(TARGET_WAVES / 4 / items, blocks / 16);
-        if (!prefix && !p.most && blocks <= 64 && items < 1024) {
-            p.own_splits = 1;
-            p.many_waves = blocks > 4;
-        }
+        // A second launch that joins ranges takes 2-3 us: up to 512 slots one range is faster
+        // (512 slots of one sequence, 64 dims: 5.9 us against 6.8 in four ranges; 1024: 8.5
+        // against 6.8 in eight), where no join follows anyway.  A workgroup's four waves take
+        // a block of 32 each at least, two of a longer cache (4096 slots: 8.3 us in 32 ranges,
+        // 7.8 in 16).
+        if (scored || blocks > 16)
+            p.own_splits = ranges(TARGET_GROUPS / items, blocks / (blocks > 64 ? 8 : 4));
     } else {
         // sequences end inside tiles: at most one more tile each
         const uint64_t cut = (uint64_t)r->n_rows * G;
@@ -295,12 +295,13 @@ static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint
         p.tile_items = cut / rows + std::min<uint64_t>(kv->n_seq, r->n_rows);
         const uint64_t span = window ? std::min<uint64_t>(kv->slots, (uint64_t)window + sinks + rows / G + 128)
                                      : kv->slots;
-        p.own_splits = ranges(512 / std::max<uint64_t>(1, p.tile_items * kv->kv_heads), span / 512);
+        p.own_splits = ranges(TARGET_GROUPS / std::max<uint64_t>(1, p.tile_items * kv->kv_heads), span / 512);
     }
     if (prefix) {
         p.prefix_groups = (uint32_t)(((uint64_t)r->n_rows * G + per - 1) / per);
         const uint64_t pitems = (uint64_t)std::max(1u, p.prefix_groups) * kv->kv_heads;
-        p.prefix_splits = ranges(TARGET_WAVES / 4 / pitems, (prefix->slots + 511) / 512);
+        const uint64_t blocks = (prefix->slots + 31) / 32;
+        p.prefix_splits = ranges(TARGET_GROUPS / pitems, blocks / (blocks > 64 ? 8 : 4));
     }
     const uint32_t splits = p.own_splits + p.prefix_splits;
     const bool steps = scored && !r->start; // scores are kept from the step to the join
@@ -357,8 +358,8 @@ static int attend(AttnKernels *K, const Plan &p, const AttnOpArgs &a, const lfm_
     const uint64_t steps = (uint64_t)p.prefix_groups * p.prefix_splits +
                            (rows->start ? 0 : (uint64_t)rows->n_rows * p.own_groups * p.own_splits);
     if (steps) {
-        hipFunction_t f = p.most ? K->step_most[t][d] : p.many_waves ? K->step_wide[t][d] : K->step_1w4[t][d];
-        RC(launch_items(f, steps, kv->kv_heads, p.many_waves ? (d ? 512 : 1024) : 256, s, a));
+        hipFunction_t f = p.most ? K->step_most[t][d] : K->step_1[t][d];
+        RC(launch_items(f, steps, kv->kv_heads, 256, s, a));
     }
     if (rows->start)
         RC(launch_items(p.tile_most ? K->tile_most[t][d] : K->tile_1[t][d], p.tile_items * p.own_splits, kv->kv_heads,

@@ -155,9 +155,8 @@ struct Pairs {
 template <typename TQ, int D, int RT> struct Queries {
     static constexpr int N = TQ::parts == 2 ? RT : 1;
     typename TQ::vec q[RT][TQ::parts][D / 32];
-    float c[N], slack[N], back[N]; // cexp / power; 8 / c; 1 / power
+    float c[N], back[N]; // cexp / power; 1 / power
     __device__ __forceinline__ float c_of(int t) const { return c[N == 1 ? 0 : t]; }
-    __device__ __forceinline__ float slack_of(int t) const { return slack[N == 1 ? 0 : t]; }
 };
 
 template <typename TQ, int D, int RT>
@@ -176,7 +175,6 @@ __device__ __forceinline__ void load_row(Queries<TQ, D, RT> &Q, int t, const Row
             Q.q[t][0][j] = v;
         }
         Q.c[0] = r.cexp;
-        Q.slack[0] = fminf(8.f / r.cexp, 3.0e38f);
     } else {
         float x[D / 32][8], top = 0.f;
 #pragma unroll
@@ -200,7 +198,6 @@ __device__ __forceinline__ void load_row(Queries<TQ, D, RT> &Q, int t, const Row
         const float s = ldexpf(1.f, up);
         Q.back[t] = ldexpf(1.f, -up);
         Q.c[t] = r.cexp * Q.back[t];
-        Q.slack[t] = fminf(8.f * __builtin_amdgcn_rcpf(Q.c[t]), 3.0e38f);
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
 #pragma unroll
@@ -214,13 +211,12 @@ __device__ __forceinline__ void load_row(Queries<TQ, D, RT> &Q, int t, const Row
 }
 
 // ------------------------------------------------------------------ softmax state
-// Of RT tiles of 16 rows: o[t][n] are dims 16 n + 4 (lane / 16) + e of row lane % 16.  m is
-// the score that weights are taken relative to (units of q . k), mc = m c - offset; l the
+// Of RT tiles of 16 rows: o[t][n] are dims 16 n + 4 (lane / 16) + e of row lane % 16, l the
 // lane's own part of the sum of the weights 2^(s c - mc), whose four parts are added at the
-// end.
+// end.  lim is what s c - mc may reach before mc follows; -inf while no number was seen.
 template <typename TQ, int D, int RT> struct State {
     floatx4 o[RT][D / 16];
-    float m[RT], mc[RT], l[RT];
+    float mc[RT], lim[RT], l[RT];
     __device__ __forceinline__ void clear()
     {
 #pragma unroll
@@ -228,38 +224,55 @@ template <typename TQ, int D, int RT> struct State {
 #pragma unroll
             for (int n = 0; n < D / 16; ++n)
                 o[t][n] = floatx4{0.f, 0.f, 0.f, 0.f};
-            m[t] = -INFINITY, mc[t] = 0.f, l[t] = 0.f;
+            mc[t] = 0.f, lim[t] = -INFINITY, l[t] = 0.f;
         }
     }
+    // for joining: -inf where there is nothing to join
+    __device__ __forceinline__ float offset(int t) const { return lim[t] > -INFINITY ? mc[t] : -INFINITY; }
 };
 
 // Scores of 32 slots and NT row tiles (s[t][0]: slots 4 (lane / 16) + e, s[t][1]: the same +
 // 16) -> weights as B operands: inner place 8 (lane / 16) + i is slot 16 (i / 4) + 4 (lane /
-// 16) + i % 4.  m follows the largest score only when that is 8 binary orders above it, for
-// all the tiles at once: after the first block hardly ever, and a weight stays below 2^15.
+// 16) + i % 4.  The largest weight is 2^offset when mc is set, and mc follows the scores only
+// when one passes it by RISE binary orders, for all the tiles at once: after the first block
+// hardly ever, and a weight stays at or below 2^15.  (The maximum is taken of the scaled
+// scores: of the matrix cores' own results the compiler first makes canonical copies, one
+// more instruction a score.)
+#define RISE 8.f
 template <int NT, typename TQ, int D, int RT>
 __device__ __forceinline__ void weigh(State<TQ, D, RT> &S, const floatx4 (&s)[RT][2], const Queries<TQ, D, RT> &Q,
                                       typename TQ::vec (&p)[RT][TQ::parts])
 {
-    float top[NT];
+    float x[NT][8];
     bool rises = false;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const floatx4 &x = s[t][0], &y = s[t][1];
-        top[t] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
-        rises |= top[t] > S.m[t] + Q.slack_of(t);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            x[t][i] = fmaf(s[t][i / 4][i % 4], Q.c_of(t), -S.mc[t]);
+        const float top = fmaxf(fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])),
+                                fmaxf(fmaxf(x[t][4], x[t][5]), fmaxf(x[t][6], x[t][7])));
+        rises |= top > S.lim[t];
     }
     if (__ballot(rises)) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const float mn = fmaxf(S.m[t], row_max(top[t]));
-            // a row of -inf alone keeps mc 0: its weights are 2^-inf = 0
-            const float mcn = mn > -INFINITY ? mn * Q.c_of(t) - TQ::offset : 0.f;
-            const float r = S.m[t] > -INFINITY ? exp2_hw(S.mc[t] - mcn) : 0.f;
-            S.m[t] = mn, S.mc[t] = mcn, S.l[t] *= r;
+            float top = x[t][0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i)
+                top = fmaxf(top, x[t][i]);
+            top = row_max(top);
+            const bool seen = S.lim[t] > -INFINITY, number = top > -INFINITY;
+            float d = top - TQ::offset;
+            d = seen ? fmaxf(d, 0.f) : number ? d : 0.f; // a row of -inf alone: weights 2^-inf = 0
+            const float r = seen ? exp2_hw(-d) : 1.f;
+            S.mc[t] += d, S.l[t] *= r, S.lim[t] = seen || number ? TQ::offset + RISE : -INFINITY;
 #pragma unroll
             for (int n = 0; n < D / 16; ++n)
                 S.o[t][n] *= r;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                x[t][i] -= d;
         }
     }
     typedef typename TQ::kv kv2 __attribute__((ext_vector_type(2)));
@@ -268,7 +281,7 @@ __device__ __forceinline__ void weigh(State<TQ, D, RT> &S, const floatx4 (&s)[RT
         float w[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            w[i] = exp2_hw(fmaf(s[t][i / 4][i % 4], Q.c_of(t), -S.mc[t]));
+            w[i] = exp2_hw(x[t][i]);
         S.l[t] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
@@ -374,8 +387,9 @@ __device__ __forceinline__ void finish_row(const AttnOpArgs &a, size_t id, bool 
 // blocks of 32 slots in turn, each with a softmax state of its own, joined at the end: a
 // wave streams K straight into A operands and V through a piece of shared memory of its own
 // (the transposed read), the next block's loads in flight, and no wave waits for another.
-template <typename TQ, int D, int RT, int NW> __device__ __forceinline__ void attn_step(const AttnOpArgs &a)
+template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_step(const AttnOpArgs &a)
 {
+    constexpr int NW = 4; // waves
     typedef typename TQ::vec vec;
     constexpr int VL = D / 16;                   // 16-byte loads of V a lane and block
     constexpr uint32_t ROWS = 16 * RT, PIECES = D / 8;
@@ -536,7 +550,7 @@ template <typename TQ, int D, int RT, int NW> __device__ __forceinline__ void at
     for (int t = 0; t < RT; ++t) {
         S.l[t] = row_sum(S.l[t]);
         if (lane < 16)
-            sml[wave][16 * t + lane] = make_float2(S.m[t] > -INFINITY ? S.mc[t] : -INFINITY, S.l[t]);
+            sml[wave][16 * t + lane] = make_float2(S.offset(t), S.l[t]);
     }
     __syncthreads();
     float *const so = (float *)smem; // [wave][row][D]
@@ -546,7 +560,7 @@ template <typename TQ, int D, int RT, int NW> __device__ __forceinline__ void at
 #pragma unroll
         for (int w = 0; w < NW; ++w)
             top = fmaxf(top, sml[w][16 * t + (lane & 15)].x);
-        const float f = S.m[t] > -INFINITY ? exp2_hw(S.mc[t] - top) : 0.f;
+        const float f = S.lim[t] > -INFINITY ? exp2_hw(S.mc[t] - top) : 0.f;
         float *to = so + ((size_t)wave * ROWS + 16 * t + (lane & 15)) * D + 4 * g;
         if (16 * t + (lane & 15) < rows)
 #pragma unroll
@@ -737,6 +751,65 @@ template <typename TQ> __device__ __forceinline__ bool has_nonfinite(uint4 v)
     return bad;
 }
 
+// One row and head over blocks b0 .. b1 of 64 slots, by a wave: a lane's score each, then
+// every lane its dims of the weighted sum, a slot that the row does not see left out whatever
+// it holds.
+template <typename TQ, int D, typename B>
+__device__ void attn_row(const AttnOpArgs &a, const B &bl, uint32_t b0, uint32_t b1, const uint16_t *kp,
+                         const uint16_t *vp, uint32_t row, uint32_t h, int32_t pos, uint32_t split, float *weights)
+{
+    typedef typename TQ::kv tk;
+    constexpr int E = D / 64;
+    const uint32_t lane = threadIdx.x & 63;
+    const typename TQ::type *q = (const typename TQ::type *)a.r.q + (int64_t)row * a.r.q_rs + (int64_t)h * a.r.q_hs;
+    float mc = 0.f, l = 0.f, o[E] = {};
+    bool none = true; // no number yet
+    for (uint32_t i = b0; i < b1; ++i) {
+        const uint32_t j0 = bl.block(i) * 64;
+        const int64_t j = j0 + lane;
+        const bool seen = j <= pos && (!a.window || j < (int64_t)a.sinks || j > (int64_t)pos - a.window);
+        float x = -INFINITY;
+        if (seen) {
+            const tk *k = (const tk *)kp + j * a.own.ts;
+            x = 0.f;
+            for (int d = 0; d < D; ++d)
+                x = fmaf((float)q[d], (float)k[d], x);
+            x *= a.r.cexp;
+        }
+        const uint64_t any = __ballot(seen);
+        const float top = wave_max(x);
+        if (top > (none ? -INFINITY : mc)) {
+            const float r = none ? 0.f : exp2_hw(mc - top);
+            mc = top, l *= r, none = false;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                o[e] *= r;
+        }
+        const float w = seen ? exp2_hw(x - mc) : 0.f;
+        l += wave_sum(w);
+        __builtin_amdgcn_wave_barrier();
+        weights[lane] = w;
+        __builtin_amdgcn_wave_barrier();
+        for (uint64_t m = any; m; m &= m - 1) {
+            const uint32_t s = (uint32_t)__ffsll((unsigned long long)m) - 1;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                o[e] += weights[s] * (float)((const tk *)vp)[(int64_t)(j0 + s) * a.own.ts + lane * E + e];
+        }
+    }
+    const float off = none ? -INFINITY : mc;
+    if (a.own_splits + a.prefix_splits == 1) {
+        store_row<TQ, D>(a, row, h, pos < 0, off, l, o);
+        return;
+    }
+    const size_t to = ((size_t)split * a.r.n_rows + row) * a.r.heads + h;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        a.o[to * D + lane * E + e] = o[e];
+    if (lane == 0)
+        a.ml[to] = make_float2(off, l);
+}
+
 #define TILE_KEYS 64
 // One workgroup: 64 RT (token, head) pairs of one sequence and kv head, 16 RT a wave, over
 // one key range.  Blocks of 64 slots pass through two buffers of shared memory, K and V as
@@ -746,16 +819,16 @@ template <typename TQ> __device__ __forceinline__ bool has_nonfinite(uint4 v)
 // its rows see whole are used without masks.
 //
 // A slot that some rows of a wave see and others do not may hold an infinity or NaN in V,
-// which times a weight of 0 would reach all of them: where a masked block holds such
-// numbers, the products leave them out and they are added row by row.
+// which times a weight of 0 would reach all of them: a wave that met such numbers in a
+// masked block computes its rows again, one by one (attn_row).
 template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(const AttnOpArgs &a)
 {
     typedef typename TQ::vec vec;
     constexpr uint32_t ROWS = 64 * RT, PIECES = D / 8, BYTES = TILE_KEYS * D * 2;
     constexpr int LD = TILE_KEYS * PIECES / 256; // 16-byte loads of K, and of V, a thread and block
     __shared__ __attribute__((aligned(16))) uint8_t ks[2][BYTES], vs[2][BYTES];
-    __shared__ float pw[4][16][33]; // one row tile's weights of 32 slots, a wave each
-    __shared__ uint64_t odd[4];     // slots of a block whose V is not all finite
+    __shared__ float weights[4][64]; // attn_row's
+    __shared__ uint64_t odd[4];      // slots of a block whose V is not all finite
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4;
     const uint32_t kh = blockIdx.x % a.own.kv_heads, G = a.group;
     const uint32_t flat = blockIdx.x / a.own.kv_heads, split = a.own_splits == 1 ? 0 : flat % a.own_splits;
@@ -833,6 +906,7 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
     if (b0 + 1 < b1)
         load(bl.block(b0 + 1));
     const uint32_t at = v_lane<D>(lane);
+    uint32_t again = 0;
     for (uint32_t i = b0; i < b1; ++i) {
         const uint32_t blk = bl.block(i), buf = (i - b0) & 1;
         __syncthreads();
@@ -852,9 +926,8 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
                 for (int x = 0; x < D / 32; ++x)
                     k[u][x] = *(const vec *)(kb + v_piece<D>(16 * u + (lane & 15), g + 4 * x) * 16);
             vec p[RT][TQ::parts];
-            uint32_t wrong = 0;
             if (!whole)
-                wrong = __builtin_amdgcn_readfirstlane((uint32_t)(odd[i & 3] >> (32 * sub)));
+                again |= __builtin_amdgcn_readfirstlane((uint32_t)(odd[i & 3] >> (32 * sub)));
             floatx4 s[RT][2];
 #pragma unroll
             for (int t = 0; t < RT; ++t)
@@ -884,42 +957,9 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
                 }
             }
             weigh<RT>(S, s, Q, p);
-            if (wrong) { // uniform; rare
-#pragma unroll
-                for (int t = 0; t < RT; ++t) {
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        float w = (float)p[t][0][x];
-                        if constexpr (TQ::parts == 2)
-                            w += (float)p[t][1][x];
-                        pw[wave][lane & 15][16 * (x / 4) + 4 * g + x % 4] = w;
-                    }
-                    __builtin_amdgcn_wave_barrier();
-                    for (uint32_t m = wrong; m; m &= m - 1) {
-                        const uint32_t j = (uint32_t)__ffs((int)m) - 1;
-                        const float w = pw[wave][lane & 15][j];
-#pragma unroll
-                        for (int n = 0; n < D / 16; ++n) {
-                            const typename TQ::kv *v =
-                                (const typename TQ::kv *)(vb + v_piece<D>(j, 2 * n + g / 2) * 16 + (g & 1) * 8);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float x = (float)v[e];
-                                if (w != 0.f && !(fabsf(x) < INFINITY))
-                                    S.o[t][n][e] += w * x;
-                            }
-                        }
-                    }
-                }
-            }
 #pragma unroll
             for (int n = 0; n < D / 16; ++n) {
-                vec v = v_operand<TQ, D>(vb, at, n);
-                if (wrong)
-#pragma unroll
-                    for (int x = 0; x < 8; ++x)
-                        if (!(fabsf((float)v[x]) < INFINITY))
-                            v[x] = (typename TQ::kv)0.f;
+                const vec v = v_operand<TQ, D>(vb, at, n);
 #pragma unroll
                 for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -933,6 +973,14 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
             load(bl.block(i + 2));
     }
     const bool final = a.own_splits + a.prefix_splits == 1;
+    if (again) { // uniform; rare
+        for (uint32_t x = 0; x < 16 * RT && w0 + x < total; ++x) {
+            const uint32_t row = pairs.row_of(x);
+            attn_row<TQ, D>(a, bl, b0, b1, kp, vp, row, kh * G + pairs.head_of(x), first + (int32_t)row - lo, split,
+                            weights[wave]);
+        }
+        return;
+    }
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const float l = row_sum(S.l[t]);
@@ -940,7 +988,7 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
         if (w0 + x >= total)
             continue;
         const uint32_t row = pairs.row_of(x), h = kh * G + pairs.head_of(x);
-        const float off = S.m[t] > -INFINITY ? S.mc[t] : -INFINITY;
+        const float off = S.offset(t);
         if (final) {
             const bool empty = pos[t] < 0;
             const float f = empty ? 0.f : inverse(l);
@@ -1060,16 +1108,15 @@ template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const
 
 // RT: row tiles of a workgroup of rows that see the same slots, as many as the registers
 // hold beside the next block's K and V.
-#define STEP(TQ, tag, D, RT, NW)                                                                               \
-    extern "C" __global__ __launch_bounds__(NW * 64, RT == 1 ? NW / 4 : 2) void k_attn_step_##tag##_##D##_r##RT##w##NW( \
+#define STEP(TQ, tag, D, RT)                                                                                   \
+    extern "C" __global__ __launch_bounds__(256, RT == 1 ? 1 : 2) void k_attn_step_##tag##_##D##_r##RT(        \
         const AttnOpArgs a)                                                                                    \
     {                                                                                                          \
-        attn_step<TQ, D, RT, NW>(a);                                                                           \
+        attn_step<TQ, D, RT>(a);                                                                               \
     }
-#define STEPS(TQ, tag, D, MOST, WAVES)                                                                         \
-    STEP(TQ, tag, D, 1, 4)                                                                                     \
-    STEP(TQ, tag, D, 1, WAVES)                                                                                    \
-    STEP(TQ, tag, D, MOST, 4)                                                                                  \
+#define STEPS(TQ, tag, D, MOST)                                                                                \
+    STEP(TQ, tag, D, 1)                                                                                        \
+    STEP(TQ, tag, D, MOST)                                                                                     \
     extern "C" __global__ __launch_bounds__(256) void k_attn_merge_##tag##_##D(const AttnOpArgs a)             \
     {                                                                                                          \
         attn_merge<TQ, D>(a);                                                                                  \
@@ -1078,12 +1125,12 @@ template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const
     {                                                                                                          \
         scored_join<TQ, D>(a);                                                                                 \
     }
-STEPS(F32, f32, 64, 4, 16)
-STEPS(F32, f32, 128, 2, 8)
-STEPS(F16, f16, 64, 4, 16)
-STEPS(F16, f16, 128, 2, 8)
-STEPS(BF16, bf16, 64, 4, 16)
-STEPS(BF16, bf16, 128, 2, 8)
+STEPS(F32, f32, 64, 4)
+STEPS(F32, f32, 128, 2)
+STEPS(F16, f16, 64, 4)
+STEPS(F16, f16, 128, 2)
+STEPS(BF16, bf16, 64, 4)
+STEPS(BF16, bf16, 128, 2)
 
 #define TILE(TQ, tag, D, RT)                                                                                   \
     extern "C" __global__ __launch_bounds__(256, 2) void k_attn_tile_##tag##_##D##_r##RT(const AttnOpArgs a)   \
