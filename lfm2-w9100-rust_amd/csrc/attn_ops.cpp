@@ -25,7 +25,7 @@
 // ------------------------------------------------------------------ code object
 // Row tiles of 16 of the larger forms, as many as the registers hold.
 static uint32_t step_tiles(uint32_t dim) { return dim == 64 ? 4 : 2; }
-static uint32_t tile_tiles(uint32_t type, uint32_t dim) { return dim == 64 && type != LFM_TYPE_F32 ? 4 : 2; }
+#define TILE_TILES 2
 
 // Kernels by [type pair][head_dim 64, 128]; the pair is the rows' type.
 struct AttnKernels {
@@ -59,7 +59,7 @@ static int load_attn(int dev)
                 hipFunction_t *f;
                 std::string name;
             } fns[] = {{&k.tile_1[t][d], "k_attn_tile" + tag + "_r1"},
-                       {&k.tile_most[t][d], "k_attn_tile" + tag + "_r" + std::to_string(tile_tiles(t, d ? 128 : 64))},
+                       {&k.tile_most[t][d], "k_attn_tile" + tag + "_r" + std::to_string(TILE_TILES)},
                        {&k.weights[t][d], "k_attn_weights" + tag},
                        {&k.step_1[t][d], "k_attn_step" + tag + "_r1"},
                        {&k.step_most[t][d], "k_attn_step" + tag + "_r" + std::to_string(step_tiles(d ? 128 : 64))},
@@ -289,8 +289,11 @@ static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint
     } else {
         // sequences end inside tiles: at most one more tile each
         const uint64_t cut = (uint64_t)r->n_rows * G;
-        const uint32_t most = 64 * tile_tiles(r->type, kv->head_dim);
-        p.tile_most = cut / most * kv->kv_heads >= 512;
+        // the larger tile reads K and V half as often; it is taken where it fills the CUs as
+        // often as they hold it (four at 64 dims, two at 128): a 2048-token prompt of 32
+        // heads over 8 of 64 dims, half of that, takes 51 us in the small one and 60 in it
+        const uint32_t most = 64 * TILE_TILES;
+        p.tile_most = cut / most * kv->kv_heads >= (kv->head_dim == 64 ? 1024 : 512);
         const uint64_t rows = p.tile_most ? most : 64;
         p.tile_items = cut / rows + std::min<uint64_t>(kv->n_seq, r->n_rows);
         const uint64_t span = window ? std::min<uint64_t>(kv->slots, (uint64_t)window + sinks + rows / G + 128)

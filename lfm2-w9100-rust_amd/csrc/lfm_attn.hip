@@ -16,6 +16,7 @@ template <int N> struct Const {
 // numbers of row (A) or column (B) l % 16, at inner places 8 (l / 16) + i, and 4 results,
 // rows 4 (l / 16) + e of column l % 16.
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef short short8v __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -443,7 +444,7 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_step(
     uint8_t *const vt = smem + wave * V_BYTES;
     const uint32_t at = v_lane<D>(lane);
     vec kr[2][D / 32];
-    uint4 vr[VL];
+    u32x4 vr[VL];
     auto load = [&](uint32_t blk) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -456,7 +457,7 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_step(
 #pragma unroll
         for (int i = 0; i < VL; ++i) {
             const uint32_t j = min(blk * 32 + (i * 64 + lane) / PIECES, bl.hi - 1);
-            vr[i] = *(const uint4 *)(vp + (int64_t)j * ts + (lane % PIECES) * 8);
+            vr[i] = *(const u32x4 *)(vp + (int64_t)j * ts + (lane % PIECES) * 8);
         }
     };
     uint32_t b = b0 + wave;
@@ -481,8 +482,8 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_step(
             for (int i = 0; i < VL; ++i) {
                 const uint32_t row = (i * 64 + lane) / PIECES;
                 if (!whole && !bl.seen(blk * 32 + row))
-                    vr[i] = make_uint4(0, 0, 0, 0);
-                *(uint4 *)(vt + v_piece<D>(row, lane % PIECES) * 16) = vr[i];
+                    vr[i] = u32x4{0, 0, 0, 0};
+                *(u32x4 *)(vt + v_piece<D>(row, lane % PIECES) * 16) = vr[i];
             }
             floatx4 s[RT][2];
 #pragma unroll
@@ -740,7 +741,7 @@ __device__ __forceinline__ bool find_item(const RowsView &r, uint32_t n_seq, uin
     return false;
 }
 
-template <typename TQ> __device__ __forceinline__ bool has_nonfinite(uint4 v)
+template <typename TQ> __device__ __forceinline__ bool has_nonfinite(u32x4 v)
 {
     constexpr uint32_t E = TQ::offset == 0.f ? 0x7F807F80u : 0x7C007C00u; // exponents of two numbers
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -870,14 +871,14 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
 
     const int64_t at0 = (int64_t)b * a.own.ss + (int64_t)kh * a.own.hs;
     const uint16_t *kp = a.own.k + at0, *vp = a.own.v + at0;
-    uint4 kr[LD], vr[LD];
+    u32x4 kr[LD], vr[LD];
     auto load = [&](uint32_t blk) {
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             const uint32_t j = min(blk * TILE_KEYS + (i * 256 + tid) / PIECES, bl.hi - 1);
             const int64_t o = (int64_t)j * a.own.ts + (tid % PIECES) * 8;
-            kr[i] = *(const uint4 *)(kp + o);
-            vr[i] = *(const uint4 *)(vp + o);
+            kr[i] = *(const u32x4 *)(kp + o);
+            vr[i] = *(const u32x4 *)(vp + o);
         }
     };
     // slots past the last visible one repeat it in K and are zeros in V
@@ -886,14 +887,14 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             const uint32_t row = (i * 256 + tid) / PIECES, to = v_piece<D>(row, tid % PIECES) * 16;
-            *(uint4 *)(ks[buf] + to) = kr[i];
+            *(u32x4 *)(ks[buf] + to) = kr[i];
             if (!whole) {
                 if (!bl.seen(blk * TILE_KEYS + row))
-                    vr[i] = make_uint4(0, 0, 0, 0);
+                    vr[i] = u32x4{0, 0, 0, 0};
                 else if (has_nonfinite<TQ>(vr[i]))
                     atomicOr((unsigned long long *)&odd[i0 & 3], 1ull << row);
             }
-            *(uint4 *)(vs[buf] + to) = vr[i];
+            *(u32x4 *)(vs[buf] + to) = vr[i];
         }
     };
     if (tid < 4)
@@ -1133,7 +1134,7 @@ STEPS(BF16, bf16, 64, 4)
 STEPS(BF16, bf16, 128, 2)
 
 #define TILE(TQ, tag, D, RT)                                                                                   \
-    extern "C" __global__ __launch_bounds__(256, 2) void k_attn_tile_##tag##_##D##_r##RT(const AttnOpArgs a)   \
+    extern "C" __global__ __launch_bounds__(256, D == 128 ? 2 : TQ::parts == 2 ? 3 : 4) void k_attn_tile_##tag##_##D##_r##RT(const AttnOpArgs a)   \
     {                                                                                                          \
         attn_tile<TQ, D, RT>(a);                                                                               \
     }
@@ -1146,9 +1147,9 @@ STEPS(BF16, bf16, 128, 2)
     }
 TILES(F32, f32, 64, 2)
 TILES(F32, f32, 128, 2)
-TILES(F16, f16, 64, 4)
+TILES(F16, f16, 64, 2)
 TILES(F16, f16, 128, 2)
-TILES(BF16, bf16, 64, 4)
+TILES(BF16, bf16, 64, 2)
 TILES(BF16, bf16, 128, 2)
 
 // ------------------------------------------------------------------ eviction
@@ -1222,7 +1223,7 @@ extern "C" __global__ __launch_bounds__(SEL_THREADS) void k_kv_select(const Evic
     bool exact = false;
     for (int pass = 3; pass >= 0 && !exact; --pass) {
         for (uint32_t i = tid; i < 256 * SEL_COPIES / 4; i += SEL_THREADS)
-            ((uint4 *)hist)[i] = make_uint4(0, 0, 0, 0);
+            ((u32x4 *)hist)[i] = u32x4{0, 0, 0, 0};
         __syncthreads();
         for (uint32_t j = tid; j < n; j += SEL_THREADS) {
             const uint32_t k = rank(j);
@@ -1234,7 +1235,7 @@ extern "C" __global__ __launch_bounds__(SEL_THREADS) void k_kv_select(const Evic
             uint32_t v = 0;
 #pragma unroll
             for (int i = 0; i < SEL_COPIES / 4; ++i) {
-                const uint4 x = ((const uint4 *)hist)[tid * (SEL_COPIES / 4) + i];
+                const u32x4 x = ((const u32x4 *)hist)[tid * (SEL_COPIES / 4) + i];
                 v += x.x + x.y + x.z + x.w;
             }
             bins[tid] = v;
@@ -1242,7 +1243,7 @@ extern "C" __global__ __launch_bounds__(SEL_THREADS) void k_kv_select(const Evic
         __syncthreads();
         // every wave: lane l holds bins 255 - 4 l downwards; the bin where the count from the
         // top reaches `need`
-        const uint4 x = ((const uint4 *)bins)[63 - lane];
+        const u32x4 x = ((const u32x4 *)bins)[63 - lane];
         const uint32_t four = x.x + x.y + x.z + x.w;
         uint32_t upto = four;
 #pragma unroll
@@ -1336,9 +1337,9 @@ extern "C" __global__ __launch_bounds__(256) void k_kv_move(const EvictArgs a)
         if (moved || !a.in_place) {
             const int64_t from = (int64_t)b * a.c.ss + (int64_t)kh * a.c.hs + (int64_t)s * a.c.ts + piece * 8;
             const int64_t to = (int64_t)b * a.oss + (int64_t)kh * a.ohs + (int64_t)n * a.ots + piece * 8;
-            const uint4 k = *(const uint4 *)(a.c.k + from), v = *(const uint4 *)(a.c.v + from);
-            *(uint4 *)((uint16_t *)a.k_out + to) = k;
-            *(uint4 *)((uint16_t *)a.v_out + to) = v;
+            const u32x4 k = *(const u32x4 *)(a.c.k + from), v = *(const u32x4 *)(a.c.v + from);
+            *(u32x4 *)((uint16_t *)a.k_out + to) = k;
+            *(u32x4 *)((uint16_t *)a.v_out + to) = v;
         }
         if (piece == 0) {
             const size_t src = bh * a.c.slots + (uint32_t)s, dst = bh * a.out_slots + n;
