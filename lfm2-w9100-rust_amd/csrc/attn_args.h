@@ -25,7 +25,11 @@ struct RowsView {
     float scale, cexp; // cexp = scale * log2(e)
 };
 
-#define MAX_GROUP 128 // query heads of a kv head
+#define MAX_GROUP 128     // query heads of a kv head
+#define TILE_TILES 2      // row tiles a wave of the larger tile kernel
+#define SCORED_SLOTS 1024 // slots a workgroup of k_scored_join
+#define SUM_KEYS 32       // slots a workgroup of k_attn_weights
+#define SUM_WAVES 8
 
 struct AttnOpArgs {
     KvView own;    // slots of the row's own sequence, causal
@@ -39,10 +43,13 @@ struct AttnOpArgs {
     // beside it in o, and k_attn_merge joins them.
     uint32_t own_splits, prefix_splits;
     uint32_t prefix_groups, own_groups; // row groups: of the whole batch, of one token
+    uint32_t step_prefix;               // items of the step kernel that are the prefix's
     float2 *ml;
     float *o;
-    // scored: scores[(b * heads + h) * slots + j], in units of q . k
+    // scored: scores[(b * heads + h) * score_row + j], in units of q . k; score_row is slots
+    // rounded up to whole blocks
     float *scores;
+    uint32_t score_row;
     float2 *stats; // nullable: per row and head {log2 offset, 1 / sum} of its weights
     const float *acc; // nullable
     float *acc_out;   // [n_seq][kv_heads][slots]

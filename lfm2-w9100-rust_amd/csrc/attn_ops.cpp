@@ -25,12 +25,11 @@
 // ------------------------------------------------------------------ code object
 // Row tiles of 16 of the larger forms, as many as the registers hold.
 static uint32_t step_tiles(uint32_t dim) { return dim == 64 ? 4 : 2; }
-#define TILE_TILES 2
 
 // Kernels by [type pair][head_dim 64, 128]; the pair is the rows' type.
 struct AttnKernels {
     hipModule_t mod = nullptr;
-    hipFunction_t tile_1[3][2], tile_most[3][2], weights[3][2];
+    hipFunction_t tile_1[3][2], tile_most[3][2], tile_prefix[3][2], weights[3][2];
     hipFunction_t step_1[3][2], step_most[3][2], merge[3][2], scored_join[3][2];
     hipFunction_t kv_select, kv_move;
 };
@@ -60,6 +59,7 @@ static int load_attn(int dev)
                 std::string name;
             } fns[] = {{&k.tile_1[t][d], "k_attn_tile" + tag + "_r1"},
                        {&k.tile_most[t][d], "k_attn_tile" + tag + "_r" + std::to_string(TILE_TILES)},
+                       {&k.tile_prefix[t][d], "k_attn_prefix" + tag + "_r" + std::to_string(TILE_TILES)},
                        {&k.weights[t][d], "k_attn_weights" + tag},
                        {&k.step_1[t][d], "k_attn_step" + tag + "_r1"},
                        {&k.step_most[t][d], "k_attn_step" + tag + "_r" + std::to_string(step_tiles(d ? 128 : 64))},
@@ -252,6 +252,7 @@ struct Plan {
     uint32_t own_splits = 1, prefix_splits = 0, own_groups = 1, prefix_groups = 0;
     bool most = false;      // the step kernel's larger form
     bool tile_most = false; // the tile kernel's
+    bool tile_prefix = false; // the prefix goes through the tile kernel too
     uint64_t tile_items = 0;
     bool join = false; // a second kernel joins the key ranges
     size_t ml_bytes = 0, o_bytes = 0, score_bytes = 0, stat_bytes = 0;
@@ -267,12 +268,16 @@ static uint32_t ranges(uint64_t wanted, uint64_t worth)
     return (uint32_t)std::min<uint64_t>({std::max<uint64_t>(1, wanted), std::max<uint64_t>(1, worth), MOST_RANGES});
 }
 
+static uint32_t score_row(const lfm_kv *kv) { return (kv->slots + 31) / 32 * 32; }
+
 static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint32_t window, uint32_t sinks, bool scored)
 {
     Plan p;
     const uint32_t G = r->heads / kv->kv_heads;
     const uint64_t pairs = (uint64_t)r->n_rows * r->heads;
-    p.most = prefix ? (uint64_t)r->n_rows * G > 16 : G > 16;
+    // from four tiles of 16 rows on, workgroups that share K and V in shared memory
+    p.tile_prefix = prefix && (uint64_t)r->n_rows * G > 64;
+    p.most = prefix && !p.tile_prefix ? (uint64_t)r->n_rows * G > 16 : G > 16;
     const uint32_t per = p.most ? 16 * step_tiles(kv->head_dim) : 16;
     if (!r->start) {
         const uint64_t span = window ? std::min<uint64_t>(kv->slots, (uint64_t)window + sinks + 63) : kv->slots;
@@ -301,10 +306,12 @@ static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint
         p.own_splits = ranges(TARGET_GROUPS / std::max<uint64_t>(1, p.tile_items * kv->kv_heads), span / 512);
     }
     if (prefix) {
-        p.prefix_groups = (uint32_t)(((uint64_t)r->n_rows * G + per - 1) / per);
+        const uint32_t rows = p.tile_prefix ? 64 * TILE_TILES : per;
+        p.prefix_groups = (uint32_t)(((uint64_t)r->n_rows * G + rows - 1) / rows);
         const uint64_t pitems = (uint64_t)std::max(1u, p.prefix_groups) * kv->kv_heads;
         const uint64_t blocks = (prefix->slots + 31) / 32;
-        p.prefix_splits = ranges(TARGET_GROUPS / pitems, blocks / (blocks > 64 ? 8 : 4));
+        const uint64_t wanted = p.tile_prefix && kv->head_dim == 64 ? 2 * TARGET_GROUPS : TARGET_GROUPS;
+        p.prefix_splits = ranges(wanted / pitems, blocks / (blocks > 64 ? 8 : 4));
     }
     const uint32_t splits = p.own_splits + p.prefix_splits;
     const bool steps = scored && !r->start; // scores are kept from the step to the join
@@ -314,7 +321,7 @@ static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint
         p.o_bytes = round256((size_t)splits * pairs * kv->head_dim * 4);
     }
     if (steps)
-        p.score_bytes = round256((size_t)pairs * kv->slots * 4);
+        p.score_bytes = round256((size_t)pairs * score_row(kv) * 4);
     else if (scored)
         p.stat_bytes = round256((size_t)pairs * 8);
     return p;
@@ -337,6 +344,7 @@ static AttnOpArgs op_args(const Plan &p, const lfm_kv *prefix, const lfm_kv *kv,
     a.ml = (float2 *)w;
     a.o = (float *)(w += p.ml_bytes);
     w += p.o_bytes;
+    a.score_row = score_row(kv);
     a.scores = p.score_bytes ? (float *)w : nullptr;
     w += p.score_bytes;
     a.stats = p.stat_bytes ? (float2 *)w : nullptr;
@@ -352,23 +360,28 @@ static int launch_items(hipFunction_t f, uint64_t items, uint32_t kv_heads, uint
     return launch(f, dim3((uint32_t)items * kv_heads), threads, s, a);
 }
 
-// One launch over (kv head, rows, key range), the prefix's items before the own ones; rows
-// of many tokens take theirs in a second launch; then the ranges are joined.
-static int attend(AttnKernels *K, const Plan &p, const AttnOpArgs &a, const lfm_kv *kv, const lfm_rows *rows,
+// Launches over (kv head, rows, key range): the prefix of many rows, then single rows (and the
+// prefix of few), then rows of many tokens; then the ranges are joined.
+static int attend(AttnKernels *K, const Plan &p, AttnOpArgs a, const lfm_kv *kv, const lfm_rows *rows,
                   hipStream_t s)
 {
     const int t = rows->type, d = dim_index(kv);
-    const uint64_t steps = (uint64_t)p.prefix_groups * p.prefix_splits +
-                           (rows->start ? 0 : (uint64_t)rows->n_rows * p.own_groups * p.own_splits);
-    if (steps) {
-        hipFunction_t f = p.most ? K->step_most[t][d] : K->step_1[t][d];
-        RC(launch_items(f, steps, kv->kv_heads, 256, s, a));
+    uint64_t steps = rows->start ? 0 : (uint64_t)rows->n_rows * p.own_groups * p.own_splits;
+    a.step_prefix = 0;
+    if (p.tile_prefix) {
+        RC(launch_items(K->tile_prefix[t][d], (uint64_t)p.prefix_groups * p.prefix_splits, kv->kv_heads, 256, s, a));
+    } else {
+        a.step_prefix = p.prefix_groups * p.prefix_splits;
+        steps += a.step_prefix;
     }
+    if (steps)
+        RC(launch_items(p.most ? K->step_most[t][d] : K->step_1[t][d], steps, kv->kv_heads, 256, s, a));
     if (rows->start)
         RC(launch_items(p.tile_most ? K->tile_most[t][d] : K->tile_1[t][d], p.tile_items * p.own_splits, kv->kv_heads,
                         256, s, a));
     if (a.scores)
-        return launch(K->scored_join[t][d], dim3((kv->slots + 511) / 512, kv->kv_heads, kv->n_seq), 256, s, a);
+        return launch(K->scored_join[t][d],
+                      dim3((kv->slots + SCORED_SLOTS - 1) / SCORED_SLOTS, kv->kv_heads, kv->n_seq), 256, s, a);
     if (p.join)
         return launch(K->merge[t][d], dim3((rows->n_rows * rows->heads + 3) / 4), 256, s, a);
     return LFM_OK;
@@ -443,8 +456,10 @@ extern "C" int lfm_attn_scored(const lfm_kv *kv, const lfm_rows *rows, const flo
         RC(attend(K, p, a, kv, rows, s));
     if (!rows->start)
         return LFM_OK;
-    return launch(K->weights[rows->type][dim_index(kv)], dim3((kv->slots + 63) / 64, kv->kv_heads, kv->n_seq), 512, s,
-                  a);
+    const uint64_t blocks = (uint64_t)(kv->slots + SUM_KEYS - 1) / SUM_KEYS * kv->kv_heads;
+    if (blocks > 0x7FFFFFFFull)
+        return fail(LFM_EINVAL, "%s: %u slots of %u kv heads", op, kv->slots, kv->kv_heads);
+    return launch(K->weights[rows->type][dim_index(kv)], dim3((uint32_t)blocks, kv->n_seq), SUM_WAVES * 64, s, a);
 }
 
 static int check_prefix(const char *op, const lfm_kv *prefix, const lfm_kv *kv)

@@ -401,8 +401,7 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_step(
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4;
     const uint32_t kh = blockIdx.x % a.own.kv_heads, G = a.group;
     uint32_t item = blockIdx.x / a.own.kv_heads;
-    const uint32_t prefix_items = a.prefix_groups * a.prefix_splits;
-    const bool pre = item < prefix_items;
+    const bool pre = item < a.step_prefix;
     uint32_t group = 0, part, parts, row0, total;
     const uint16_t *kp, *vp;
     int64_t ts;
@@ -419,7 +418,7 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_step(
         const int64_t at = (int64_t)kh * a.prefix.hs;
         kp = a.prefix.k + at, vp = a.prefix.v + at, ts = a.prefix.ts;
     } else {
-        item -= prefix_items;
+        item -= a.step_prefix;
         if (a.own_groups > 1) {
             const uint32_t q = item / a.own_groups;
             group = item - q * a.own_groups, item = q;
@@ -499,24 +498,20 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_step(
                 }
             if (b + NW < b1)
                 load(bl.block(b + NW));
-            if (a.scores && !pre) { // uniform
+            if (a.scores && !pre) { // uniform; rows of whole blocks, slots past the length among them
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
-                    if (16 * t + (lane & 15) < rows)
+                    if (16 * t + (lane & 15) < rows) {
+                        float *to = a.scores + ((size_t)row0 * a.r.heads + kh * G + i0 + 16 * t + (lane & 15)) * a.score_row +
+                                    blk * 32 + 4 * g;
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
-                            const uint32_t j = blk * 32 + 16 * u + 4 * g;
-                            float *to = a.scores +
-                                        ((size_t)row0 * a.r.heads + kh * G + i0 + 16 * t + (lane & 15)) * a.own.slots + j;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (j + e < bl.hi) {
-                                    if constexpr (TQ::parts == 2)
-                                        to[e] = s[t][u][e] * Q.back[t];
-                                    else
-                                        to[e] = s[t][u][e];
-                                }
+                            if constexpr (TQ::parts == 2)
+                                *(floatx4 *)(to + 16 * u) = s[t][u] * Q.back[t];
+                            else
+                                *(floatx4 *)(to + 16 * u) = s[t][u];
                         }
+                    }
             }
             if (!whole) {
 #pragma unroll
@@ -671,11 +666,11 @@ template <typename TQ, int D> __device__ __forceinline__ void attn_merge(const A
     store_row<TQ, D>(a, row, h, pos < 0 && (!a.prefix.k || clamp_len(a.prefix, 0) == 0), top, sum, o);
 }
 
-#define SCORED_SLOTS 512
 // After a scored step: joins the key ranges of one (sequence, kv head) and adds every
-// slot's weights, SCORED_SLOTS slots a workgroup.  Scores were kept as they left the
-// matrix cores, so a weight is one exponential here: 16 bytes a slot and kv head at four
-// query heads, where reading K again would be 128 or 256.
+// slot's weights, SCORED_SLOTS slots a workgroup, four a thread.  Scores were kept as they
+// left the matrix cores, so a weight is one exponential here: 16 bytes a slot and kv head at
+// four query heads, where reading K again would be 128 or 256.  The first four heads' scores
+// are loaded before the ranges are joined.
 template <typename TQ, int D> __device__ __forceinline__ void scored_join(const AttnOpArgs &a)
 {
     const uint32_t chunk = blockIdx.x, kh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x,
@@ -683,6 +678,21 @@ template <typename TQ, int D> __device__ __forceinline__ void scored_join(const 
     const uint32_t G = a.group, n = (uint32_t)clamp_len(a.own, b);
     if (chunk && chunk * SCORED_SLOTS >= n)
         return;
+    constexpr int EACH = SCORED_SLOTS / 256, EARLY = 4;
+    const float *scores = a.scores + ((size_t)b * a.r.heads + kh * G) * a.score_row;
+    const size_t at = ((size_t)b * a.own.kv_heads + kh) * a.own.slots;
+    uint32_t j[EACH];
+    float had[EACH] = {}, s[EACH][EARLY] = {};
+    if (n) // uniform
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            j[i] = min(chunk * SCORED_SLOTS + i * 256 + tid, n - 1);
+            if (a.acc)
+                had[i] = a.acc[at + j[i]];
+#pragma unroll
+            for (int g = 0; g < EARLY; ++g)
+                s[i][g] = scores[(size_t)min((uint32_t)g, G - 1) * a.score_row + j[i]];
+        }
     __shared__ float2 st[MAX_GROUP]; // offset and 1 / sum
     // the outputs of the G heads are spread over the workgroups in use
     const uint32_t chunks = max(1u, (n + SCORED_SLOTS - 1) / SCORED_SLOTS);
@@ -696,16 +706,19 @@ template <typename TQ, int D> __device__ __forceinline__ void scored_join(const 
             store_row<TQ, D>(a, b, kh * G + g, n == 0, top, sum, o);
     }
     __syncthreads();
-    for (uint32_t j = chunk * SCORED_SLOTS + tid; j < min(n, (chunk + 1) * SCORED_SLOTS); j += 256) {
-        const float *s = a.scores + ((size_t)b * a.r.heads + kh * G) * a.own.slots + j;
-        const size_t at = ((size_t)b * a.own.kv_heads + kh) * a.own.slots + j;
-        const float had = a.acc ? a.acc[at] : 0.f;
-        float sum = 0.f;
-#pragma unroll 4
-        for (uint32_t g = 0; g < G; ++g)
-            sum += exp2_hw(fmaf(s[(size_t)g * a.own.slots], a.r.cexp, -st[g].x)) * st[g].y;
-        a.acc_out[at] = had + sum;
-    }
+    if (n)
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            float sum = 0.f;
+#pragma unroll
+            for (int g = 0; g < EARLY; ++g)
+                if (g < (int)G)
+                    sum += exp2_hw(fmaf(s[i][g], a.r.cexp, -st[g].x)) * st[g].y;
+            for (uint32_t g = EARLY; g < G; ++g)
+                sum += exp2_hw(fmaf(scores[(size_t)g * a.score_row + j[i]], a.r.cexp, -st[g].x)) * st[g].y;
+            if (chunk * SCORED_SLOTS + i * 256 + tid < n)
+                a.acc_out[at + j[i]] = had[i] + sum;
+        }
 }
 
 // ------------------------------------------------------------------ rows of many tokens
@@ -813,7 +826,7 @@ __device__ void attn_row(const AttnOpArgs &a, const B &bl, uint32_t b0, uint32_t
 
 #define TILE_KEYS 64
 // One workgroup: 64 RT (token, head) pairs of one sequence and kv head, 16 RT a wave, over
-// one key range.  Blocks of 64 slots pass through two buffers of shared memory, K and V as
+// one key range; PRE: of the whole batch over the prefix.  Blocks of 64 slots pass through two buffers of shared memory, K and V as
 // they lie in the cache with their 16-byte pieces exchanged (v_piece); every wave reads K as
 // A operands and V through the transposed read.  The next block's loads are in flight while
 // a block is used.  Blocks that no row of a wave sees are passed over by it, those that all
@@ -822,7 +835,7 @@ __device__ void attn_row(const AttnOpArgs &a, const B &bl, uint32_t b0, uint32_t
 // A slot that some rows of a wave see and others do not may hold an infinity or NaN in V,
 // which times a weight of 0 would reach all of them: a wave that met such numbers in a
 // masked block computes its rows again, one by one (attn_row).
-template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(const AttnOpArgs &a)
+template <typename TQ, int D, int RT, bool PRE> __device__ __forceinline__ void attn_tile(const AttnOpArgs &a)
 {
     typedef typename TQ::vec vec;
     constexpr uint32_t ROWS = 64 * RT, PIECES = D / 8, BYTES = TILE_KEYS * D * 2;
@@ -832,20 +845,31 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
     __shared__ uint64_t odd[4];      // slots of a block whose V is not all finite
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4;
     const uint32_t kh = blockIdx.x % a.own.kv_heads, G = a.group;
-    const uint32_t flat = blockIdx.x / a.own.kv_heads, split = a.own_splits == 1 ? 0 : flat % a.own_splits;
-    uint32_t b, tile, tiles;
-    if (!find_item(a.r, a.own.n_seq, a.own_splits == 1 ? flat : flat / a.own_splits, G, ROWS, &b, &tile, &tiles))
-        return;
-    tile = tiles - 1 - tile; // the longest first
-    int32_t lo, hi;
-    seq_rows(a.r, b, &lo, &hi);
-    const uint32_t total = (uint32_t)(hi - lo) * G, p0 = tile * ROWS;
-    const int32_t first = clamp_len(a.own, b) - (hi - lo); // position of the sequence's first row
-    const int32_t pos_lo = first + (int32_t)(p0 / G), pos_hi = first + (int32_t)((min(p0 + ROWS, total) - 1) / G);
+    const KvView &c = PRE ? a.prefix : a.own;
+    const uint32_t splits = PRE ? a.prefix_splits : a.own_splits;
+    const uint32_t flat = blockIdx.x / a.own.kv_heads, split = splits == 1 ? 0 : flat % splits;
+    // rows lo .. hi of one sequence, row lo at position `first` and each next one `step` further;
+    // over the prefix all rows, each at its last position
+    uint32_t b = 0, tile, tiles;
+    int32_t lo = 0, hi = (int32_t)a.r.n_rows, first, step = PRE ? 0 : 1;
+    if (PRE) {
+        tile = splits == 1 ? flat : flat / splits;
+        first = clamp_len(c, 0) - 1;
+    } else {
+        if (!find_item(a.r, a.own.n_seq, splits == 1 ? flat : flat / splits, G, ROWS, &b, &tile, &tiles))
+            return;
+        tile = tiles - 1 - tile; // the longest first
+        seq_rows(a.r, b, &lo, &hi);
+        first = clamp_len(c, b) - (hi - lo);
+    }
+    const uint32_t total = (uint32_t)(hi - lo) * G, p0 = tile * ROWS, window = PRE ? 0 : a.window,
+                   sinks = PRE ? 0 : a.sinks;
+    const int32_t pos_lo = first + step * (int32_t)(p0 / G),
+                  pos_hi = first + step * (int32_t)((min(p0 + ROWS, total) - 1) / G);
     Blocks<TILE_KEYS> bl;
-    bl.set(pos_lo, pos_hi, a.window, a.sinks);
+    bl.set(pos_lo, pos_hi, window, sinks);
     uint32_t b0, b1;
-    share(bl.count, split, a.own_splits, &b0, &b1);
+    share(bl.count, split, splits, &b0, &b1);
 
     Queries<TQ, D, RT> Q;
     State<TQ, D, RT> S;
@@ -858,25 +882,26 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
         const uint32_t x = 16 * t + (lane & 15), row = pairs.row_of(x);
         const bool in = w0 + x < total;
         load_row<TQ, D, RT>(Q, t, a.r, in, row, kh * G + pairs.head_of(x));
-        pos[t] = in ? first + (int32_t)row - lo : -1;
+        pos[t] = in ? first + step * ((int32_t)row - lo) : -1;
     }
     // what this wave's rows see: some row of it, every row of it
     const bool any_row = w0 < total;
-    const int32_t wpos_lo = first + (int32_t)(w0 / G), wpos_hi = first + (int32_t)((min(w0 + 16 * RT, total) - 1) / G);
+    const int32_t wpos_lo = first + step * (int32_t)(w0 / G),
+                  wpos_hi = first + step * (int32_t)((min(w0 + 16 * RT, total) - 1) / G);
     Blocks<32> some, each;
-    some.set(wpos_lo, wpos_hi, a.window, a.sinks);
-    each.set(wpos_hi, wpos_lo, a.window, a.sinks);
+    some.set(wpos_lo, wpos_hi, window, sinks);
+    each.set(wpos_hi, wpos_lo, window, sinks);
     Blocks<TILE_KEYS> all; // every row of the workgroup
-    all.set(pos_hi, pos_lo, a.window, a.sinks);
+    all.set(pos_hi, pos_lo, window, sinks);
 
-    const int64_t at0 = (int64_t)b * a.own.ss + (int64_t)kh * a.own.hs;
-    const uint16_t *kp = a.own.k + at0, *vp = a.own.v + at0;
+    const int64_t at0 = (int64_t)b * c.ss + (int64_t)kh * c.hs;
+    const uint16_t *kp = c.k + at0, *vp = c.v + at0;
     u32x4 kr[LD], vr[LD];
     auto load = [&](uint32_t blk) {
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             const uint32_t j = min(blk * TILE_KEYS + (i * 256 + tid) / PIECES, bl.hi - 1);
-            const int64_t o = (int64_t)j * a.own.ts + (tid % PIECES) * 8;
+            const int64_t o = (int64_t)j * c.ts + (tid % PIECES) * 8;
             kr[i] = *(const u32x4 *)(kp + o);
             vr[i] = *(const u32x4 *)(vp + o);
         }
@@ -891,7 +916,7 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
             if (!whole) {
                 if (!bl.seen(blk * TILE_KEYS + row))
                     vr[i] = u32x4{0, 0, 0, 0};
-                else if (has_nonfinite<TQ>(vr[i]))
+                else if (!PRE && has_nonfinite<TQ>(vr[i]))
                     atomicOr((unsigned long long *)&odd[i0 & 3], 1ull << row);
             }
             *(u32x4 *)(vs[buf] + to) = vr[i];
@@ -927,7 +952,7 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
                 for (int x = 0; x < D / 32; ++x)
                     k[u][x] = *(const vec *)(kb + v_piece<D>(16 * u + (lane & 15), g + 4 * x) * 16);
             vec p[RT][TQ::parts];
-            if (!whole)
+            if (!PRE && !whole)
                 again |= __builtin_amdgcn_readfirstlane((uint32_t)(odd[i & 3] >> (32 * sub)));
             floatx4 s[RT][2];
 #pragma unroll
@@ -946,13 +971,13 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
 #pragma unroll
                 for (int t = 0; t < RT; ++t) {
                     const int32_t from =
-                        a.window && (uint32_t)max(pos[t], 0) >= a.window ? pos[t] - (int32_t)a.window : -1;
+                        window && (uint32_t)max(pos[t], 0) >= window ? pos[t] - (int32_t)window : -1;
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int32_t j = (int32_t)j0 + 16 * u + 4 * g + e;
-                            const bool hidden = (j > pos[t]) | ((j <= from) & ((uint32_t)j >= a.sinks));
+                            const bool hidden = (j > pos[t]) | ((j <= from) & ((uint32_t)j >= sinks));
                             s[t][u][e] = hidden ? -INFINITY : s[t][u][e];
                         }
                 }
@@ -973,8 +998,8 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
         if (i + 2 < b1)
             load(bl.block(i + 2));
     }
-    const bool final = a.own_splits + a.prefix_splits == 1;
-    if (again) { // uniform; rare
+    const bool final = !PRE && a.own_splits + a.prefix_splits == 1;
+    if (!PRE && again) { // uniform; rare (over the prefix all rows see the same slots)
         for (uint32_t x = 0; x < 16 * RT && w0 + x < total; ++x) {
             const uint32_t row = pairs.row_of(x);
             attn_row<TQ, D>(a, bl, b0, b1, kp, vp, row, kh * G + pairs.head_of(x), first + (int32_t)row - lo, split,
@@ -999,7 +1024,7 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
             if (g == 0)
                 finish_row(a, row * a.r.heads + h, empty, off, l);
         } else {
-            const size_t to = ((size_t)split * a.r.n_rows + row) * a.r.heads + h;
+            const size_t to = ((size_t)(PRE ? a.own_splits + split : split) * a.r.n_rows + row) * a.r.heads + h;
 #pragma unroll
             for (int n = 0; n < D / 16; ++n)
                 *(floatx4 *)(a.o + to * D + 16 * n + 4 * g) = S.o[t][n];
@@ -1009,24 +1034,27 @@ template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_tile(
     }
 }
 
-#define SUM_KEYS 64
-#define SUM_WAVES 8
 // The weights that SUM_KEYS slots of one (sequence, kv head) receive from all rows: scores
 // once more, with the slots as A operands in registers and 16 (token, head) pairs at a time
-// as B operands, a wave every SUM_WAVES-th, the next pairs' loads in flight.  A lane's scores
-// are of one row (its softmax state: offset and 1 / sum) and four slots a tile; it adds its
-// slots' weights 2^(s c - offset) / sum over its rows.  The lanes' and the waves' sums are
-// joined in a fixed order.
+// as B operands, a wave every SUM_WAVES-th, two of a wave's tiles of pairs in flight beside
+// the one in use.  A lane's scores are of one row (its softmax state: offset and 1 / sum) and
+// four slots a tile; it adds its slots' weights 2^(s c - offset) / sum over its rows.  The
+// lanes' and the waves' sums are joined in a fixed order.
+//
+// Early slots are seen by more rows than late ones: workgroups take the first half of the
+// slots from the front and then the second half from the back, so that those that share a CU
+// add up to the same.
 template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const AttnOpArgs &a)
 {
     typedef typename TQ::vec vec;
     constexpr int KT = SUM_KEYS / 16;
     __shared__ float part[SUM_WAVES][SUM_KEYS];
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4;
-    const uint32_t kh = blockIdx.y, b = blockIdx.z, G = a.group;
-    const uint32_t n = (uint32_t)clamp_len(a.own, b), j0 = blockIdx.x * SUM_KEYS;
-    if (j0 >= n)
+    const uint32_t kh = blockIdx.x % a.own.kv_heads, order = blockIdx.x / a.own.kv_heads, b = blockIdx.y, G = a.group;
+    const uint32_t n = (uint32_t)clamp_len(a.own, b), blocks = (n + SUM_KEYS - 1) / SUM_KEYS;
+    if (order >= blocks)
         return;
+    const uint32_t half = (blocks + 1) / 2, j0 = (order < half ? order : blocks - 1 - (order - half)) * SUM_KEYS;
     int32_t lo, hi;
     seq_rows(a.r, b, &lo, &hi);
     const uint32_t total = (uint32_t)(hi - lo) * G;
@@ -1041,48 +1069,64 @@ template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const
             k[t][x] = *(const vec *)(p + 32 * x);
     }
     floatx4 sum[KT] = {};
-    struct Next {
+    // pairs before the first that sees slot j0 add nothing
+    const uint32_t from = (int32_t)j0 > first ? ((j0 - first) * G) / 16 : 0, end = (total + 15) / 16;
+    struct Tile {
         Queries<TQ, D, 1> q;
         float2 st;
         int32_t pos;
     };
-    auto load = [&](uint32_t i0, Next &x) {
-        const Pairs pairs((uint32_t)lo, i0 * 16, G);
-        const bool in = i0 * 16 + (lane & 15) < total;
-        const uint32_t row = pairs.row_of(lane & 15), h = kh * G + pairs.head_of(lane & 15);
-        load_row<TQ, D, 1>(x.q, 0, a.r, in, row, h);
-        x.st = in ? a.stats[(size_t)row * a.r.heads + h] : make_float2(0.f, 0.f);
-        x.pos = in ? first + (int32_t)row - lo : -1;
-    };
-    // pairs before the first that sees slot j0 add nothing
-    const uint32_t from = (int32_t)j0 > first ? ((j0 - first) * G) / 16 : 0, end = (total + 15) / 16;
-    Next cur, nxt;
     uint32_t i0 = from + wave;
-    if (i0 < end)
-        load(i0, nxt);
-    for (; i0 < end; i0 += SUM_WAVES) {
-        cur = nxt;
-        if (i0 + SUM_WAVES < end)
-            load(i0 + SUM_WAVES, nxt);
-        const bool whole = __ballot(cur.pos < (int32_t)(j0 + SUM_KEYS - 1)) == 0;
+    Pairs pairs((uint32_t)lo, i0 * 16, G); // of the tile that is loaded next
+    const uint32_t step_rows = SUM_WAVES * 16 / G, step_rem = SUM_WAVES * 16 % G;
+    uint32_t ahead = i0;
+    auto load = [&](Tile &x) {
+        const bool in = ahead * 16 + (lane & 15) < total;
+        const uint32_t row = in ? pairs.row_of(lane & 15) : (uint32_t)lo, h = kh * G + (in ? pairs.head_of(lane & 15) : 0);
+        if (ahead < end) { // uniform
+            load_row<TQ, D, 1>(x.q, 0, a.r, in, row, h);
+            x.st = in ? a.stats[(size_t)row * a.r.heads + h] : make_float2(0.f, 0.f);
+        }
+        x.pos = in ? first + (int32_t)row - lo : -1;
+        ahead += SUM_WAVES;
+        pairs.row += step_rows, pairs.rem += step_rem;
+        if (pairs.rem >= G)
+            pairs.rem -= G, ++pairs.row;
+    };
+    auto use = [&](const Tile &x) {
+        const bool whole = __ballot(x.pos < (int32_t)(j0 + SUM_KEYS - 1)) == 0;
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
             floatx4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int x = 0; x < D / 32; ++x)
+            for (int i = 0; i < D / 32; ++i)
 #pragma unroll
                 for (int y = 0; y < TQ::parts; ++y)
-                    s = mma(k[t][x], cur.q.q[0][y][x], s);
+                    s = mma(k[t][i], x.q.q[0][y][i], s);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float w = exp2_hw(fmaf(s[e], cur.q.c[0], -cur.st.x));
-                const float to = fmaf(w, cur.st.y, sum[t][e]);
+                const float w = exp2_hw(fmaf(s[e], x.q.c[0], -x.st.x));
+                const float to = fmaf(w, x.st.y, sum[t][e]);
                 if (whole)
                     sum[t][e] = to;
                 else // a row's NaN stays with the slots it sees
-                    sum[t][e] = (int32_t)(j0 + 16 * t + 4 * g + e) <= cur.pos ? to : sum[t][e];
+                    sum[t][e] = (int32_t)(j0 + 16 * t + 4 * g + e) <= x.pos ? to : sum[t][e];
             }
         }
+    };
+    Tile x0, x1, x2;
+    load(x0), load(x1);
+    for (; i0 < end; i0 += 3 * SUM_WAVES) {
+        load(x2);
+        use(x0);
+        if (i0 + SUM_WAVES >= end)
+            break;
+        load(x0);
+        use(x1);
+        if (i0 + 2 * SUM_WAVES >= end)
+            break;
+        load(x1);
+        use(x2);
     }
     // the 16 lanes of a slot's row are its rows' sums
 #pragma unroll
@@ -1133,24 +1177,26 @@ STEPS(F16, f16, 128, 2)
 STEPS(BF16, bf16, 64, 4)
 STEPS(BF16, bf16, 128, 2)
 
-#define TILE(TQ, tag, D, RT)                                                                                   \
-    extern "C" __global__ __launch_bounds__(256, D == 128 ? 2 : TQ::parts == 2 ? 3 : 4) void k_attn_tile_##tag##_##D##_r##RT(const AttnOpArgs a)   \
+#define TILE(TQ, tag, D, RT, PRE, name)                                                                        \
+    extern "C" __global__ __launch_bounds__(256, D == 128 ? 2 : TQ::parts == 2 ? 3 : 4) void                   \
+    k_attn_##name##_##tag##_##D##_r##RT(const AttnOpArgs a)                                                    \
     {                                                                                                          \
-        attn_tile<TQ, D, RT>(a);                                                                               \
+        attn_tile<TQ, D, RT, PRE>(a);                                                                          \
     }
-#define TILES(TQ, tag, D, MOST)                                                                                \
-    TILE(TQ, tag, D, 1)                                                                                        \
-    TILE(TQ, tag, D, MOST)                                                                                     \
+#define TILES(TQ, tag, D)                                                                                      \
+    TILE(TQ, tag, D, 1, false, tile)                                                                           \
+    TILE(TQ, tag, D, 2, false, tile)                                                                           \
+    TILE(TQ, tag, D, 2, true, prefix)                                                                          \
     extern "C" __global__ __launch_bounds__(SUM_WAVES * 64) void k_attn_weights_##tag##_##D(const AttnOpArgs a)\
     {                                                                                                          \
         attn_weights<TQ, D>(a);                                                                                \
     }
-TILES(F32, f32, 64, 2)
-TILES(F32, f32, 128, 2)
-TILES(F16, f16, 64, 2)
-TILES(F16, f16, 128, 2)
-TILES(BF16, bf16, 64, 2)
-TILES(BF16, bf16, 128, 2)
+TILES(F32, f32, 64)
+TILES(F32, f32, 128)
+TILES(F16, f16, 64)
+TILES(F16, f16, 128)
+TILES(BF16, bf16, 64)
+TILES(BF16, bf16, 128)
 
 // ------------------------------------------------------------------ eviction
 // Rank of a slot as an integer: NaN below every number, the protected slots above all.
