@@ -12,7 +12,9 @@ from __future__ import annotations
 
 import atexit
 import ctypes as C
+import functools
 import os
+import struct
 import weakref
 from typing import Iterable, List, Optional, Sequence
 
@@ -195,14 +197,14 @@ def lib():
         "lfm_q6k_matvec": (i32, [P, u64, u64, P, P, P]),
         "lfm_q6k_matvec_time": (i32, [P, u32, u64, u64, P, P, u32, pf32]),
         "lfm_q6k_gemm": (i32, [P, u64, u64, P, u32, P, P]),
-        "lfm_attn_window": (i32, [C.POINTER(Kv), C.POINTER(Rows), u32, u32, P, sz, P]),
-        "lfm_attn_window_workspace": (i32, [C.POINTER(Kv), C.POINTER(Rows), u32, u32, C.POINTER(sz)]),
-        "lfm_attn_scored": (i32, [C.POINTER(Kv), C.POINTER(Rows), P, P, P, sz, P]),
-        "lfm_attn_scored_workspace": (i32, [C.POINTER(Kv), C.POINTER(Rows), C.POINTER(sz)]),
-        "lfm_attn_prefix": (i32, [C.POINTER(Kv), C.POINTER(Kv), C.POINTER(Rows), P, sz, P]),
-        "lfm_attn_prefix_workspace": (i32, [C.POINTER(Kv), C.POINTER(Kv), C.POINTER(Rows), C.POINTER(sz)]),
-        "lfm_kv_evict": (i32, [C.POINTER(Kv), P, P, u32, u32, u32, C.POINTER(Kv), P, P, P, sz, P]),
-        "lfm_kv_evict_workspace": (i32, [C.POINTER(Kv), u32, C.POINTER(sz)]),
+        "lfm_attn_window": (i32, [P, P, u32, u32, P, sz, P]),
+        "lfm_attn_window_workspace": (i32, [P, P, u32, u32, C.POINTER(sz)]),
+        "lfm_attn_scored": (i32, [P, P, P, P, P, sz, P]),
+        "lfm_attn_scored_workspace": (i32, [P, P, C.POINTER(sz)]),
+        "lfm_attn_prefix": (i32, [P, P, P, P, sz, P]),
+        "lfm_attn_prefix_workspace": (i32, [P, P, P, C.POINTER(sz)]),
+        "lfm_kv_evict": (i32, [P, P, P, u32, u32, u32, P, P, P, P, sz, P]),
+        "lfm_kv_evict_workspace": (i32, [P, u32, C.POINTER(sz)]),
         "lfm_argmax": (i32, [P, u32, pu32, pf32]),
         "lfm_argmax_noalloc": (i32, [P, u32, pu32, pf32]),
         "lfm_synth_default_opts": (None, [C.POINTER(SynthOpts)]),
@@ -659,6 +661,7 @@ class DeviceTensor:
         return self.buf.download(np.uint16 if self.dtype == "bf16" else self.dtype)
 
 
+@functools.lru_cache(maxsize=256)
 def _row_major(shape):
     out, n = [], 1
     for d in reversed(shape):
@@ -670,18 +673,26 @@ def _row_major(shape):
 _DTYPES = {"float32": "f32", "torch.float32": "f32", "float16": "f16", "torch.float16": "f16",
            "bf16": "bf16", "torch.bfloat16": "bf16", "int32": "i32", "torch.int32": "i32"}
 _TYPES = {"f32": TYPE_F32, "f16": TYPE_F16, "bf16": TYPE_BF16}
+_known_dtypes = {}  # dtype object -> name
 
 
 def _dtype(t) -> str:
-    return _DTYPES.get(str(t.dtype), str(t.dtype))
+    d = t.dtype
+    name = _known_dtypes.get(d)
+    if name is None:
+        name = _known_dtypes[d] = _DTYPES.get(str(d), str(d))
+    return name
 
 
 def _dense(t, what: str, dtype: str, shape) -> int:
     """Address of a row-major device array of this type and shape."""
-    if _dtype(t) != dtype or tuple(t.shape) != tuple(shape) or \
-            any(n > 1 and s != r for n, s, r in zip(shape, t.stride(), _row_major(shape))):
-        raise LfmError(LFM_EINVAL, f"{what}: a row-major {dtype} array of {tuple(shape)} expected, got "
-                       f"{_dtype(t)} {tuple(t.shape)} with strides {tuple(t.stride())}")
+    have = tuple(t.shape)
+    if _dtype(t) != dtype or have != shape or tuple(t.stride()) != _row_major(shape):
+        # a dimension of size one may have any stride: it is never used
+        if _dtype(t) != dtype or have != tuple(shape) or \
+                any(n > 1 and s != r for n, s, r in zip(shape, t.stride(), _row_major(shape))):
+            raise LfmError(LFM_EINVAL, f"{what}: a row-major {dtype} array of {tuple(shape)} expected, got "
+                           f"{_dtype(t)} {have} with strides {tuple(t.stride())}")
     return t.data_ptr()
 
 
@@ -707,29 +718,38 @@ class KvCache:
         self._c = Kv(k.data_ptr(), v.data_ptr(), _dense(length, "length", "i32", (n,)),
                      ks[0] if n > 1 else 0, ks[1] if heads > 1 else 0, ks[2] if slots > 1 else 0, kind, n,
                      heads, slots, dim)
-        self._ref = C.byref(self._c)
+        self._ref = C.addressof(self._c)
+        self._acc_shape = (n, heads, slots)
 
 
-def _rows(q, cache: KvCache, out, start, scale, lse):
-    if len(q.shape) != 3 or q.shape[2] != cache.head_dim:
-        raise LfmError(LFM_EINVAL, f"q: [n_rows][heads][{cache.head_dim}] expected, got {tuple(q.shape)}")
-    n, heads, dim = q.shape
-    qs = q.stride()
+# lfm_rows as bytes: a third of the time that filling the ctypes structure takes
+_pack_rows = struct.Struct("@PPPPqqqqIIIf").pack
+assert struct.calcsize("@PPPPqqqqIIIf") == C.sizeof(Rows)
+
+
+def _rows(q, cache: KvCache, out, start, scale, lse) -> bytes:
+    shape, qs = tuple(q.shape), q.stride()
+    if len(shape) != 3 or shape[2] != cache.head_dim:
+        raise LfmError(LFM_EINVAL, f"q: [n_rows][heads][{cache.head_dim}] expected, got {shape}")
+    n, heads, dim = shape
     kind = _TYPES.get(_dtype(q))
     if kind is None or qs[2] != 1:
         raise LfmError(LFM_EINVAL, f"q: {_dtype(q)} with strides {tuple(qs)} (float32, binary16 or bfloat16, the last "
                        "dimension contiguous)")
-    os_, optr = qs, None
+    os_, optr = qs, 0
     if out is not None:
         os_ = out.stride()
-        if tuple(out.shape) != tuple(q.shape) or _dtype(out) != _dtype(q) or os_[2] != 1:
+        if tuple(out.shape) != shape or _dtype(out) != _dtype(q) or os_[2] != 1:
             raise LfmError(LFM_EINVAL, "out: q's shape and type expected, the last dimension contiguous")
         optr = out.data_ptr()
-    one, single = n > 1, heads > 1
-    return Rows(q.data_ptr(), optr, None if lse is None else _dense(lse, "lse", "f32", (n, heads)),
-                None if start is None else _dense(start, "start", "i32", (cache.n_seq + 1,)),
-                qs[0] if one else 0, qs[1] if single else 0, os_[0] if one else 0, os_[1] if single else 0,
-                kind, heads, n, dim ** -0.5 if scale is None else scale)
+    q0, q1, o0, o1 = qs[0], qs[1], os_[0], os_[1]
+    if n == 1:
+        q0 = o0 = 0
+    if heads == 1:
+        q1 = o1 = 0
+    return _pack_rows(q.data_ptr(), optr, 0 if lse is None else _dense(lse, "lse", "f32", (n, heads)),
+                      0 if start is None else _dense(start, "start", "i32", (cache.n_seq + 1,)), q0, q1, o0, o1,
+                      kind, heads, n, dim ** -0.5 if scale is None else scale)
 
 
 def _space(workspace):
@@ -741,7 +761,7 @@ def _space(workspace):
 
 def attn_window_workspace(q, cache: KvCache, *, window: int = 0, sinks: int = 0, start=None) -> int:
     n = C.c_size_t()
-    _check(lib().lfm_attn_window_workspace(cache._ref, C.byref(_rows(q, cache, None, start, None, None)), window,
+    _check(lib().lfm_attn_window_workspace(cache._ref, _rows(q, cache, None, start, None, None), window,
                                            sinks, C.byref(n)))
     return n.value
 
@@ -755,12 +775,12 @@ def attn_window(q, cache: KvCache, out, workspace, *, window: int = 0, sinks: in
     attn_window_workspace(...) bytes for the same arguments."""
     r = _rows(q, cache, out, start, scale, lse)
     p, n = _space(workspace)
-    _check(lib().lfm_attn_window(cache._ref, C.byref(r), window, sinks, p, n, stream))
+    _check(lib().lfm_attn_window(cache._ref, r, window, sinks, p, n, stream))
 
 
 def attn_scored_workspace(q, cache: KvCache, *, start=None) -> int:
     n = C.c_size_t()
-    _check(lib().lfm_attn_scored_workspace(cache._ref, C.byref(_rows(q, cache, None, start, None, None)),
+    _check(lib().lfm_attn_scored_workspace(cache._ref, _rows(q, cache, None, start, None, None),
                                            C.byref(n)))
     return n.value
 
@@ -771,9 +791,9 @@ def attn_scored(q, cache: KvCache, out, acc_in, acc_out, workspace, *, start=Non
     use receives from its kv head's query heads and the sequence's rows (lfm_attn_scored).
     acc [n_seq][kv_heads][slots] float32; acc_in None counts as zeros, and may be acc_out."""
     r = _rows(q, cache, out, start, scale, lse)
-    shape = (cache.n_seq, cache.kv_heads, cache.slots)
+    shape = cache._acc_shape
     p, n = _space(workspace)
-    _check(lib().lfm_attn_scored(cache._ref, C.byref(r),
+    _check(lib().lfm_attn_scored(cache._ref, r,
                                  None if acc_in is None else _dense(acc_in, "acc_in", "f32", shape),
                                  _dense(acc_out, "acc_out", "f32", shape), p, n, stream))
 
@@ -781,7 +801,7 @@ def attn_scored(q, cache: KvCache, out, acc_in, acc_out, workspace, *, start=Non
 def attn_prefix_workspace(q, prefix: KvCache, cache: KvCache, *, start=None) -> int:
     n = C.c_size_t()
     _check(lib().lfm_attn_prefix_workspace(prefix._ref, cache._ref,
-                                           C.byref(_rows(q, cache, None, start, None, None)), C.byref(n)))
+                                           _rows(q, cache, None, start, None, None), C.byref(n)))
     return n.value
 
 
@@ -791,7 +811,7 @@ def attn_prefix(q, prefix: KvCache, cache: KvCache, out, workspace, *, start=Non
     the whole prefix, then its own sequence up to its position (lfm_attn_prefix)."""
     r = _rows(q, cache, out, start, scale, lse)
     p, n = _space(workspace)
-    _check(lib().lfm_attn_prefix(prefix._ref, cache._ref, C.byref(r), p, n, stream))
+    _check(lib().lfm_attn_prefix(prefix._ref, cache._ref, r, p, n, stream))
 
 
 def kv_evict_workspace(cache: KvCache, keep: int) -> int:
@@ -805,8 +825,7 @@ def kv_evict(cache: KvCache, acc, pos, keep: int, out: KvCache, acc_out, pos_out
     """Keeps ``keep`` slots of every longer sequence, per kv head: the first ``sinks`` and the
     newest ``recent`` positions, then the slots of highest acc (lfm_kv_evict).  In place
     where out is cache, acc_out is acc and pos_out is pos."""
-    a = (cache.n_seq, cache.kv_heads, cache.slots)
-    b = (cache.n_seq, cache.kv_heads, out.slots)
+    a, b = cache._acc_shape, out._acc_shape
     p, n = _space(workspace)
     _check(lib().lfm_kv_evict(cache._ref, _dense(acc, "acc", "f32", a), _dense(pos, "pos", "i32", a), keep, sinks,
                               recent, out._ref, _dense(acc_out, "acc_out", "f32", b),

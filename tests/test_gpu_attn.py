@@ -575,7 +575,7 @@ def test_bad_pointers_are_refused(gpu):
     ws = workspace(gpu, gpu.attn_scored_workspace(r.q, cache.view))
     L = gpu.lib()
     host = np.zeros(1 << 12)
-    good = gpu._rows(r.q, cache.view, r.out, None, None, r.lse)
+    good = gpu.Rows.from_buffer_copy(gpu._rows(r.q, cache.view, r.out, None, None, r.lse))
 
     def rows(**kw):
         x = gpu.Rows.from_buffer_copy(good)
