@@ -765,6 +765,35 @@ template <typename TQ> __device__ __forceinline__ bool has_nonfinite(u32x4 v)
     return bad;
 }
 
+// 16 bytes a lane from memory to shared memory, lane x's to byte `to` + 16 x (uniform),
+// with no register between.  Written out because the compiler makes every read of shared
+// memory wait for such loads, the other buffer's too: whoever reads waits with wait_loads
+// and a barrier.
+__device__ __forceinline__ void load_to_lds(const void *from, uint32_t to)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(void *p)
+{
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)p;
+}
+
+// Until this wave's loads into shared memory have arrived.
+__device__ __forceinline__ void wait_loads()
+{
+    __builtin_amdgcn_s_waitcnt(0x0f70); // vmcnt(0)
+    asm volatile("" ::: "memory");
+}
+
+// A barrier that leaves loads from memory in flight.
+__device__ __forceinline__ void lds_barrier()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f); // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // One row and head over blocks b0 .. b1 of 64 slots, by a wave: a lane's score each, then
 // every lane its dims of the weighted sum, a slot that the row does not see left out whatever
 // it holds.
@@ -839,7 +868,7 @@ template <typename TQ, int D, int RT, bool PRE> __device__ __forceinline__ void 
 {
     typedef typename TQ::vec vec;
     constexpr uint32_t ROWS = 64 * RT, PIECES = D / 8, BYTES = TILE_KEYS * D * 2;
-    constexpr int LD = TILE_KEYS * PIECES / 256; // 16-byte loads of K, and of V, a thread and block
+    constexpr int LD = TILE_KEYS * PIECES / 256; // 16-byte pieces of K, and of V, a thread and block
     __shared__ __attribute__((aligned(16))) uint8_t ks[2][BYTES], vs[2][BYTES];
     __shared__ float weights[4][64]; // attn_row's
     __shared__ uint64_t odd[4];      // slots of a block whose V is not all finite
@@ -896,48 +925,53 @@ template <typename TQ, int D, int RT, bool PRE> __device__ __forceinline__ void 
 
     const int64_t at0 = (int64_t)b * c.ss + (int64_t)kh * c.hs;
     const uint16_t *kp = c.k + at0, *vp = c.v + at0;
-    u32x4 kr[LD], vr[LD];
-    auto load = [&](uint32_t blk) {
+    // A block's K and V from memory straight into shared memory: thread x's piece i goes to
+    // place 256 i + x, so the exchange of pieces is made in the address that it reads.  Past
+    // the last visible slot that one is read again.
+    const uint32_t row_in = tid / PIECES, piece_in = (tid % PIECES) ^ (row_in & (PIECES - 1));
+    const uint16_t *const kl = kp + (int64_t)row_in * c.ts + piece_in * 8, *const vl = vp + (kl - kp);
+    const uint32_t ks_at = __builtin_amdgcn_readfirstlane(lds_address(ks)),
+                   vs_at = __builtin_amdgcn_readfirstlane(lds_address(vs));
+    auto fetch = [&](uint32_t blk, uint32_t buf) {
+        const bool inside = blk * TILE_KEYS + TILE_KEYS <= bl.hi;
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
-            const uint32_t j = min(blk * TILE_KEYS + (i * 256 + tid) / PIECES, bl.hi - 1);
-            const int64_t o = (int64_t)j * c.ts + (tid % PIECES) * 8;
-            kr[i] = *(const u32x4 *)(kp + o);
-            vr[i] = *(const u32x4 *)(vp + o);
-        }
-    };
-    // slots past the last visible one repeat it in K and are zeros in V
-    auto store = [&](uint32_t i0, uint32_t blk, uint32_t buf) {
-        const bool whole = all.whole(blk);
-#pragma unroll
-        for (int i = 0; i < LD; ++i) {
-            const uint32_t row = (i * 256 + tid) / PIECES, to = v_piece<D>(row, tid % PIECES) * 16;
-            *(u32x4 *)(ks[buf] + to) = kr[i];
-            if (!whole) {
-                if (!bl.seen(blk * TILE_KEYS + row))
-                    vr[i] = u32x4{0, 0, 0, 0};
-                else if (!PRE && has_nonfinite<TQ>(vr[i]))
-                    atomicOr((unsigned long long *)&odd[i0 & 3], 1ull << row);
-            }
-            *(u32x4 *)(vs[buf] + to) = vr[i];
+            const uint32_t row = blk * TILE_KEYS + i * (256 / PIECES);
+            int64_t o = (int64_t)row * c.ts;
+            if (!inside)
+                o = ((int64_t)min(row + row_in, bl.hi - 1) - row_in) * c.ts;
+            const uint32_t to = buf * BYTES + (i * 256 + wave * 64) * 16;
+            load_to_lds(kl + o, ks_at + to);
+            load_to_lds(vl + o, vs_at + to);
         }
     };
     if (tid < 4)
         odd[tid] = 0;
-    __syncthreads();
-    if (b0 < b1) {
-        load(bl.block(b0));
-        store(b0, bl.block(b0), 0);
-    }
-    if (b0 + 1 < b1)
-        load(bl.block(b0 + 1));
+    if (b0 < b1)
+        fetch(bl.block(b0), 0);
     const uint32_t at = v_lane<D>(lane);
-    uint32_t again = 0;
+    bool again = false;
     for (uint32_t i = b0; i < b1; ++i) {
         const uint32_t blk = bl.block(i), buf = (i - b0) & 1;
+        wait_loads();
         __syncthreads();
+        if (i + 1 < b1)
+            fetch(bl.block(i + 1), buf ^ 1);
         if (tid == 0)
-            odd[(i + 2) & 3] = 0; // used last at i - 2, filled next at i + 1
+            odd[(i + 2) & 3] = 0; // used last at i - 2, filled next at i + 2
+        if (!all.whole(blk)) {
+            // V of slots that no row sees becomes zeros; numbers that are not finite are noted
+#pragma unroll
+            for (int x = 0; x < LD; ++x) {
+                const uint32_t row = (x * 256 + tid) / PIECES;
+                u32x4 *const v = (u32x4 *)(vs[buf] + (x * 256 + tid) * 16);
+                if (!bl.seen(blk * TILE_KEYS + row))
+                    *v = u32x4{0, 0, 0, 0};
+                else if (!PRE && has_nonfinite<TQ>(*v))
+                    atomicOr((unsigned long long *)&odd[i & 3], 1ull << row);
+            }
+            lds_barrier();
+        }
 #pragma unroll
         for (uint32_t sub = 0; sub < 2; ++sub) {
             const uint32_t j0 = blk * TILE_KEYS + 32 * sub;
@@ -993,10 +1027,6 @@ template <typename TQ, int D, int RT, bool PRE> __device__ __forceinline__ void 
                         S.o[t][n] = mma(v, p[t][y], S.o[t][n]);
             }
         }
-        if (i + 1 < b1)
-            store(i + 1, bl.block(i + 1), buf ^ 1);
-        if (i + 2 < b1)
-            load(bl.block(i + 2));
     }
     const bool final = !PRE && a.own_splits + a.prefix_splits == 1;
     if (!PRE && again) { // uniform; rare (over the prefix all rows see the same slots)
