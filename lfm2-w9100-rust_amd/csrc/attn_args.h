@@ -28,8 +28,8 @@ struct RowsView {
 #define MAX_GROUP 128     // query heads of a kv head
 #define TILE_TILES 2      // row tiles a wave of the larger tile kernel
 #define SCORED_SLOTS 1024 // slots a workgroup of k_scored_join
-#define SUM_KEYS 32       // slots a workgroup of k_attn_weights
-#define SUM_WAVES 8
+#define SUM_KEYS 256      // slots a workgroup of k_attn_weights: four waves of 64
+#define MOST_SUM_PARTS 16 // parts of the rows that k_attn_weights sums apart
 
 struct AttnOpArgs {
     KvView own;    // slots of the row's own sequence, causal
@@ -50,6 +50,8 @@ struct AttnOpArgs {
     // rounded up to whole blocks
     float *scores;
     uint32_t score_row;
+    uint32_t sum_parts;
+    float *sums;   // [sum_parts][n_seq][kv_heads][slots] where there is more than one
     float2 *stats; // nullable: per row and head {log2 offset, 1 / sum} of its weights
     const float *acc; // nullable
     float *acc_out;   // [n_seq][kv_heads][slots]

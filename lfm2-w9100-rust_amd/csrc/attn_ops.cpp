@@ -31,7 +31,7 @@ struct AttnKernels {
     hipModule_t mod = nullptr;
     hipFunction_t tile_1[3][2], tile_most[3][2], tile_prefix[3][2], weights[3][2];
     hipFunction_t step_1[3][2], step_most[3][2], merge[3][2], scored_join[3][2];
-    hipFunction_t kv_select, kv_move;
+    hipFunction_t sums, kv_select, kv_move;
 };
 
 static std::mutex g_mu;
@@ -69,6 +69,8 @@ static int load_attn(int dev)
                 if (rc == LFM_OK)
                     rc = get(f.f, f.name);
         }
+    if (rc == LFM_OK)
+        rc = get(&k.sums, "k_attn_sums");
     if (rc == LFM_OK)
         rc = get(&k.kv_select, "k_kv_select");
     if (rc == LFM_OK)
@@ -255,8 +257,9 @@ struct Plan {
     bool tile_prefix = false; // the prefix goes through the tile kernel too
     uint64_t tile_items = 0;
     bool join = false; // a second kernel joins the key ranges
-    size_t ml_bytes = 0, o_bytes = 0, score_bytes = 0, stat_bytes = 0;
-    size_t bytes() const { return ml_bytes + o_bytes + score_bytes + stat_bytes; }
+    uint32_t sum_parts = 1; // of the rows, in the slots' weights
+    size_t ml_bytes = 0, o_bytes = 0, score_bytes = 0, stat_bytes = 0, sum_bytes = 0;
+    size_t bytes() const { return ml_bytes + o_bytes + score_bytes + stat_bytes + sum_bytes; }
 };
 
 
@@ -310,8 +313,9 @@ static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint
         p.prefix_groups = (uint32_t)(((uint64_t)r->n_rows * G + rows - 1) / rows);
         const uint64_t pitems = (uint64_t)std::max(1u, p.prefix_groups) * kv->kv_heads;
         const uint64_t blocks = (prefix->slots + 31) / 32;
-        const uint64_t wanted = p.tile_prefix && kv->head_dim == 64 ? 2 * TARGET_GROUPS : TARGET_GROUPS;
-        p.prefix_splits = ranges(wanted / pitems, blocks / (blocks > 64 ? 8 : 4));
+        // (a tile's range of 16 blocks: 64 sequences over 8192 slots take 31 us in ranges of
+        // 16, 35 in ranges of 8, whose joining costs more)
+        p.prefix_splits = ranges(TARGET_GROUPS / pitems, blocks / (blocks > 64 ? (p.tile_prefix ? 16 : 8) : 4));
     }
     const uint32_t splits = p.own_splits + p.prefix_splits;
     const bool steps = scored && !r->start; // scores are kept from the step to the join
@@ -322,8 +326,16 @@ static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint
     }
     if (steps)
         p.score_bytes = round256((size_t)pairs * score_row(kv) * 4);
-    else if (scored)
+    else if (scored) {
         p.stat_bytes = round256((size_t)pairs * 8);
+        // parts of eight steps of 64 pairs and more (one sequence's rows are at most all of them)
+        const uint64_t groups = (uint64_t)((kv->slots + SUM_KEYS - 1) / SUM_KEYS) * kv->kv_heads * std::max(1u, kv->n_seq);
+        p.sum_parts = (uint32_t)std::min<uint64_t>(
+            {MOST_SUM_PARTS, std::max<uint64_t>(1, 2 * TARGET_GROUPS / groups),
+             std::max<uint64_t>(1, (uint64_t)r->n_rows * G / 512)});
+        if (p.sum_parts > 1)
+            p.sum_bytes = round256((size_t)p.sum_parts * kv->n_seq * kv->kv_heads * kv->slots * 4);
+    }
     return p;
 }
 
@@ -348,6 +360,9 @@ static AttnOpArgs op_args(const Plan &p, const lfm_kv *prefix, const lfm_kv *kv,
     a.scores = p.score_bytes ? (float *)w : nullptr;
     w += p.score_bytes;
     a.stats = p.stat_bytes ? (float2 *)w : nullptr;
+    w += p.stat_bytes;
+    a.sum_parts = p.sum_parts;
+    a.sums = (float *)w;
     return a;
 }
 
@@ -459,7 +474,10 @@ extern "C" int lfm_attn_scored(const lfm_kv *kv, const lfm_rows *rows, const flo
     const uint64_t blocks = (uint64_t)(kv->slots + SUM_KEYS - 1) / SUM_KEYS * kv->kv_heads;
     if (blocks > 0x7FFFFFFFull)
         return fail(LFM_EINVAL, "%s: %u slots of %u kv heads", op, kv->slots, kv->kv_heads);
-    return launch(K->weights[rows->type][dim_index(kv)], dim3((uint32_t)blocks, kv->n_seq), SUM_WAVES * 64, s, a);
+    RC(launch(K->weights[rows->type][dim_index(kv)], dim3((uint32_t)blocks, kv->n_seq * p.sum_parts), 256, s, a));
+    if (p.sum_parts == 1)
+        return LFM_OK;
+    return launch(K->sums, dim3((kv->slots + 255) / 256, kv->kv_heads, kv->n_seq), 256, s, a);
 }
 
 static int check_prefix(const char *op, const lfm_kv *prefix, const lfm_kv *kv)

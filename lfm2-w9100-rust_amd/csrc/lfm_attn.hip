@@ -160,6 +160,14 @@ template <typename TQ, int D, int RT> struct Queries {
     __device__ __forceinline__ float c_of(int t) const { return c[N == 1 ? 0 : t]; }
 };
 
+__device__ __forceinline__ int power_up(float top)
+{
+    int ex = 14;
+    if (top > 0.f && top < INFINITY)
+        frexpf(top, &ex);
+    return min(14 - ex, 126);
+}
+
 template <typename TQ, int D, int RT>
 __device__ __forceinline__ void load_row(Queries<TQ, D, RT> &Q, int t, const RowsView &r, bool valid, uint32_t row,
                                          uint32_t h)
@@ -192,10 +200,7 @@ __device__ __forceinline__ void load_row(Queries<TQ, D, RT> &Q, int t, const Row
             }
         }
         top = row_max(top);
-        int ex = 14;
-        if (top > 0.f && top < INFINITY)
-            frexpf(top, &ex);
-        const int up = min(14 - ex, 126);
+        const int up = power_up(top);
         const float s = ldexpf(1.f, up);
         Q.back[t] = ldexpf(1.f, -up);
         Q.c[t] = r.cexp * Q.back[t];
@@ -873,10 +878,10 @@ template <typename TQ, int D, int RT, bool PRE> __device__ __forceinline__ void 
     __shared__ float weights[4][64]; // attn_row's
     __shared__ uint64_t odd[4];      // slots of a block whose V is not all finite
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4;
-    const uint32_t kh = blockIdx.x % a.own.kv_heads, G = a.group;
+    const uint32_t kh = blockIdx.x % a.own.kv_heads, flat = blockIdx.x / a.own.kv_heads, G = a.group;
     const KvView &c = PRE ? a.prefix : a.own;
     const uint32_t splits = PRE ? a.prefix_splits : a.own_splits;
-    const uint32_t flat = blockIdx.x / a.own.kv_heads, split = splits == 1 ? 0 : flat % splits;
+    const uint32_t split = splits == 1 ? 0 : flat % splits;
     // rows lo .. hi of one sequence, row lo at position `first` and each next one `step` further;
     // over the prefix all rows, each at its last position
     uint32_t b = 0, tile, tiles;
@@ -887,7 +892,11 @@ template <typename TQ, int D, int RT, bool PRE> __device__ __forceinline__ void 
     } else {
         if (!find_item(a.r, a.own.n_seq, splits == 1 ? flat : flat / splits, G, ROWS, &b, &tile, &tiles))
             return;
-        tile = tiles - 1 - tile; // the longest first
+        // The longest first, every second 32 (an XCD's CUs) in reverse: a CU's workgroups add
+        // up to about the same.
+        if (tile & 32 && (tile | 31) < tiles)
+            tile ^= 31;
+        tile = tiles - 1 - tile;
         seq_rows(a.r, b, &lo, &hi);
         first = clamp_len(c, b) - (hi - lo);
     }
@@ -1064,101 +1073,168 @@ template <typename TQ, int D, int RT, bool PRE> __device__ __forceinline__ void 
     }
 }
 
-// The weights that SUM_KEYS slots of one (sequence, kv head) receive from all rows: scores
-// once more, with the slots as A operands in registers and 16 (token, head) pairs at a time
-// as B operands, a wave every SUM_WAVES-th, two of a wave's tiles of pairs in flight beside
-// the one in use.  A lane's scores are of one row (its softmax state: offset and 1 / sum) and
-// four slots a tile; it adds its slots' weights 2^(s c - offset) / sum over its rows.  The
-// lanes' and the waves' sums are joined in a fixed order.
-//
-// Early slots are seen by more rows than late ones: workgroups take the first half of the
-// slots from the front and then the second half from the back, so that those that share a CU
-// add up to the same.
+// The weights that SUM_KEYS slots of one (sequence, kv head) receive from a part of its rows:
+// scores once more, a wave's 32 slots as A operands in registers and (token, head) pairs, 64
+// at a time through two buffers of shared memory, as B operands.  A lane's scores are of one
+// row (its softmax state: offset and 1 / sum) and four slots a tile; it adds its slots'
+// weights 2^(s c - offset) / sum over its rows, and the 16 lanes of a slot are added at the
+// end, all in a fixed order.  (Rows read as operands by every wave for itself, 16 rows a load,
+// kept the first-level cache busy with 64-byte pieces: a prompt of 2048 tokens, 32 heads over
+// 8 of 64 dims, took 42 us so, 29 this way and 5 for the adding of the parts.)
 template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const AttnOpArgs &a)
 {
     typedef typename TQ::vec vec;
-    constexpr int KT = SUM_KEYS / 16;
-    __shared__ float part[SUM_WAVES][SUM_KEYS];
+    typedef typename TQ::type tq;
+    constexpr uint32_t STEP = 64, PIECES = D / 8, BYTES = STEP * D * 2;
+    constexpr int PER = STEP * PIECES / 256; // pieces of 8 numbers a thread and step
+    constexpr int KT = SUM_KEYS / 4 / 16;    // tiles of 16 slots a wave
+    struct Row {
+        float c, offset, inverse;
+        int32_t pos;
+    };
+    __shared__ __attribute__((aligned(16))) uint8_t qs[2][TQ::parts][BYTES];
+    __shared__ __attribute__((aligned(16))) Row rows[2][STEP];
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4;
-    const uint32_t kh = blockIdx.x % a.own.kv_heads, order = blockIdx.x / a.own.kv_heads, b = blockIdx.y, G = a.group;
-    const uint32_t n = (uint32_t)clamp_len(a.own, b), blocks = (n + SUM_KEYS - 1) / SUM_KEYS;
-    if (order >= blocks)
+    const uint32_t kh = blockIdx.x % a.own.kv_heads, G = a.group;
+    uint32_t tile = blockIdx.x / a.own.kv_heads;
+    const uint32_t b = a.sum_parts == 1 ? blockIdx.y : blockIdx.y / a.sum_parts, part = blockIdx.y - b * a.sum_parts;
+    const uint32_t n = (uint32_t)clamp_len(a.own, b), tiles = (n + SUM_KEYS - 1) / SUM_KEYS;
+    if (tile >= tiles)
         return;
-    const uint32_t half = (blocks + 1) / 2, j0 = (order < half ? order : blocks - 1 - (order - half)) * SUM_KEYS;
+    // early slots are seen by more rows: each part starts with another one, so that a CU's
+    // workgroups differ
+    tile = (tile + blockIdx.y + blockIdx.y / 4) % tiles;
+    const uint32_t j0 = tile * SUM_KEYS;
     int32_t lo, hi;
     seq_rows(a.r, b, &lo, &hi);
     const uint32_t total = (uint32_t)(hi - lo) * G;
     const int32_t first = (int32_t)n - (hi - lo);
+    // steps of 64 pairs: those before the first that sees slot j0 add nothing; of the others
+    // this part's
+    const uint32_t skipped = (int32_t)j0 > first ? (uint32_t)((int32_t)j0 - first) * G / STEP : 0;
+    uint32_t s0, s1;
+    share((total + STEP - 1) / STEP - min(skipped, (total + STEP - 1) / STEP), part, a.sum_parts, &s0, &s1);
+    s0 += skipped, s1 += skipped;
+    const uint32_t jw = j0 + 16 * KT * wave; // the wave's slots
     vec k[KT][D / 32];
     const uint16_t *kp = a.own.k + (int64_t)b * a.own.ss + (int64_t)kh * a.own.hs + 8 * g;
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
-        const uint16_t *p = kp + (int64_t)min(j0 + 16 * t + (lane & 15), n - 1) * a.own.ts;
+        const uint16_t *p = kp + (int64_t)min(jw + 16 * t + (lane & 15), n - 1) * a.own.ts;
 #pragma unroll
         for (int x = 0; x < D / 32; ++x)
             k[t][x] = *(const vec *)(p + 32 * x);
     }
     floatx4 sum[KT] = {};
-    // pairs before the first that sees slot j0 add nothing
-    const uint32_t from = (int32_t)j0 > first ? ((j0 - first) * G) / 16 : 0, end = (total + 15) / 16;
-    struct Tile {
-        Queries<TQ, D, 1> q;
-        float2 st;
-        int32_t pos;
-    };
-    uint32_t i0 = from + wave;
-    Pairs pairs((uint32_t)lo, i0 * 16, G); // of the tile that is loaded next
-    const uint32_t step_rows = SUM_WAVES * 16 / G, step_rem = SUM_WAVES * 16 % G;
-    uint32_t ahead = i0;
-    auto load = [&](Tile &x) {
-        const bool in = ahead * 16 + (lane & 15) < total;
-        const uint32_t row = in ? pairs.row_of(lane & 15) : (uint32_t)lo, h = kh * G + (in ? pairs.head_of(lane & 15) : 0);
-        if (ahead < end) { // uniform
-            load_row<TQ, D, 1>(x.q, 0, a.r, in, row, h);
-            x.st = in ? a.stats[(size_t)row * a.r.heads + h] : make_float2(0.f, 0.f);
-        }
-        x.pos = in ? first + (int32_t)row - lo : -1;
-        ahead += SUM_WAVES;
-        pairs.row += step_rows, pairs.rem += step_rem;
-        if (pairs.rem >= G)
-            pairs.rem -= G, ++pairs.row;
-    };
-    auto use = [&](const Tile &x) {
-        const bool whole = __ballot(x.pos < (int32_t)(j0 + SUM_KEYS - 1)) == 0;
+    // a thread's pieces of a step, and the state of the row that it holds for thread < 64
+    typedef tq tq8 __attribute__((ext_vector_type(8)));
+    tq8 piece[PER];
+    float2 st;
+    int32_t pos = -1;
+    auto load = [&](uint32_t step) {
+        const Pairs pairs((uint32_t)lo, step * STEP, G);
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-            floatx4 s = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t x = (i * 256 + tid) / PIECES, in = step * STEP + x < total ? x : 0;
+            piece[i] = *(const tq8 *)((const tq *)a.r.q + (int64_t)pairs.row_of(in) * a.r.q_rs +
+                                      (int64_t)(kh * G + pairs.head_of(in)) * a.r.q_hs + (tid % PIECES) * 8);
+        }
+        if (tid < STEP) {
+            const uint32_t in = step * STEP + tid < total ? tid : 0, row = pairs.row_of(in);
+            st = a.stats[(size_t)row * a.r.heads + kh * G + pairs.head_of(in)];
+            pos = in == tid ? first + (int32_t)row - lo : -1;
+        }
+    };
+    auto store = [&](uint32_t buf) {
+        if (tid < STEP) {
+            rows[buf][tid].offset = st.x, rows[buf][tid].inverse = st.y, rows[buf][tid].pos = pos;
+            if constexpr (TQ::parts == 1)
+                rows[buf][tid].c = a.r.cexp;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t x = (i * 256 + tid) / PIECES, to = v_piece<D>(x, tid % PIECES) * 16;
+            if constexpr (TQ::parts == 1) {
+                *(vec *)(qs[buf][0] + to) = piece[i];
+            } else { // as load_row does, a row in PIECES neighbouring lanes
+                float top = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    top = fmaxf(top, fabsf(piece[i][e]));
+#pragma unroll
+                for (uint32_t d = 1; d < PIECES; d <<= 1)
+                    top = fmaxf(top, __shfl_xor(top, d));
+                const int up = power_up(top);
+                const float scale = ldexpf(1.f, up);
+                vec hi, lo_;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float y = piece[i][e] * scale;
+                    hi[e] = (_Float16)y;
+                    lo_[e] = (_Float16)(y - (float)hi[e]);
+                }
+                *(vec *)(qs[buf][0] + to) = hi;
+                *(vec *)(qs[buf][1] + to) = lo_;
+                if (tid % PIECES == 0)
+                    rows[buf][x].c = a.r.cexp * ldexpf(1.f, -up);
+            }
+        }
+    };
+    if (s0 < s1) {
+        load(s0);
+        store(0);
+    }
+    for (uint32_t s = s0; s < s1; ++s) {
+        const uint32_t buf = (s - s0) & 1;
+        __syncthreads();
+        if (s + 1 < s1)
+            load(s + 1);
+#pragma unroll 2
+        for (uint32_t x = 0; x < STEP / 16; ++x) {
+            const Row row = rows[buf][16 * x + (lane & 15)];
+            if (__ballot(row.pos >= (int32_t)jw) == 0) // uniform: no row sees the wave's first slot
+                continue;
+            const bool whole = __ballot(row.pos < (int32_t)(jw + 16 * KT - 1)) == 0;
+            vec q[TQ::parts][D / 32];
+#pragma unroll
+            for (int y = 0; y < TQ::parts; ++y)
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i)
+                    q[y][i] = *(const vec *)(qs[buf][y] + v_piece<D>(16 * x + (lane & 15), g + 4 * i) * 16);
+            floatx4 v[KT] = {};
 #pragma unroll
             for (int i = 0; i < D / 32; ++i)
 #pragma unroll
                 for (int y = 0; y < TQ::parts; ++y)
-                    s = mma(k[t][i], x.q.q[0][y][i], s);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float w = exp2_hw(fmaf(s[e], x.q.c[0], -x.st.x));
-                const float to = fmaf(w, x.st.y, sum[t][e]);
-                if (whole)
-                    sum[t][e] = to;
-                else // a row's NaN stays with the slots it sees
-                    sum[t][e] = (int32_t)(j0 + 16 * t + 4 * g + e) <= x.pos ? to : sum[t][e];
+                    for (int t = 0; t < KT; ++t)
+                        v[t] = mma(k[t][i], q[y][i], v[t]);
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[t][e] = exp2_hw(fmaf(v[t][e], row.c, -row.offset));
+            if (whole) { // uniform
+#pragma unroll
+                for (int t = 0; t < KT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        sum[t][e] = fmaf(v[t][e], row.inverse, sum[t][e]);
+                continue;
             }
+            // a row's NaN stays with the slots it sees
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float to = fmaf(v[t][e], row.inverse, sum[t][e]);
+                    sum[t][e] = (int32_t)(jw + 16 * t + 4 * g + e) <= row.pos ? to : sum[t][e];
+                }
         }
-    };
-    Tile x0, x1, x2;
-    load(x0), load(x1);
-    for (; i0 < end; i0 += 3 * SUM_WAVES) {
-        load(x2);
-        use(x0);
-        if (i0 + SUM_WAVES >= end)
-            break;
-        load(x0);
-        use(x1);
-        if (i0 + 2 * SUM_WAVES >= end)
-            break;
-        load(x1);
-        use(x2);
+        if (s + 1 < s1)
+            store(buf ^ 1);
     }
-    // the 16 lanes of a slot's row are its rows' sums
+    // the 16 lanes of a slot are its rows' sums
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -1168,17 +1244,34 @@ template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const
             v += dpp_mov<0x4e>(v, 0.f);  // quad_perm [2,3,0,1]
             v += dpp_mov<0x114>(v, 0.f); // row_shr:4
             v += dpp_mov<0x118>(v, 0.f); // row_shr:8: the row's sum in lane 15 of 16
-            if ((lane & 15) == 15)
-                part[wave][16 * t + 4 * g + e] = v;
+            const uint32_t j = jw + 16 * t + 4 * g + e;
+            if ((lane & 15) == 15 && j < n) {
+                const size_t at = ((size_t)b * a.own.kv_heads + kh) * a.own.slots + j;
+                if (a.sum_parts == 1)
+                    a.acc_out[at] = (a.acc ? a.acc[at] : 0.f) + v;
+                else
+                    a.sums[(size_t)part * a.own.n_seq * a.own.kv_heads * a.own.slots + at] = v;
+            }
         }
-    __syncthreads();
-    if (tid < SUM_KEYS && j0 + tid < n) {
-        float v = 0.f;
-        for (int w = 0; w < SUM_WAVES; ++w)
-            v += part[w][tid];
-        const size_t at = ((size_t)b * a.own.kv_heads + kh) * a.own.slots + j0 + tid;
-        a.acc_out[at] = (a.acc ? a.acc[at] : 0.f) + v;
-    }
+}
+
+// acc_out = acc + the parts of attn_weights, in order.
+extern "C" __global__ __launch_bounds__(256) void k_attn_sums(const AttnOpArgs a)
+{
+    const uint32_t j = blockIdx.x * 256 + threadIdx.x, kh = blockIdx.y, b = blockIdx.z;
+    if (j >= (uint32_t)clamp_len(a.own, b))
+        return;
+    const size_t at = ((size_t)b * a.own.kv_heads + kh) * a.own.slots + j,
+                 part = (size_t)a.own.n_seq * a.own.kv_heads * a.own.slots;
+    float v[MOST_SUM_PARTS];
+#pragma unroll
+    for (uint32_t p = 0; p < MOST_SUM_PARTS; ++p)
+        v[p] = p < a.sum_parts ? a.sums[p * part + at] : 0.f;
+    float sum = 0.f;
+#pragma unroll
+    for (uint32_t p = 0; p < MOST_SUM_PARTS; ++p)
+        sum += v[p];
+    a.acc_out[at] = (a.acc ? a.acc[at] : 0.f) + sum;
 }
 
 // RT: row tiles of a workgroup of rows that see the same slots, as many as the registers
@@ -1217,7 +1310,7 @@ STEPS(BF16, bf16, 128, 2)
     TILE(TQ, tag, D, 1, false, tile)                                                                           \
     TILE(TQ, tag, D, 2, false, tile)                                                                           \
     TILE(TQ, tag, D, 2, true, prefix)                                                                          \
-    extern "C" __global__ __launch_bounds__(SUM_WAVES * 64) void k_attn_weights_##tag##_##D(const AttnOpArgs a)\
+    extern "C" __global__ __launch_bounds__(256) void k_attn_weights_##tag##_##D(const AttnOpArgs a)           \
     {                                                                                                          \
         attn_weights<TQ, D>(a);                                                                                \
     }
