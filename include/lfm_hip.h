@@ -302,7 +302,8 @@ typedef struct lfm_kv {
 /* Query rows and their outputs, q[row][head][d]: row and head strides in elements, in
  * multiples of 16 bytes, not negative; q and out 16-byte aligned and apart.  Types: F16
  * or BF16 as the cache's, or F32 with an F16 cache.  heads is a multiple of the cache's
- * kv_heads; head h reads kv head h * kv_heads / heads.
+ * kv_heads, at most 128 times; head h reads kv head h * kv_heads / heads.  n_rows * heads
+ * is below 2^24.
  * start (device, n_seq + 1 ascending entries) gives sequence b the rows start[b] ..
  * start[b + 1] - 1; NULL: one row per sequence (n_rows = n_seq).  Rows of no sequence
  * are left as they are.  A sequence's rows are its newest tokens, whose K and V are in
@@ -348,7 +349,7 @@ int lfm_attn_prefix_workspace(const lfm_kv *prefix, const lfm_kv *kv, const lfm_
 /* Eviction by accumulated weight.  Where a sequence has more than `keep` slots in use,
  * each kv head keeps `keep` of them: the protected ones (pos < sinks, or among the newest
  * `recent` positions: pos > newest pos - recent), then those of highest acc, ties to the
- * lowest slot, NaN below every number.  sinks + recent is at most keep.  Kept slots below
+ * lowest slot, NaN below every number.  keep is 1..2^28, sinks + recent at most keep.  Kept slots below
  * `keep` stay where they are; the i-th slot that leaves from below `keep` is replaced by
  * the i-th kept slot from `keep` on.  K, V, acc and pos ([n_seq][kv_heads][slots], the
  * position of each slot's token) move alike, and out->len receives min(len, keep).

@@ -108,6 +108,9 @@ template <typename A> static int launch(hipFunction_t f, dim3 grid, uint32_t thr
 }
 
 // ------------------------------------------------------------------ argument checks
+// A grid of 256 threads each stays below 2^32 threads.
+#define MOST_WORKGROUPS 0xFFFFFFu
+
 // Sizes and strides; they decide the workspace and need no device.
 static int check_kv(const char *op, const char *name, const lfm_kv *c)
 {
@@ -139,8 +142,9 @@ static int check_rows(const char *op, const lfm_kv *c, const lfm_rows *r)
     if (r->heads == 0 || r->heads % c->kv_heads || r->heads / c->kv_heads > MAX_GROUP || r->heads > 65535)
         return fail(LFM_EINVAL, "%s: %u heads over %u kv heads (a multiple, at most %u times)", op, r->heads,
                     c->kv_heads, MAX_GROUP);
-    if ((uint64_t)r->n_rows * r->heads > 0x7FFFFFFFu)
-        return fail(LFM_EINVAL, "%s: %u rows of %u heads (2^31 - 1 of them at most)", op, r->n_rows, r->heads);
+    if ((uint64_t)r->n_rows * r->heads > MOST_WORKGROUPS)
+        return fail(LFM_EINVAL, "%s: %u rows of %u heads (%u of them at most)", op, r->n_rows, r->heads,
+                    MOST_WORKGROUPS);
     if (!r->start && r->n_rows != c->n_seq)
         return fail(LFM_EINVAL, "%s: %u rows for %u sequences without start (one row each)", op, r->n_rows, c->n_seq);
     if (!(r->scale > 0.f) || !(r->scale < INFINITY))
@@ -367,12 +371,22 @@ static AttnOpArgs op_args(const Plan &p, const lfm_kv *prefix, const lfm_kv *kv,
 }
 
 // Grids are flat, kv heads fastest: with 8 of them each XCD's cache serves one.
-static int launch_items(hipFunction_t f, uint64_t items, uint32_t kv_heads, uint32_t threads, hipStream_t s,
-                        const AttnOpArgs &a)
+static int launch_items(hipFunction_t f, uint64_t items, uint32_t kv_heads, hipStream_t s, const AttnOpArgs &a)
 {
-    if (items * kv_heads > 0x7FFFFFFFull)
-        return fail(LFM_EINVAL, "attention: %llu work items of %u kv heads", (unsigned long long)items, kv_heads);
-    return launch(f, dim3((uint32_t)items * kv_heads), threads, s, a);
+    return launch(f, dim3((uint32_t)items * kv_heads), 256, s, a);
+}
+
+// Whether the grids of a call can be launched.
+static int check_grids(const char *op, const Plan &p, const lfm_kv *kv, const lfm_rows *r, bool scored)
+{
+    const uint64_t most = std::max({(uint64_t)p.prefix_groups * p.prefix_splits +
+                                        (r->start ? 0 : (uint64_t)r->n_rows * p.own_groups * p.own_splits),
+                                    p.tile_items * p.own_splits,
+                                    scored && r->start ? (uint64_t)(kv->slots + SUM_KEYS - 1) / SUM_KEYS : 0});
+    if (most * kv->kv_heads > MOST_WORKGROUPS)
+        return fail(LFM_EINVAL, "%s: %llu pieces of work for each of %u kv heads", op, (unsigned long long)most,
+                    kv->kv_heads);
+    return LFM_OK;
 }
 
 // Launches over (kv head, rows, key range): the prefix of many rows, then single rows (and the
@@ -384,16 +398,16 @@ static int attend(AttnKernels *K, const Plan &p, AttnOpArgs a, const lfm_kv *kv,
     uint64_t steps = rows->start ? 0 : (uint64_t)rows->n_rows * p.own_groups * p.own_splits;
     a.step_prefix = 0;
     if (p.tile_prefix) {
-        RC(launch_items(K->tile_prefix[t][d], (uint64_t)p.prefix_groups * p.prefix_splits, kv->kv_heads, 256, s, a));
+        RC(launch_items(K->tile_prefix[t][d], (uint64_t)p.prefix_groups * p.prefix_splits, kv->kv_heads, s, a));
     } else {
         a.step_prefix = p.prefix_groups * p.prefix_splits;
         steps += a.step_prefix;
     }
     if (steps)
-        RC(launch_items(p.most ? K->step_most[t][d] : K->step_1[t][d], steps, kv->kv_heads, 256, s, a));
+        RC(launch_items(p.most ? K->step_most[t][d] : K->step_1[t][d], steps, kv->kv_heads, s, a));
     if (rows->start)
         RC(launch_items(p.tile_most ? K->tile_most[t][d] : K->tile_1[t][d], p.tile_items * p.own_splits, kv->kv_heads,
-                        256, s, a));
+                        s, a));
     if (a.scores)
         return launch(K->scored_join[t][d],
                       dim3((kv->slots + SCORED_SLOTS - 1) / SCORED_SLOTS, kv->kv_heads, kv->n_seq), 256, s, a);
@@ -410,7 +424,9 @@ extern "C" int lfm_attn_window_workspace(const lfm_kv *kv, const lfm_rows *rows,
     RC(check_rows(op, kv, rows));
     if (!bytes)
         return fail(LFM_EINVAL, "%s: bytes is null", op);
-    *bytes = plan(nullptr, kv, rows, window, sinks, false).bytes();
+    const Plan p = plan(nullptr, kv, rows, window, sinks, false);
+    RC(check_grids(op, p, kv, rows, false));
+    *bytes = p.bytes();
     return LFM_OK;
 }
 
@@ -440,7 +456,9 @@ extern "C" int lfm_attn_scored_workspace(const lfm_kv *kv, const lfm_rows *rows,
     RC(check_rows(op, kv, rows));
     if (!bytes)
         return fail(LFM_EINVAL, "%s: bytes is null", op);
-    *bytes = plan(nullptr, kv, rows, 0, 0, true).bytes();
+    const Plan p = plan(nullptr, kv, rows, 0, 0, true);
+    RC(check_grids(op, p, kv, rows, true));
+    *bytes = p.bytes();
     return LFM_OK;
 }
 
@@ -471,10 +489,8 @@ extern "C" int lfm_attn_scored(const lfm_kv *kv, const lfm_rows *rows, const flo
         RC(attend(K, p, a, kv, rows, s));
     if (!rows->start)
         return LFM_OK;
-    const uint64_t blocks = (uint64_t)(kv->slots + SUM_KEYS - 1) / SUM_KEYS * kv->kv_heads;
-    if (blocks > 0x7FFFFFFFull)
-        return fail(LFM_EINVAL, "%s: %u slots of %u kv heads", op, kv->slots, kv->kv_heads);
-    RC(launch(K->weights[rows->type][dim_index(kv)], dim3((uint32_t)blocks, kv->n_seq * p.sum_parts), 256, s, a));
+    const uint32_t blocks = (kv->slots + SUM_KEYS - 1) / SUM_KEYS * kv->kv_heads;
+    RC(launch(K->weights[rows->type][dim_index(kv)], dim3(blocks, kv->n_seq * p.sum_parts), 256, s, a));
     if (p.sum_parts == 1)
         return LFM_OK;
     return launch(K->sums, dim3((kv->slots + 255) / 256, kv->kv_heads, kv->n_seq), 256, s, a);
@@ -498,7 +514,9 @@ extern "C" int lfm_attn_prefix_workspace(const lfm_kv *prefix, const lfm_kv *kv,
     RC(check_rows(op, kv, rows));
     if (!bytes)
         return fail(LFM_EINVAL, "%s: bytes is null", op);
-    *bytes = plan(prefix, kv, rows, 0, 0, false).bytes();
+    const Plan p = plan(prefix, kv, rows, 0, 0, false);
+    RC(check_grids(op, p, kv, rows, false));
+    *bytes = p.bytes();
     return LFM_OK;
 }
 
@@ -532,8 +550,8 @@ extern "C" int lfm_kv_evict_workspace(const lfm_kv *kv, uint32_t keep, size_t *b
 {
     const char *op = "lfm_kv_evict_workspace";
     RC(check_kv(op, "kv", kv));
-    if (keep == 0 || keep > 0x7FFFFF00u)
-        return fail(LFM_EINVAL, "%s: keep %u", op, keep);
+    if (keep == 0 || keep > 0x10000000u)
+        return fail(LFM_EINVAL, "%s: keep %u (1..2^28)", op, keep);
     if (!bytes)
         return fail(LFM_EINVAL, "%s: bytes is null", op);
     *bytes = 2 * evict_list_bytes(kv, keep) + (size_t)kv->n_seq * kv->kv_heads * 8;

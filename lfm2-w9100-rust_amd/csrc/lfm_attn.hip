@@ -1334,14 +1334,17 @@ __device__ __forceinline__ uint32_t evict_key(const EvictArgs &a, float acc, int
 }
 
 #define SEL_THREADS 1024
-#define SEL_HELD 32768 // slots whose ranks are held in shared memory; further ones are made again
+#define SEL_HELD 24576 // ranks held in shared memory beside the registers'; further ones are made again
 #define SEL_COPIES 16  // of each histogram, by lane: ranks share their upper bits
-// The `keep` slots of highest rank of one (sequence, kv head), ties to the lowest slot: the
-// rank of the last one by 8-bit histograms from the top (as many as it takes until a bin is
-// taken whole), then each wave counts and places its own run of slots.
+// The `keep` slots of highest rank of one (sequence, kv head), ties to the lowest slot.  Each
+// of 16 waves has a run of slots, 64 at a time, the first eight times with their ranks in
+// registers.  The rank of the last slot that stays is found by 8-bit histograms from the top
+// (as many as it takes until a bin is taken whole); then each wave counts and places its run.
 extern "C" __global__ __launch_bounds__(SEL_THREADS) void k_kv_select(const EvictArgs a)
 {
-    const uint32_t kh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    constexpr uint32_t IN_REGS = 8;
+    const uint32_t kh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63,
+                   wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const size_t bh = (size_t)b * a.c.kv_heads + kh;
     const uint32_t n = (uint32_t)clamp_len(a.c, b), keep = a.keep;
     if (tid == 0) {
@@ -1357,24 +1360,25 @@ extern "C" __global__ __launch_bounds__(SEL_THREADS) void k_kv_select(const Evic
     __shared__ __attribute__((aligned(16))) uint32_t hist[256 * SEL_COPIES], bins[256];
     __shared__ int32_t wmax[16];
     __shared__ uint32_t cnt_eq[16], cnt_hole[16], cnt_move[16];
-    // positions first (their maximum), the first ranks' weights loaded beside them
-    constexpr int EARLY = 8;
-    float early[EARLY];
+    const uint32_t run = ((n + 15) / 16 + 63) / 64 * 64, j0 = min(n, wave * run), j1 = min(n, j0 + run);
+    const uint32_t rounds = (j1 - j0 + 63) / 64; // of this wave
+    const uint32_t hold = wave * (SEL_HELD / 16); // its part of held: rounds from IN_REGS on
+    uint32_t key[IN_REGS];
+    float weight[IN_REGS];
     int32_t newest = INT32_MIN;
 #pragma unroll
-    for (int i = 0; i < EARLY; ++i) {
-        const uint32_t j = min(tid + i * SEL_THREADS, n - 1);
-        early[i] = acc[j];
-        const int32_t p = pos[j];
-        newest = max(newest, p);
-        held[tid + i * SEL_THREADS] = (uint32_t)p;
-    }
-    for (uint32_t j = tid + EARLY * SEL_THREADS; j < n; j += SEL_THREADS) {
-        const int32_t p = pos[j];
-        newest = max(newest, p);
-        if (j < SEL_HELD)
-            held[j] = (uint32_t)p;
-    }
+    for (uint32_t i = 0; i < IN_REGS; ++i)
+        if (i < rounds) { // uniform
+            const uint32_t j = min(j0 + 64 * i + lane, n - 1);
+            weight[i] = acc[j];
+            key[i] = (uint32_t)pos[j];
+        }
+    for (uint32_t i = IN_REGS; i < rounds; ++i)
+        newest = max(newest, pos[min(j0 + 64 * i + lane, n - 1)]);
+#pragma unroll
+    for (uint32_t i = 0; i < IN_REGS; ++i)
+        if (i < rounds)
+            newest = max(newest, (int32_t)key[i]);
     newest = wave_max_i(newest);
     if (lane == 0)
         wmax[wave] = newest;
@@ -1383,29 +1387,42 @@ extern "C" __global__ __launch_bounds__(SEL_THREADS) void k_kv_select(const Evic
     for (int w = 0; w < 16; ++w)
         newest = max(newest, wmax[w]);
 #pragma unroll
-    for (int i = 0; i < EARLY; ++i) // each thread its own slots: no barrier between
-        held[tid + i * SEL_THREADS] = evict_key(a, early[i], (int32_t)held[tid + i * SEL_THREADS], newest);
-    for (uint32_t j = tid + EARLY * SEL_THREADS; j < min(n, (uint32_t)SEL_HELD); j += SEL_THREADS)
-        held[j] = evict_key(a, acc[j], (int32_t)held[j], newest);
-    auto rank = [&](uint32_t j) { return j < SEL_HELD ? held[j] : evict_key(a, acc[j], pos[j], newest); };
+    for (uint32_t i = 0; i < IN_REGS; ++i)
+        if (i < rounds)
+            key[i] = evict_key(a, weight[i], (int32_t)key[i], newest);
+    auto made = [&](uint32_t i) { // the rank of a later round's slot, from memory
+        const uint32_t j = min(j0 + 64 * i + lane, n - 1);
+        return evict_key(a, acc[j], pos[j], newest);
+    };
+    for (uint32_t i = IN_REGS; i < rounds && (i - IN_REGS) * 64 < SEL_HELD / 16; ++i)
+        held[hold + (i - IN_REGS) * 64 + lane] = made(i);
+    // f(round, slot, rank) for every round; lanes past the run have slots from j1 on
+    auto each = [&](auto &&f) {
+#pragma unroll
+        for (uint32_t i = 0; i < IN_REGS; ++i)
+            if (i < rounds)
+                f(j0 + 64 * i + lane, key[i]);
+        for (uint32_t i = IN_REGS; i < rounds; ++i)
+            f(j0 + 64 * i + lane,
+              (i - IN_REGS) * 64 < SEL_HELD / 16 ? held[hold + (i - IN_REGS) * 64 + lane] : made(i));
+    };
     uint32_t last = 0, mask = 0, need = keep; // kept: rank & mask above `last`, and `need` of those at it
     bool exact = false;
     for (int pass = 3; pass >= 0 && !exact; --pass) {
         for (uint32_t i = tid; i < 256 * SEL_COPIES / 4; i += SEL_THREADS)
             ((u32x4 *)hist)[i] = u32x4{0, 0, 0, 0};
         __syncthreads();
-        for (uint32_t j = tid; j < n; j += SEL_THREADS) {
-            const uint32_t k = rank(j);
-            if ((k & mask) == last)
+        each([&](uint32_t j, uint32_t k) {
+            if (j < j1 && (k & mask) == last)
                 atomicAdd(&hist[((k >> (8 * pass)) & 255) * SEL_COPIES + (lane & (SEL_COPIES - 1))], 1u);
-        }
+        });
         __syncthreads();
         if (tid < 256) {
             uint32_t v = 0;
 #pragma unroll
             for (int i = 0; i < SEL_COPIES / 4; ++i) {
                 const u32x4 x = ((const u32x4 *)hist)[tid * (SEL_COPIES / 4) + i];
-                v += x.x + x.y + x.z + x.w;
+                v += x[0] + x[1] + x[2] + x[3];
             }
             bins[tid] = v;
         }
@@ -1413,7 +1430,7 @@ extern "C" __global__ __launch_bounds__(SEL_THREADS) void k_kv_select(const Evic
         // every wave: lane l holds bins 255 - 4 l downwards; the bin where the count from the
         // top reaches `need`
         const u32x4 x = ((const u32x4 *)bins)[63 - lane];
-        const uint32_t four = x.x + x.y + x.z + x.w;
+        const uint32_t four = x[0] + x[1] + x[2] + x[3];
         uint32_t upto = four;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -1422,8 +1439,10 @@ extern "C" __global__ __launch_bounds__(SEL_THREADS) void k_kv_select(const Evic
         }
         const uint32_t at = (uint32_t)__ffsll((unsigned long long)__ballot(upto >= need)) - 1;
         uint32_t left = need - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(four, at));
-        const uint32_t c[4] = {(uint32_t)__builtin_amdgcn_readlane(x.w, at), (uint32_t)__builtin_amdgcn_readlane(x.z, at),
-                               (uint32_t)__builtin_amdgcn_readlane(x.y, at), (uint32_t)__builtin_amdgcn_readlane(x.x, at)};
+        uint32_t c[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            c[i] = __builtin_amdgcn_readlane(x[3 - i], at);
         uint32_t bin = 255 - 4 * at, count = c[0];
 #pragma unroll
         for (int i = 1; i < 4; ++i)
@@ -1437,13 +1456,11 @@ extern "C" __global__ __launch_bounds__(SEL_THREADS) void k_kv_select(const Evic
         need = left;
         exact = left == count;
     }
-    const uint32_t run = ((n + 15) / 16 + 63) / 64 * 64, j0 = wave * run, j1 = min(n, j0 + run);
     const uint64_t below = (1ull << lane) - 1;
     uint32_t eq0 = 0;
     if (!exact) { // uniform: only some of the slots at the last rank stay, the lowest
         uint32_t eq = 0;
-        for (uint32_t j = j0; j < j1; j += 64)
-            eq += __popcll(__ballot(j + lane < j1 && (rank(min(j + lane, n - 1)) & mask) == last));
+        each([&](uint32_t j, uint32_t k) { eq += __popcll(__ballot(j < j1 && (k & mask) == last)); });
         if (lane == 0)
             cnt_eq[wave] = eq;
         __syncthreads();
@@ -1453,23 +1470,22 @@ extern "C" __global__ __launch_bounds__(SEL_THREADS) void k_kv_select(const Evic
     uint32_t holes = 0, moves = 0, hole0 = 0, move0 = 0;
     for (int place = 0; place < 2; ++place) {
         uint32_t e = eq0;
-        for (uint32_t j = j0; j < j1; j += 64) {
-            const uint32_t s = j + lane;
-            const bool in = s < j1;
-            const uint32_t k = in ? rank(s) & mask : 0;
+        each([&](uint32_t j, uint32_t rank) {
+            const bool in = j < j1;
+            const uint32_t k = rank & mask;
             const uint64_t meq = __ballot(in && k == last);
             const bool kept = in && (k > last || (k == last && (exact || e + __popcll(meq & below) < need)));
             e += __popcll(meq);
-            const uint64_t mh = __ballot(in && s < keep && !kept), mm = __ballot(s >= keep && kept);
+            const uint64_t mh = __ballot(in && j < keep && !kept), mm = __ballot(j >= keep && kept);
             if (place) {
-                if (in && s < keep)
-                    map[s] = kept ? (int32_t)s : ~(int32_t)(hole0 + holes + __popcll(mh & below));
+                if (in && j < keep)
+                    map[j] = kept ? (int32_t)j : ~(int32_t)(hole0 + holes + __popcll(mh & below));
                 else if (kept)
-                    movers[move0 + moves + __popcll(mm & below)] = (int32_t)s;
+                    movers[move0 + moves + __popcll(mm & below)] = (int32_t)j;
             }
             holes += __popcll(mh);
             moves += __popcll(mm);
-        }
+        });
         if (place)
             break;
         if (lane == 0)

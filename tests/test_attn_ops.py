@@ -53,7 +53,7 @@ def test_bad_caches(lfm, change):
 
 @pytest.mark.parametrize("change", [
     dict(type=2), dict(type=3), dict(heads=0), dict(heads=33), dict(heads=80000), dict(n_rows=2),
-    dict(n_rows=1 << 31, start=FAKE), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
+    dict(n_rows=1 << 31, start=FAKE), dict(n_rows=1 << 19, start=FAKE), dict(heads=8 * 129), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
     dict(scale=float("inf")), dict(q_row_stride=-64), dict(q_head_stride=4), dict(out_row_stride=63),
     dict(out_row_stride=0), dict(out_head_stride=0)], ids=str)
 def test_bad_rows(lfm, change):
@@ -100,6 +100,15 @@ def test_bad_evictions(lfm, out, keep, sinks, recent):
     assert L.lfm_kv_evict(C.byref(c), f, f, keep, sinks, recent, C.byref(o), 9 * f, 9 * f, f, 1 << 40,
                           None) == lfm.LFM_EINVAL
     assert L.lfm_last_error()
+
+
+def test_grids_that_cannot_be_launched_are_refused(lfm):
+    n = C.c_size_t()
+    k = kv(lfm, slots=0x7FFFFF00, kv_heads=8)
+    r = rows(lfm, start=FAKE)
+    assert lfm.lib().lfm_attn_scored_workspace(C.byref(k), C.byref(r), C.byref(n)) == lfm.LFM_EINVAL
+    assert lfm.lib().lfm_attn_window_workspace(C.byref(k), C.byref(r), 0, 0, C.byref(n)) == 0
+    assert lfm.lib().lfm_kv_evict_workspace(C.byref(k), (1 << 28) + 1, C.byref(n)) == lfm.LFM_EINVAL
 
 
 def test_acc_in_place_needs_equal_slots(lfm):

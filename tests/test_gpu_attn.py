@@ -116,6 +116,38 @@ def test_window_long_prompt(gpu, kind, dim, window, sinks):
     check_window(gpu, r, cache, [0, 700, 830], window, sinks)
 
 
+@pytest.mark.parametrize("heads, kv", [(128, 1), (130, 2), (33, 1)])
+def test_many_heads_a_group(gpu, heads, kv):
+    """More query heads than a row tile holds, in single rows and in chunks."""
+    rng = np.random.default_rng(heads)
+    cache = Cache(rng, [70, 300, 5], kv, 301, 64, "f16")
+    check_window(gpu, Rows(gpu, rng, 3, heads, 64, "f16"), cache, None, 90, 3)
+    check_window(gpu, Rows(gpu, rng, 9, heads, 64, "f32"), cache, [0, 3, 7, 9], 90, 3)
+    check_scored(gpu, Rows(gpu, rng, 3, heads, 64, "f32"), cache, None, None)
+    check_scored(gpu, Rows(gpu, rng, 9, heads, 64, "f16"), cache, [0, 3, 7, 9], None)
+
+
+def test_many_sequences(gpu):
+    """More sequences than a wave has lanes, most of few rows, some of none."""
+    rng = np.random.default_rng(17)
+    counts = rng.choice([0, 1, 1, 2, 5, 40], 150)
+    start = np.concatenate([[0], np.cumsum(counts)])
+    cache = Cache(rng, rng.integers(0, 60, 150), 2, 60, 64, "f16", "slot")
+    check_window(gpu, Rows(gpu, rng, int(start[-1]), 2, 64, "f16"), cache, start, 0, 0)
+    check_window(gpu, Rows(gpu, rng, int(start[-1]), 2, 64, "f16"), cache, start, 11, 2)
+    check_scored(gpu, Rows(gpu, rng, int(start[-1]), 2, 64, "f32"), cache, start, None)
+    prefix = Cache(rng, [77], 2, 80, 64, "f16", "slot")
+    check_prefix(gpu, Rows(gpu, rng, int(start[-1]), 2, 64, "f16"), prefix, cache, start)
+
+
+def test_window_and_sinks_past_every_length(gpu):
+    rng = np.random.default_rng(18)
+    cache = Cache(rng, [70, 130], 2, 150, 64, "f16")
+    for window, sinks in ((0xFFFFFFFF, 0), (0xFFFFFFFF, 0xFFFFFFFF), (0x80000000, 5), (1, 0xFFFFFFFF)):
+        check_window(gpu, Rows(gpu, rng, 2, 4, 64, "f16"), cache, None, window, sinks)
+        check_window(gpu, Rows(gpu, rng, 80, 4, 64, "f16"), cache, [0, 30, 80], window, sinks)
+
+
 def test_window_lengths_out_of_range_count_as_their_ends(gpu):
     rng = np.random.default_rng(5)
     cache = Cache(rng, [-3, 500, 60, 2147483647, -2147483648], 2, 60, 64, "f16")
@@ -332,6 +364,17 @@ def test_prefix_ragged_rows(gpu, layout):
     assert r.untouched([0, -1, -2])
 
 
+@pytest.mark.parametrize("kind, dim", [("f32", 64), ("bf16", 128), ("f16", 64)])
+def test_prefix_of_few_ragged_rows(gpu, kind, dim):
+    rng = np.random.default_rng([dim, 6])
+    cached = kind if kind == "bf16" else "f16"
+    prefix = Cache(rng, [1200], 3, 1201, dim, cached)
+    for counts, heads in (([2, 0, 3], 3), ([1, 1, 1], 6), ([4, 3, 9], 12)):
+        start = np.concatenate([[0], np.cumsum(counts)])
+        cache = Cache(rng, [5, 9, 40], 3, 41, dim, cached)
+        check_prefix(gpu, Rows(gpu, rng, int(start[-1]), heads, dim, kind), prefix, cache, start)
+
+
 @pytest.mark.parametrize("kind, dim, heads, kv, n", [("f32", 64, 8, 2, 70), ("bf16", 128, 3, 1, 41), ("f16", 64, 2, 2, 1)])
 def test_prefix_batches(gpu, kind, dim, heads, kv, n):
     rng = np.random.default_rng([n, 5])
@@ -403,6 +446,26 @@ def test_evict(gpu, slots, keep, sinks, recent, dim, kind, order, pattern, place
     assert np.array_equal(bits(src(oa).reshape(want[2].shape)), bits(want[2]))
     assert np.array_equal(src(op).reshape(want[3].shape), want[3])
     assert np.array_equal(ol.download(), np.minimum(np.clip(length, 0, slots), keep))
+
+
+@pytest.mark.parametrize("pattern", ["plain", "ties"])
+def test_evict_long(gpu, pattern):
+    """Past the slots whose ranks are held in registers and in shared memory."""
+    rng = np.random.default_rng(19)
+    slots, keep = 41003, 20011
+    length = [slots, 33000]
+    acc, pos = evict_inputs(rng, 2, 1, slots, pattern)
+    cache = Cache(rng, length, 1, slots, 64, "f16")
+    ta, tp = f32(acc), i32(pos)
+    ws = workspace(gpu, gpu.kv_evict_workspace(cache.view, keep))
+    gpu.kv_evict(cache.view, ta, tp, keep, cache.view, ta, tp, ws, sinks=4, recent=1000)
+    p = tp.download().reshape(pos.shape)
+    k, _ = read_cache(cache.view, "f16", "head")
+    for b in range(2):
+        s = U.keep_slots(acc[b, 0], pos[b, 0], length[b], keep, 4, 1000)
+        assert np.array_equal(p[b, 0, :keep], pos[b, 0][s])
+        assert np.array_equal(k[b, 0, :keep], cache.k[b, 0][s])
+        assert np.array_equal(k[b, 0, keep:], cache.k[b, 0, keep:])
 
 
 def read_cache(view, kind, order):
