@@ -1025,7 +1025,10 @@ template <typename TQ, int D, int RT, bool PRE> __device__ __forceinline__ void 
                         }
                 }
             }
+            // matrix work of other waves goes before this one's softmax (2 % of a long call)
+            __builtin_amdgcn_s_setprio(0);
             weigh<RT>(S, s, Q, p);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int n = 0; n < D / 16; ++n) {
                 const vec v = v_operand<TQ, D>(vb, at, n);
