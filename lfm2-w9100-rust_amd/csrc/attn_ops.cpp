@@ -59,7 +59,7 @@ static int load_attn(int dev)
                 std::string name;
             } fns[] = {{&k.tile_1[t][d], "k_attn_tile" + tag + "_r1"},
                        {&k.tile_most[t][d], "k_attn_tile" + tag + "_r" + std::to_string(TILE_TILES)},
-                       {&k.tile_prefix[t][d], "k_attn_prefix" + tag + "_r" + std::to_string(TILE_TILES)},
+                       {&k.tile_prefix[t][d], "k_attn_prefix" + tag},
                        {&k.weights[t][d], "k_attn_weights" + tag},
                        {&k.step_1[t][d], "k_attn_step" + tag + "_r1"},
                        {&k.step_most[t][d], "k_attn_step" + tag + "_r" + std::to_string(step_tiles(d ? 128 : 64))},
@@ -398,7 +398,9 @@ static int attend(AttnKernels *K, const Plan &p, AttnOpArgs a, const lfm_kv *kv,
     uint64_t steps = rows->start ? 0 : (uint64_t)rows->n_rows * p.own_groups * p.own_splits;
     a.step_prefix = 0;
     if (p.tile_prefix) {
-        RC(launch_items(K->tile_prefix[t][d], (uint64_t)p.prefix_groups * p.prefix_splits, kv->kv_heads, s, a));
+        const uint64_t with = p.most ? 0 : steps; // in the same launch
+        RC(launch_items(K->tile_prefix[t][d], (uint64_t)p.prefix_groups * p.prefix_splits + with, kv->kv_heads, s, a));
+        steps -= with;
     } else {
         a.step_prefix = p.prefix_groups * p.prefix_splits;
         steps += a.step_prefix;

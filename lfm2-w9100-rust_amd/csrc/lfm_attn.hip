@@ -393,19 +393,24 @@ __device__ __forceinline__ void finish_row(const AttnOpArgs &a, size_t id, bool 
 // blocks of 32 slots in turn, each with a softmax state of its own, joined at the end: a
 // wave streams K straight into A operands and V through a piece of shared memory of its own
 // (the transposed read), the next block's loads in flight, and no wave waits for another.
-template <typename TQ, int D, int RT> __device__ __forceinline__ void attn_step(const AttnOpArgs &a)
+constexpr int STEP_WAVES = 4;
+template <int D, int RT> struct StepShared {
+    static constexpr uint32_t V_BYTES = 32 * D * 2, O_BYTES = 16 * RT * D * 4;
+    __attribute__((aligned(16))) uint8_t bytes[STEP_WAVES * (V_BYTES > O_BYTES ? V_BYTES : O_BYTES)];
+    float2 ml[STEP_WAVES][16 * RT];
+};
+
+template <typename TQ, int D, int RT>
+__device__ __forceinline__ void attn_step(const AttnOpArgs &a, StepShared<D, RT> &shared, uint32_t item)
 {
-    constexpr int NW = 4; // waves
+    constexpr int NW = STEP_WAVES;
     typedef typename TQ::vec vec;
     constexpr int VL = D / 16;                   // 16-byte loads of V a lane and block
-    constexpr uint32_t ROWS = 16 * RT, PIECES = D / 8;
-    constexpr uint32_t V_BYTES = 32 * D * 2, O_BYTES = ROWS * D * 4;
-    constexpr uint32_t SMEM = NW * (V_BYTES > O_BYTES ? V_BYTES : O_BYTES);
-    __shared__ __attribute__((aligned(16))) uint8_t smem[SMEM];
-    __shared__ float2 sml[NW][ROWS];
+    constexpr uint32_t ROWS = 16 * RT, PIECES = D / 8, V_BYTES = StepShared<D, RT>::V_BYTES;
+    uint8_t *const smem = shared.bytes;
+    auto &sml = shared.ml;
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4;
     const uint32_t kh = blockIdx.x % a.own.kv_heads, G = a.group;
-    uint32_t item = blockIdx.x / a.own.kv_heads;
     const bool pre = item < a.step_prefix;
     uint32_t group = 0, part, parts, row0, total;
     const uint16_t *kp, *vp;
@@ -869,16 +874,23 @@ __device__ void attn_row(const AttnOpArgs &a, const B &bl, uint32_t b0, uint32_t
 // A slot that some rows of a wave see and others do not may hold an infinity or NaN in V,
 // which times a weight of 0 would reach all of them: a wave that met such numbers in a
 // masked block computes its rows again, one by one (attn_row).
-template <typename TQ, int D, int RT, bool PRE> __device__ __forceinline__ void attn_tile(const AttnOpArgs &a)
+template <int D> struct TileShared {
+    static constexpr uint32_t BYTES = TILE_KEYS * D * 2;
+    __attribute__((aligned(16))) uint8_t k[2][BYTES], v[2][BYTES];
+    uint64_t odd[4];      // slots of a block whose V is not all finite
+    float weights[4][64]; // attn_row's
+};
+
+template <typename TQ, int D, int RT, bool PRE>
+__device__ __forceinline__ void attn_tile(const AttnOpArgs &a, TileShared<D> &shared, uint32_t flat)
 {
     typedef typename TQ::vec vec;
-    constexpr uint32_t ROWS = 64 * RT, PIECES = D / 8, BYTES = TILE_KEYS * D * 2;
+    constexpr uint32_t ROWS = 64 * RT, PIECES = D / 8, BYTES = TileShared<D>::BYTES;
     constexpr int LD = TILE_KEYS * PIECES / 256; // 16-byte pieces of K, and of V, a thread and block
-    __shared__ __attribute__((aligned(16))) uint8_t ks[2][BYTES], vs[2][BYTES];
-    __shared__ float weights[4][64]; // attn_row's
-    __shared__ uint64_t odd[4];      // slots of a block whose V is not all finite
+    auto &ks = shared.k, &vs = shared.v;
+    auto &odd = shared.odd;
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4;
-    const uint32_t kh = blockIdx.x % a.own.kv_heads, flat = blockIdx.x / a.own.kv_heads, G = a.group;
+    const uint32_t kh = blockIdx.x % a.own.kv_heads, G = a.group;
     const KvView &c = PRE ? a.prefix : a.own;
     const uint32_t splits = PRE ? a.prefix_splits : a.own_splits;
     const uint32_t split = splits == 1 ? 0 : flat % splits;
@@ -1045,7 +1057,7 @@ template <typename TQ, int D, int RT, bool PRE> __device__ __forceinline__ void 
         for (uint32_t x = 0; x < 16 * RT && w0 + x < total; ++x) {
             const uint32_t row = pairs.row_of(x);
             attn_row<TQ, D>(a, bl, b0, b1, kp, vp, row, kh * G + pairs.head_of(x), first + (int32_t)row - lo, split,
-                            weights[wave]);
+                            shared.weights[wave]);
         }
         return;
     }
@@ -1283,7 +1295,8 @@ extern "C" __global__ __launch_bounds__(256) void k_attn_sums(const AttnOpArgs a
     extern "C" __global__ __launch_bounds__(256, RT == 1 ? 1 : 2) void k_attn_step_##tag##_##D##_r##RT(        \
         const AttnOpArgs a)                                                                                    \
     {                                                                                                          \
-        attn_step<TQ, D, RT>(a);                                                                               \
+        __shared__ StepShared<D, RT> shared;                                                                   \
+        attn_step<TQ, D, RT>(a, shared, blockIdx.x / a.own.kv_heads);                                          \
     }
 #define STEPS(TQ, tag, D, MOST)                                                                                \
     STEP(TQ, tag, D, 1)                                                                                        \
@@ -1303,16 +1316,37 @@ STEPS(F16, f16, 128, 2)
 STEPS(BF16, bf16, 64, 4)
 STEPS(BF16, bf16, 128, 2)
 
-#define TILE(TQ, tag, D, RT, PRE, name)                                                                        \
-    extern "C" __global__ __launch_bounds__(256, D == 128 ? 2 : TQ::parts == 2 ? 3 : 4) void                   \
-    k_attn_##name##_##tag##_##D##_r##RT(const AttnOpArgs a)                                                    \
+// The prefix of many rows, and single rows' own slots (where the call has such) in the same
+// launch: a piece of the one and a piece of the other in turn, so that a CU has matrix work
+// and loads from memory at once.
+template <typename TQ, int D> __device__ __forceinline__ void attn_prefix(const AttnOpArgs &a)
+{
+    union Shared {
+        TileShared<D> tile;
+        StepShared<D, 1> step;
+    };
+    __shared__ Shared shared;
+    const uint32_t item = blockIdx.x / a.own.kv_heads, tiles = a.prefix_groups * a.prefix_splits;
+    if (item < tiles)
+        attn_tile<TQ, D, TILE_TILES, true>(a, shared.tile, item);
+    else
+        attn_step<TQ, D, 1>(a, shared.step, item - tiles);
+}
+
+#define TILE_BOUNDS(TQ, D) __launch_bounds__(256, D == 128 ? 2 : TQ::parts == 2 ? 3 : 4)
+#define TILE(TQ, tag, D, RT)                                                                                   \
+    extern "C" __global__ TILE_BOUNDS(TQ, D) void k_attn_tile_##tag##_##D##_r##RT(const AttnOpArgs a)          \
     {                                                                                                          \
-        attn_tile<TQ, D, RT, PRE>(a);                                                                          \
+        __shared__ TileShared<D> shared;                                                                       \
+        attn_tile<TQ, D, RT, false>(a, shared, blockIdx.x / a.own.kv_heads);                                   \
     }
 #define TILES(TQ, tag, D)                                                                                      \
-    TILE(TQ, tag, D, 1, false, tile)                                                                           \
-    TILE(TQ, tag, D, 2, false, tile)                                                                           \
-    TILE(TQ, tag, D, 2, true, prefix)                                                                          \
+    TILE(TQ, tag, D, 1)                                                                                        \
+    TILE(TQ, tag, D, 2)                                                                                        \
+    extern "C" __global__ TILE_BOUNDS(TQ, D) void k_attn_prefix_##tag##_##D(const AttnOpArgs a)                \
+    {                                                                                                          \
+        attn_prefix<TQ, D>(a);                                                                                 \
+    }                                                                                                          \
     extern "C" __global__ __launch_bounds__(256) void k_attn_weights_##tag##_##D(const AttnOpArgs a)           \
     {                                                                                                          \
         attn_weights<TQ, D>(a);                                                                                \
