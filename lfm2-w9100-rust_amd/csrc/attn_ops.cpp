@@ -317,9 +317,19 @@ static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint
         p.prefix_groups = (uint32_t)(((uint64_t)r->n_rows * G + rows - 1) / rows);
         const uint64_t pitems = (uint64_t)std::max(1u, p.prefix_groups) * kv->kv_heads;
         const uint64_t blocks = (prefix->slots + 31) / 32;
-        // (a tile's range of 16 blocks: 64 sequences over 8192 slots take 31 us in ranges of
-        // 16, 35 in ranges of 8, whose joining costs more)
-        p.prefix_splits = ranges(TARGET_GROUPS / pitems, blocks / (blocks > 64 ? (p.tile_prefix ? 16 : 8) : 4));
+        uint64_t target = TARGET_GROUPS, least = blocks > 64 ? 8 : 4;
+        if (p.tile_prefix) {
+            // At 64 dims a CU holds four tiles: 600 rows over 32000 slots take 74 us as 480
+            // tiles, 70 as 760, 73 as 1000.  A range of 16 blocks and more (8192 slots for 64
+            // sequences: 60 us with 16, 70 with 8, which have to be joined); of 32 where the
+            // sequences' own slots are read meanwhile for longer than the prefix takes (the
+            // same: 53; where own and prefix are alike, 24 sequences of 2000 after 30000, 39 and 42).
+            if (kv->head_dim == 64)
+                target = TARGET_GROUPS * 3 / 2;
+            if (blocks > 64)
+                least = (uint64_t)r->n_rows * kv->slots >= 3 * (uint64_t)prefix->slots * p.prefix_groups ? 32 : 16;
+        }
+        p.prefix_splits = ranges(target / pitems, blocks / least);
     }
     const uint32_t splits = p.own_splits + p.prefix_splits;
     const bool steps = scored && !r->start; // scores are kept from the step to the join
