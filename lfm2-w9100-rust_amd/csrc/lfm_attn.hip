@@ -1289,11 +1289,11 @@ extern "C" __global__ __launch_bounds__(256) void k_attn_sums(const AttnOpArgs a
     a.acc_out[at] = (a.acc ? a.acc[at] : 0.f) + sum;
 }
 
-// RT: row tiles of a workgroup of rows that see the same slots, as many as the registers
-// hold beside the next block's K and V.
+// RT: row tiles of a workgroup of rows that see the same slots, as many as the registers hold
+// beside the next block's K and V at one wave a SIMD (64 sequences over 8192 slots, 32 heads
+// over 1 of 128 dims, F32 rows: 58 us; held to two waves, with what spills in memory, 85).
 #define STEP(TQ, tag, D, RT)                                                                                   \
-    extern "C" __global__ __launch_bounds__(256, RT == 1 ? 1 : 2) void k_attn_step_##tag##_##D##_r##RT(        \
-        const AttnOpArgs a)                                                                                    \
+    extern "C" __global__ __launch_bounds__(256) void k_attn_step_##tag##_##D##_r##RT(const AttnOpArgs a)      \
     {                                                                                                          \
         __shared__ StepShared<D, RT> shared;                                                                   \
         attn_step<TQ, D, RT>(a, shared, blockIdx.x / a.own.kv_heads);                                          \
