@@ -292,20 +292,22 @@ static Plan plan(const lfm_kv *prefix, const lfm_kv *kv, const lfm_rows *r, uint
         p.own_groups = (G + per - 1) / per;
         const uint64_t items = (uint64_t)std::max(1u, r->n_rows) * p.own_groups * kv->kv_heads;
         // A second launch that joins ranges takes 2-3 us: up to 512 slots one range is faster
-        // (512 slots of one sequence, 64 dims: 5.9 us against 6.8 in four ranges; 1024: 8.5
-        // against 6.8 in eight), where no join follows anyway.  A workgroup's four waves take
-        // a block of 32 each at least, two of a longer cache (4096 slots: 8.3 us in 32 ranges,
-        // 7.8 in 16).
+        // (512 slots of one sequence, 64 dims, F16: 4.9 us against 6.0 in four ranges; 1024: 7.1
+        // against 5.9 in eight; 128 dims: 7.6 and 7.1, 11.9 and 7.0), where no join follows
+        // anyway.  A workgroup's four waves take a block of 32 each at least, two of a longer
+        // cache (4096 slots: 7.5 us in 32 ranges, 7.0 in 16).
         if (scored || blocks > 16)
             p.own_splits = ranges(TARGET_GROUPS / items, blocks / (blocks > 64 ? 8 : 4));
     } else {
         // sequences end inside tiles: at most one more tile each
         const uint64_t cut = (uint64_t)r->n_rows * G;
-        // the larger tile reads K and V half as often; it is taken where it fills the CUs as
-        // often as they hold it (four at 64 dims, two at 128): a 2048-token prompt of 32
-        // heads over 8 of 64 dims, half of that, takes 51 us in the small one and 60 in it
+        // The larger tile reads K and V half as often; it is taken where there are enough of
+        // them to fill the CUs (a CU holds four at 64 dims, two at 128).  One prompt, 32 heads
+        // over 8, small and large tile: 64 dims, 2048 tokens (512 large tiles) 38 and 43 us,
+        // 2700 (675) 54 and 57, 3200 (800) 74 and 70, 8192 411 and 325; 128 dims, 1024 (256)
+        // 27 and 32, 2048 65 and 60, 8192 789 and 584.
         const uint32_t most = 64 * TILE_TILES;
-        p.tile_most = cut / most * kv->kv_heads >= (kv->head_dim == 64 ? 1024 : 512);
+        p.tile_most = cut / most * kv->kv_heads >= (kv->head_dim == 64 ? 720 : 512);
         const uint64_t rows = p.tile_most ? most : 64;
         p.tile_items = cut / rows + std::min<uint64_t>(kv->n_seq, r->n_rows);
         const uint64_t span = window ? std::min<uint64_t>(kv->slots, (uint64_t)window + sinks + rows / G + 128)
