@@ -393,6 +393,12 @@ __device__ __forceinline__ void finish_row(const AttnOpArgs &a, size_t id, bool 
 // blocks of 32 slots in turn, each with a softmax state of its own, joined at the end: a
 // wave streams K straight into A operands and V through a piece of shared memory of its own
 // (the transposed read), the next block's loads in flight, and no wave waits for another.
+//
+// Many sequences are bound by memory: 64 of up to 4112 visible slots, 32 heads over 8 of 128
+// dims, take 177 us, 5.55 TB/s (a copy reaches 5.2).  One is bound by latency: 1028 slots, 32
+// heads over 8 of 64 dims, 5.8 us, of which a launch is 2 and a half.  (Sixteen waves, or
+// eight, with no join after them are slower: 1024 slots take 9.4 and 8.0 us against 6.7
+// with a join, 256 slots 6.3 and 5.3 against 4.5.)
 constexpr int STEP_WAVES = 4;
 template <int D, int RT> struct StepShared {
     static constexpr uint32_t V_BYTES = 32 * D * 2, O_BYTES = 16 * RT * D * 4;
@@ -660,7 +666,8 @@ __device__ __forceinline__ void store_row(const AttnOpArgs &a, uint32_t row, uin
         finish_row(a, (size_t)row * a.r.heads + h, empty, top, sum);
 }
 
-// Joins the key ranges of a row and head: a wave each.
+// Joins the key ranges of a row and head: a wave each, so that one row of 32 heads takes 8
+// CUs.  Bound by latency: 3.1 us there, 5.1 for 64 rows of 32 heads, 128 dims and 9 ranges.
 template <typename TQ, int D> __device__ __forceinline__ void attn_merge(const AttnOpArgs &a)
 {
     const uint32_t id = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
@@ -680,7 +687,8 @@ template <typename TQ, int D> __device__ __forceinline__ void attn_merge(const A
 // slot's weights, SCORED_SLOTS slots a workgroup, four a thread.  Scores were kept as they
 // left the matrix cores, so a weight is one exponential here: 16 bytes a slot and kv head at
 // four query heads, where reading K again would be 128 or 256.  The first four heads' scores
-// are loaded before the ranges are joined.
+// are loaded before the ranges are joined.  Six sequences of up to 32768 slots, 32 heads over
+// 8: 10 us after the step's 139; eight of up to 4096: 4.9 after 12.1, mostly latency.
 template <typename TQ, int D> __device__ __forceinline__ void scored_join(const AttnOpArgs &a)
 {
     const uint32_t chunk = blockIdx.x, kh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x,
@@ -865,11 +873,20 @@ __device__ void attn_row(const AttnOpArgs &a, const B &bl, uint32_t b0, uint32_t
 
 #define TILE_KEYS 64
 // One workgroup: 64 RT (token, head) pairs of one sequence and kv head, 16 RT a wave, over
-// one key range; PRE: of the whole batch over the prefix.  Blocks of 64 slots pass through two buffers of shared memory, K and V as
-// they lie in the cache with their 16-byte pieces exchanged (v_piece); every wave reads K as
-// A operands and V through the transposed read.  The next block's loads are in flight while
-// a block is used.  Blocks that no row of a wave sees are passed over by it, those that all
-// its rows see whole are used without masks.
+// one key range; PRE: of the whole batch over the prefix.  Blocks of 64 slots pass through two
+// buffers of shared memory, K and V as they lie in the cache with their 16-byte pieces
+// exchanged (v_piece); every wave reads K as A operands and V through the transposed read.
+// The next block's loads are in flight while a block is used.  Blocks that no row of a wave
+// sees are passed over by it, those that all its rows see whole are used without masks.
+//
+// Bound by a SIMD's issue, which softmax and matrix work share: for 32 rows and 32 slots of 64
+// dims a wave has 16 products of 16 cycles, 16 exponentials of 10 and some 70 other
+// instructions, and products and other work hardly overlap (8 products and 32 multiply-adds
+// of four waves take 194 cycles together, 132 and 82 alone).  4096 tokens, window 1024, 32
+// heads over 8 of 64 dims: 50 us, 600 TFLOP/s; 8192 causal: 324 us, 850; of 128 dims, with
+// half as much softmax a product, 583 us, 940.  Two groups of 32 slots in one softmax take more
+// registers than four waves a SIMD have (72 us for 60), four row tiles a wave leave two waves
+// (55 for 53), and V's operands before the softmax cost 71 for 59.
 //
 // A slot that some rows of a wave see and others do not may hold an infinity or NaN in V,
 // which times a weight of 0 would reach all of them: a wave that met such numbers in a
@@ -1095,7 +1112,9 @@ __device__ __forceinline__ void attn_tile(const AttnOpArgs &a, TileShared<D> &sh
 // weights 2^(s c - offset) / sum over its rows, and the 16 lanes of a slot are added at the
 // end, all in a fixed order.  (Rows read as operands by every wave for itself, 16 rows a load,
 // kept the first-level cache busy with 64-byte pieces: a prompt of 2048 tokens, 32 heads over
-// 8 of 64 dims, took 42 us so, 29 this way and 5 for the adding of the parts.)
+// 8 of 64 dims, took 42 us so, 28 this way and 5 for the adding of the parts.)  Bound by vector
+// instructions, three a score and one of them an exponential: they fill 31 of 50 thousand cycles
+// of a SIMD, the products 8.
 template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const AttnOpArgs &a)
 {
     typedef typename TQ::vec vec;
@@ -1270,7 +1289,9 @@ template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const
         }
 }
 
-// acc_out = acc + the parts of attn_weights, in order.
+// acc_out = acc + the parts of attn_weights, in their order: equal calls give equal bits, which
+// atomic additions would not.  A launch and little more, 4.6 us for 16 parts of 2048 slots and
+// 8 kv heads.
 extern "C" __global__ __launch_bounds__(256) void k_attn_sums(const AttnOpArgs a)
 {
     const uint32_t j = blockIdx.x * 256 + threadIdx.x, kh = blockIdx.y, b = blockIdx.z;
@@ -1317,8 +1338,11 @@ STEPS(BF16, bf16, 64, 4)
 STEPS(BF16, bf16, 128, 2)
 
 // The prefix of many rows, and single rows' own slots (where the call has such) in the same
-// launch: a piece of the one and a piece of the other in turn, so that a CU has matrix work
-// and loads from memory at once.
+// launch, the prefix first: one or two of its workgroups come to a CU, which then has matrix
+// work and loads from memory at once.  64 sequences of 8192 + up to 1024 slots, 32 heads over 8
+// of 128 dims: 53 us (66 in two launches); 150 of 32000 + up to 257, 64 dims: 69 (77).  In turn,
+// a workgroup of the prefix and one of the own slots, the second takes 103: the prefix's come to
+// the same CUs.
 template <typename TQ, int D> __device__ __forceinline__ void attn_prefix(const AttnOpArgs &a)
 {
     union Shared {
@@ -1377,6 +1401,8 @@ __device__ __forceinline__ uint32_t evict_key(const EvictArgs &a, float acc, int
 // of 16 waves has a run of slots, 64 at a time, the first eight times with their ranks in
 // registers.  The rank of the last slot that stays is found by 8-bit histograms from the top
 // (as many as it takes until a bin is taken whole); then each wave counts and places its run.
+// Bound by the chain of its steps, some ten barriers: 8 us for 1034 slots, 14 for 16 times 8
+// of up to 8192.
 extern "C" __global__ __launch_bounds__(SEL_THREADS) void k_kv_select(const EvictArgs a)
 {
     constexpr uint32_t IN_REGS = 8;
@@ -1537,7 +1563,8 @@ extern "C" __global__ __launch_bounds__(SEL_THREADS) void k_kv_select(const Evic
 #define MOVE_ROWS 32
 // Copies `keep` slots (in place: only the moved ones) of one (sequence, kv head), 32 per
 // workgroup, 16 bytes a lane.  A moved slot's source is at or past `keep` and its target
-// below: in place, nothing is read that another thread writes.
+// below: in place, nothing is read that another thread writes.  Bound by memory: 16 sequences of
+// 8 kv heads cut to 2048 slots of 128 dims take 47 us, 5.7 TB/s.
 extern "C" __global__ __launch_bounds__(256) void k_kv_move(const EvictArgs a)
 {
     const uint32_t kh = blockIdx.y, b = blockIdx.z, n0 = blockIdx.x * MOVE_ROWS;
