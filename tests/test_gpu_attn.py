@@ -1,6 +1,7 @@
 """Cache-attention operators on the GPU against their formulas in 64 bits.  Tolerances are
 derived per element in attn_util."""
 import ctypes as C
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
@@ -125,6 +126,57 @@ def test_many_heads_a_group(gpu, heads, kv):
     check_window(gpu, Rows(gpu, rng, 9, heads, 64, "f32"), cache, [0, 3, 7, 9], 90, 3)
     check_scored(gpu, Rows(gpu, rng, 3, heads, 64, "f32"), cache, None, None)
     check_scored(gpu, Rows(gpu, rng, 9, heads, 64, "f16"), cache, [0, 3, 7, 9], None)
+
+
+@pytest.mark.parametrize("kind, dim", [("f32", 64), ("f16", 64), ("bf16", 64), ("f32", 128), ("bf16", 128)])
+def test_window_large_prompts(gpu, kind, dim):
+    """Enough rows for the larger tiles: some rows of them, against single rows in 64 bits.
+    Slot 3000 of the first prompt holds NaN in V: rows before it and those whose window has
+    passed it do not see it."""
+    rng = np.random.default_rng([dim, 19])
+    length, counts, heads, kv = [3907, 333], [3850, 130], 24, 8
+
+    def edit(k, v):
+        v[0, :, 3000] = np.nan
+
+    cache = Cache(rng, length, kv, 3911, dim, "bf16" if kind == "bf16" else "f16", "slot", edit)
+    start = np.concatenate([[0], np.cumsum(counts)])
+    r = Rows(gpu, rng, int(start[-1]), heads, dim, kind)
+    for window, sinks in ((0, 0), (700, 5)):
+        run_window(gpu, r, cache, window=window, sinks=sinks, start=i32(start))
+        got, lse = r.result(), r.lse.download().reshape(r.shape[:2])
+        rows = np.concatenate([rng.choice(r.shape[0], 25, replace=False), [0, 1, 2942, 2943, 3642, 3643, 3849, 3850, 3979]])
+        for row in rows:
+            b = int(row >= start[1])
+            pos = length[b] - start[b + 1] + row
+            one = SimpleNamespace(k=cache.k[b:b + 1], v=cache.v[b:b + 1], length=[pos + 1])
+            out, want, _, extra = U.reference(r.values[row:row + 1], one, None, window, sinks)
+            if b == 0 and pos >= 3000 and (window == 0 or pos < 3700):
+                assert np.isnan(got[row]).all()
+            else:
+                check_out(got[row:row + 1], out, extra, kind, dim)
+            assert (np.abs(lse[row] - want[0]) <= U.lse_tolerance(want, extra, dim)[0]).all()
+
+
+@pytest.mark.parametrize("kind, dim", [("f16", 64), ("bf16", 128)])
+def test_many_prompts(gpu, kind, dim):
+    """The larger tiles over many short sequences, each ending inside one."""
+    rng = np.random.default_rng([dim, 20])
+    counts = rng.integers(40, 80, 68 if dim == 64 else 50)
+    start = np.concatenate([[0], np.cumsum(counts)])
+    cache = Cache(rng, counts + rng.integers(-20, 40, len(counts)), 8, 120, dim, kind)
+    r = Rows(gpu, rng, int(start[-1]), 24, dim, kind)
+    check_scored(gpu, r, cache, start, None)
+
+
+@pytest.mark.parametrize("heads, kv", [(128, 1), (33, 1), (34, 2)])
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_many_heads_a_group_of_128_dims(gpu, heads, kv, kind):
+    rng = np.random.default_rng([heads, 21])
+    cache = Cache(rng, [70, 700, 5], kv, 701, 128, "bf16" if kind == "bf16" else "f16")
+    check_window(gpu, Rows(gpu, rng, 3, heads, 128, kind), cache, None, 0, 0)
+    check_window(gpu, Rows(gpu, rng, 3, heads, 128, kind), cache, None, 90, 3)
+    check_scored(gpu, Rows(gpu, rng, 3, heads, 128, kind), cache, None, None)
 
 
 def test_many_sequences(gpu):
@@ -382,6 +434,22 @@ def test_prefix_batches(gpu, kind, dim, heads, kv, n):
     prefix = Cache(rng, [2049], kv, 2100, dim, cached)
     cache = Cache(rng, rng.integers(0, 30, n), kv, 30, dim, cached)
     check_prefix(gpu, Rows(gpu, rng, n, heads, dim, kind), prefix, cache)
+
+
+@pytest.mark.parametrize("kind, dim", [("f32", 64), ("f16", 64), ("f32", 128), ("bf16", 128)])
+@pytest.mark.parametrize("heads, kv, n, n_prefix, slots", [
+    (3, 1, 40, 2203, 1000),  # own slots in several ranges, longer than the prefix
+    (4, 2, 45, 9001, 70),    # the prefix in many ranges
+    (34, 2, 9, 700, 150),    # more query heads than a row tile, in a launch of their own
+    (10, 2, 13, 2500, 700)])
+def test_prefix_and_own_slots_together(gpu, kind, dim, heads, kv, n, n_prefix, slots):
+    """Prefix of many rows and their own slots in one launch, each in key ranges."""
+    rng = np.random.default_rng([heads, dim, 22])
+    cached = kind if kind == "bf16" else "f16"
+    prefix = Cache(rng, [n_prefix], kv, n_prefix + 5, dim, cached)
+    length = rng.integers(0, slots + 1, n)
+    length[[0, 1, -1]] = 0, slots, 1
+    check_prefix(gpu, Rows(gpu, rng, n, heads, dim, kind), prefix, Cache(rng, length, kv, slots, dim, cached, "slot"))
 
 
 # ------------------------------------------------------------------ eviction
