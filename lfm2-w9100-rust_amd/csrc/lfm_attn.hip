@@ -219,10 +219,11 @@ __device__ __forceinline__ void load_row(Queries<TQ, D, RT> &Q, int t, const Row
 // ------------------------------------------------------------------ softmax state
 // Of RT tiles of 16 rows: o[t][n] are dims 16 n + 4 (lane / 16) + e of row lane % 16, l the
 // lane's own part of the sum of the weights 2^(s c - mc), whose four parts are added at the
-// end.  lim is what s c - mc may reach before mc follows; -inf while no number was seen.
+// end.  mc is UNSEEN while no number was seen: then the weight of any number is infinite.
+#define UNSEEN (-3.4028235e38f)
 template <typename TQ, int D, int RT> struct State {
     floatx4 o[RT][D / 16];
-    float mc[RT], lim[RT], l[RT];
+    float mc[RT], l[RT];
     __device__ __forceinline__ void clear()
     {
 #pragma unroll
@@ -230,73 +231,75 @@ template <typename TQ, int D, int RT> struct State {
 #pragma unroll
             for (int n = 0; n < D / 16; ++n)
                 o[t][n] = floatx4{0.f, 0.f, 0.f, 0.f};
-            mc[t] = 0.f, lim[t] = -INFINITY, l[t] = 0.f;
+            mc[t] = UNSEEN, l[t] = 0.f;
         }
     }
+    __device__ __forceinline__ bool seen(int t) const { return mc[t] > UNSEEN; }
     // for joining: -inf where there is nothing to join
-    __device__ __forceinline__ float offset(int t) const { return lim[t] > -INFINITY ? mc[t] : -INFINITY; }
+    __device__ __forceinline__ float offset(int t) const { return seen(t) ? mc[t] : -INFINITY; }
 };
 
 // Scores of 32 slots and NT row tiles (s[t][0]: slots 4 (lane / 16) + e, s[t][1]: the same +
 // 16) -> weights as B operands: inner place 8 (lane / 16) + i is slot 16 (i / 4) + 4 (lane /
 // 16) + i % 4.  The largest weight is 2^offset when mc is set, and mc follows the scores only
-// when one passes it by RISE binary orders, for all the tiles at once: after the first block
-// hardly ever, and a weight stays at or below 2^15.  (The maximum is taken of the scaled
-// scores: of the matrix cores' own results the compiler first makes canonical copies, one
-// more instruction a score.)
+// when the weights of a lane's eight slots pass that by RISE binary orders together: after
+// the first block hardly ever, and a weight stays at or below 2^15.  So their sum, which is
+// needed anyway, stands for the maximum (2700 tokens of 64 dims 54.8 us with it, 53.1 without).
+// Two tiles share a check, where four would keep more in registers than there are.
 #define RISE 8.f
 template <int NT, typename TQ, int D, int RT>
 __device__ __forceinline__ void weigh(State<TQ, D, RT> &S, const floatx4 (&s)[RT][2], const Queries<TQ, D, RT> &Q,
                                       typename TQ::vec (&p)[RT][TQ::parts])
 {
-    float x[NT][8];
-    bool rises = false;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            x[t][i] = fmaf(s[t][i / 4][i % 4], Q.c_of(t), -S.mc[t]);
-        const float top = fmaxf(fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])),
-                                fmaxf(fmaxf(x[t][4], x[t][5]), fmaxf(x[t][6], x[t][7])));
-        rises |= top > S.lim[t];
-    }
-    if (__ballot(rises)) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float top = x[t][0];
-#pragma unroll
-            for (int i = 1; i < 8; ++i)
-                top = fmaxf(top, x[t][i]);
-            top = row_max(top);
-            const bool seen = S.lim[t] > -INFINITY, number = top > -INFINITY;
-            float d = top - TQ::offset;
-            d = seen ? fmaxf(d, 0.f) : number ? d : 0.f; // a row of -inf alone: weights 2^-inf = 0
-            const float r = seen ? exp2_hw(-d) : 1.f;
-            S.mc[t] += d, S.l[t] *= r, S.lim[t] = seen || number ? TQ::offset + RISE : -INFINITY;
-#pragma unroll
-            for (int n = 0; n < D / 16; ++n)
-                S.o[t][n] *= r;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                x[t][i] -= d;
-        }
-    }
+    constexpr float MOST = 1 << (int)(TQ::offset + RISE);
+    constexpr int AT_ONCE = NT < 2 ? NT : 2;
     typedef typename TQ::kv kv2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        float w[8];
+    for (int t0 = 0; t0 < NT; t0 += AT_ONCE) {
+        float w[AT_ONCE][8], sum[AT_ONCE];
+        bool passes = false;
+        auto weights = [&](int u) {
+            const int t = t0 + u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            w[i] = exp2_hw(x[t][i]);
-        S.l[t] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+            for (int i = 0; i < 8; ++i)
+                w[u][i] = exp2_hw(fmaf(s[t][i / 4][i % 4], Q.c_of(t), -S.mc[t]));
+            sum[u] = ((w[u][0] + w[u][1]) + (w[u][2] + w[u][3])) + ((w[u][4] + w[u][5]) + (w[u][6] + w[u][7]));
+        };
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            const kv2 hi = __builtin_convertvector((float2v){w[i], w[i + 1]}, kv2);
-            p[t][0][i] = hi[0], p[t][0][i + 1] = hi[1];
-            if constexpr (TQ::parts == 2) {
-                const float2v back = __builtin_convertvector(hi, float2v);
-                const kv2 lo = __builtin_convertvector((float2v){w[i] - back[0], w[i + 1] - back[1]}, kv2);
-                p[t][1][i] = lo[0], p[t][1][i + 1] = lo[1];
+        for (int u = 0; u < AT_ONCE; ++u) {
+            weights(u);
+            passes |= !(sum[u] <= MOST);
+        }
+        if (__ballot(passes)) {
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const int t = t0 + u;
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    top = fmaxf(top, s[t][i / 4][i % 4] * Q.c_of(t));
+                const float mc = fmaxf(S.mc[t], row_max(top) - TQ::offset),
+                            r = S.seen(t) ? exp2_hw(S.mc[t] - mc) : 1.f;
+                S.mc[t] = mc, S.l[t] *= r;
+#pragma unroll
+                for (int n = 0; n < D / 16; ++n)
+                    S.o[t][n] *= r;
+                weights(u);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int t = t0 + u;
+            S.l[t] += sum[u];
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const kv2 hi = __builtin_convertvector((float2v){w[u][i], w[u][i + 1]}, kv2);
+                p[t][0][i] = hi[0], p[t][0][i + 1] = hi[1];
+                if constexpr (TQ::parts == 2) {
+                    const float2v back = __builtin_convertvector(hi, float2v);
+                    const kv2 lo = __builtin_convertvector((float2v){w[u][i] - back[0], w[u][i + 1] - back[1]}, kv2);
+                    p[t][1][i] = lo[0], p[t][1][i + 1] = lo[1];
+                }
             }
         }
     }
@@ -572,7 +575,7 @@ __device__ __forceinline__ void attn_step(const AttnOpArgs &a, StepShared<D, RT>
 #pragma unroll
         for (int w = 0; w < NW; ++w)
             top = fmaxf(top, sml[w][16 * t + (lane & 15)].x);
-        const float f = S.lim[t] > -INFINITY ? exp2_hw(S.mc[t] - top) : 0.f;
+        const float f = S.seen(t) ? exp2_hw(S.mc[t] - top) : 0.f;
         float *to = so + ((size_t)wave * ROWS + 16 * t + (lane & 15)) * D + 4 * g;
         if (16 * t + (lane & 15) < rows)
 #pragma unroll
@@ -1312,9 +1315,11 @@ extern "C" __global__ __launch_bounds__(256) void k_attn_sums(const AttnOpArgs a
 
 // RT: row tiles of a workgroup of rows that see the same slots, as many as the registers hold
 // beside the next block's K and V at one wave a SIMD (64 sequences over 8192 slots, 32 heads
-// over 1 of 128 dims, F32 rows: 58 us; held to two waves, with what spills in memory, 85).
+// over 1 of 128 dims, F32 rows: 58 us; held to two waves, with what spills in memory, 85).  At
+// 64 dims and 16-bit rows two waves find room (28 us; 32 with one).
 #define STEP(TQ, tag, D, RT)                                                                                   \
-    extern "C" __global__ __launch_bounds__(256) void k_attn_step_##tag##_##D##_r##RT(const AttnOpArgs a)      \
+    extern "C" __global__ __launch_bounds__(256, RT == 4 && TQ::parts == 1 ? 2 : 1) void                          \
+    k_attn_step_##tag##_##D##_r##RT(const AttnOpArgs a)                                                        \
     {                                                                                                          \
         __shared__ StepShared<D, RT> shared;                                                                   \
         attn_step<TQ, D, RT>(a, shared, blockIdx.x / a.own.kv_heads);                                          \

@@ -234,6 +234,27 @@ def test_window_large_scores(gpu):
     check_window(gpu, r, cache, None, 0, 0, scale=1e9)
 
 
+@pytest.mark.parametrize("kind, dim, first", [("f32", 64, 0), ("f16", 64, 300), ("bf16", 64, 0), ("f32", 128, 300),
+                                              ("bf16", 128, -300)])
+def test_scores_that_rise_and_fall(gpu, kind, dim, first):
+    """K of slot j is (first + j / 2) times one vector: for some rows every block's scores pass
+    all before them, for others the first slots' are the largest, far below zero or above."""
+    rng = np.random.default_rng([dim, abs(first), 23])
+    length = [500, 130, 33]
+
+    def edit(k, v):
+        k[:] = (first + 0.5 * np.arange(k.shape[2]))[:, None] * k[:, :, :1]
+
+    cache = Cache(rng, length, 2, 501, dim, "bf16" if kind == "bf16" else "f16", edit=edit)
+    check_window(gpu, Rows(gpu, rng, 3, 8, dim, kind), cache, None, 0, 0)
+    check_scored(gpu, Rows(gpu, rng, 3, 40, dim, kind), cache, None, None)
+    check_window(gpu, Rows(gpu, rng, 99, 6, dim, kind), cache, [0, 60, 66, 99], 70, 3)
+    check_scored(gpu, Rows(gpu, rng, 99, 6, dim, kind), cache, [0, 60, 66, 99], None)
+    prefix = Cache(rng, [700], 2, 700, dim, "bf16" if kind == "bf16" else "f16", edit=edit)
+    check_prefix(gpu, Rows(gpu, rng, 3, 40, dim, kind), prefix, cache)
+    check_prefix(gpu, Rows(gpu, rng, 3, 10, dim, kind), prefix, cache)
+
+
 @pytest.mark.parametrize("kind, dim", [("f32", 64), ("f16", 128), ("bf16", 64)], ids=ids)
 def test_window_unseen_slots_hold_anything(gpu, kind, dim):
     """NaN and infinities in slots that a row does not see: past the length, before the
