@@ -883,11 +883,11 @@ __device__ void attn_row(const AttnOpArgs &a, const B &bl, uint32_t b0, uint32_t
 // sees are passed over by it, those that all its rows see whole are used without masks.
 //
 // Bound by a SIMD's issue, which softmax and matrix work share: for 32 rows and 32 slots of 64
-// dims a wave has 16 products of 16 cycles, 16 exponentials of 10 and some 70 other
+// dims a wave has 16 products of 16 cycles, 16 exponentials of 10 and some 55 other
 // instructions, and products and other work hardly overlap (8 products and 32 multiply-adds
 // of four waves take 194 cycles together, 132 and 82 alone).  4096 tokens, window 1024, 32
-// heads over 8 of 64 dims: 50 us, 600 TFLOP/s; 8192 causal: 324 us, 850; of 128 dims, with
-// half as much softmax a product, 583 us, 940.  Two groups of 32 slots in one softmax take more
+// heads over 8 of 64 dims: 50 us, 600 TFLOP/s; 8192 causal: 323 us, 850; of 128 dims, with
+// half as much softmax a product, 589 us, 930.  Two groups of 32 slots in one softmax take more
 // registers than four waves a SIMD have (72 us for 60), four row tiles a wave leave two waves
 // (55 for 53), and V's operands before the softmax cost 71 for 59.
 //
