@@ -203,17 +203,18 @@ static const char *const KV_NAMES[3] = {"kv->k", "kv->v", "kv->len"};
 static const char *const PREFIX_NAMES[3] = {"prefix->k", "prefix->v", "prefix->len"};
 static const char *const OUT_NAMES[3] = {"out->k", "out->v", "out->len"};
 
+// start is read without rows too: a scored call then still copies acc.
 static int check_rows_ptrs(const char *op, const lfm_rows *r, int dev)
 {
+    if (r->start)
+        RC(check_ptr(op, "rows->start", r->start, 4, dev));
+    if (r->n_rows == 0)
+        return LFM_OK;
     RC(check_ptr(op, "rows->q", r->q, 16, dev));
     RC(check_ptr(op, "rows->out", r->out, 16, dev));
     if (r->q == r->out)
         return fail(LFM_EINVAL, "%s: out is q", op);
-    if (r->lse)
-        RC(check_ptr(op, "rows->lse", r->lse, 4, dev));
-    if (r->start)
-        RC(check_ptr(op, "rows->start", r->start, 4, dev));
-    return LFM_OK;
+    return r->lse ? check_ptr(op, "rows->lse", r->lse, 4, dev) : LFM_OK;
 }
 
 static int check_workspace(const char *op, void *p, size_t have, size_t need, int dev)
@@ -487,8 +488,7 @@ extern "C" int lfm_attn_scored(const lfm_kv *kv, const lfm_rows *rows, const flo
     int dev;
     RC(current_device(op, (hipStream_t)stream, &dev));
     RC(check_kv_ptrs(op, KV_NAMES, kv, dev));
-    if (rows->n_rows)
-        RC(check_rows_ptrs(op, rows, dev));
+    RC(check_rows_ptrs(op, rows, dev));
     if (acc_in)
         RC(check_ptr(op, "acc_in", acc_in, 4, dev));
     RC(check_ptr(op, "acc_out", acc_out, 4, dev));
