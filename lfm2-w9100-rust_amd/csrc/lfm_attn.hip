@@ -789,10 +789,11 @@ template <typename TQ> __device__ __forceinline__ bool has_nonfinite(u32x4 v)
 // 16 bytes a lane from memory to shared memory, lane x's to byte `to` + 16 x (uniform),
 // with no register between.  Written out because the compiler makes every read of shared
 // memory wait for such loads, the other buffer's too: whoever reads waits with wait_loads
-// and a barrier.
+// and a barrier.  The place in shared memory is an operand in M0, which the compiler so
+// knows to be in use (the load may follow M0's writing after one wait state).
 __device__ __forceinline__ void load_to_lds(const void *from, uint32_t to)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(to), "v"(from) : "memory");
 }
 __device__ __forceinline__ uint32_t lds_address(void *p)
 {
