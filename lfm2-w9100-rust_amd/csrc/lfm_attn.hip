@@ -1165,7 +1165,9 @@ template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const
     }
     floatx4 sum[KT] = {};
     // a thread's pieces of a step, and the state of the row that it holds for thread < 64
-    typedef tq tq8 __attribute__((ext_vector_type(8)));
+    // rows are 16-byte aligned; the natural alignment of eight floats is 32
+    typedef tq tq8 __attribute__((ext_vector_type(8), aligned(16)));
+    static_assert(alignof(tq8) == 16, "no more than the rows' own alignment");
     tq8 piece[PER];
     float2 st;
     int32_t pos = -1;
