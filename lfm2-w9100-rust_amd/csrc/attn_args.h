@@ -22,7 +22,8 @@ struct RowsView {
     const int32_t *start;
     int64_t q_rs, q_hs, o_rs, o_hs;
     uint32_t heads, n_rows;
-    float scale, cexp; // cexp = scale * log2(e)
+    float cexp, cfrac; // scale * log2(e), a normal number; cexp = cfrac * 2^cpow, cfrac in [0.5, 1)
+    int32_t cpow;
 };
 
 #define MAX_GROUP 128     // query heads of a kv head
@@ -46,8 +47,8 @@ struct AttnOpArgs {
     uint32_t step_prefix;               // items of the step kernel that are the prefix's
     float2 *ml;
     float *o;
-    // scored: scores[(b * heads + h) * score_row + j], in units of q . k; score_row is slots
-    // rounded up to whole blocks
+    // scored: scores[(b * heads + h) * score_row + j] = q . k (F32 rows: 2^cpow q . k, which is in
+    // range where the score is); score_row is slots rounded up to whole blocks
     float *scores;
     uint32_t score_row;
     uint32_t sum_parts;

@@ -1,5 +1,6 @@
 // attn_ops.cpp -- C ABI of the cache-attention operators: argument checks, work splits and
 // launches of the kernels in lfm_attn.hip.
+#include <float.h>
 #include <hip/hip_runtime_api.h>
 #include <math.h>
 #include <stdint.h>
@@ -244,8 +245,13 @@ static RowsView view(const lfm_rows *r)
     v.q_rs = r->q_row_stride, v.q_hs = r->q_head_stride;
     v.o_rs = r->out_row_stride, v.o_hs = r->out_head_stride;
     v.heads = r->heads, v.n_rows = r->n_rows;
-    v.scale = r->scale;
-    v.cexp = (float)((double)r->scale * 1.4426950408889634);
+    // Kept a normal number at both ends of 32 bits, so that a masked score of -infinity and one of
+    // 0 stay such; the scores of 16-bit rows are no others for it.
+    const double c = (double)r->scale * 1.4426950408889634;
+    v.cexp = (float)std::min(std::max(c, (double)FLT_MIN), (double)FLT_MAX);
+    int pow;
+    v.cfrac = frexpf(v.cexp, &pow);
+    v.cpow = pow;
     return v;
 }
 

@@ -152,11 +152,11 @@ struct Pairs {
 
 // RT tiles of 16 query rows as B operands (the lane's row: lane % 16).  An F32 row is scaled
 // by the power of two that brings its largest value into binary16's range, and its scores
-// back by c.
+// back by c = cfrac * back.
 template <typename TQ, int D, int RT> struct Queries {
     static constexpr int N = TQ::parts == 2 ? RT : 1;
     typename TQ::vec q[RT][TQ::parts][D / 32];
-    float c[N], back[N]; // cexp / power; 1 / power
+    float c[N], back[N];
     __device__ __forceinline__ float c_of(int t) const { return c[N == 1 ? 0 : t]; }
 };
 
@@ -166,6 +166,15 @@ __device__ __forceinline__ int power_up(float top)
     if (top > 0.f && top < INFINITY)
         frexpf(top, &ex);
     return min(14 - ex, 126);
+}
+
+// 2^cpow over the power that a row was scaled by.  Row and scale may each be far out of the
+// scores' range: the two powers meet here first, and where their quotient would be no normal
+// number (the scores are 0 or past 32 bits then) it stays one, so that a masked score remains
+// an infinity and no 0 becomes NaN.
+__device__ __forceinline__ float power_back(const RowsView &r, int up)
+{
+    return ldexpf(1.f, max(-125, min(r.cpow - up, 127)));
 }
 
 template <typename TQ, int D, int RT>
@@ -202,8 +211,8 @@ __device__ __forceinline__ void load_row(Queries<TQ, D, RT> &Q, int t, const Row
         top = row_max(top);
         const int up = power_up(top);
         const float s = ldexpf(1.f, up);
-        Q.back[t] = ldexpf(1.f, -up);
-        Q.c[t] = r.cexp * Q.back[t];
+        Q.back[t] = power_back(r, up);
+        Q.c[t] = r.cfrac * Q.back[t];
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
 #pragma unroll
@@ -727,6 +736,7 @@ template <typename TQ, int D> __device__ __forceinline__ void scored_join(const 
             store_row<TQ, D>(a, b, kh * G + g, n == 0, top, sum, o);
     }
     __syncthreads();
+    const float c = TQ::parts == 2 ? a.r.cfrac : a.r.cexp;
     if (n)
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
@@ -734,9 +744,9 @@ template <typename TQ, int D> __device__ __forceinline__ void scored_join(const 
 #pragma unroll
             for (int g = 0; g < EARLY; ++g)
                 if (g < (int)G)
-                    sum += exp2_hw(fmaf(s[i][g], a.r.cexp, -st[g].x)) * st[g].y;
+                    sum += exp2_hw(fmaf(s[i][g], c, -st[g].x)) * st[g].y;
             for (uint32_t g = EARLY; g < G; ++g)
-                sum += exp2_hw(fmaf(scores[(size_t)g * a.score_row + j[i]], a.r.cexp, -st[g].x)) * st[g].y;
+                sum += exp2_hw(fmaf(scores[(size_t)g * a.score_row + j[i]], c, -st[g].x)) * st[g].y;
             if (chunk * SCORED_SLOTS + i * 256 + tid < n)
                 a.acc_out[at + j[i]] = had[i] + sum;
         }
@@ -838,8 +848,7 @@ __device__ void attn_row(const AttnOpArgs &a, const B &bl, uint32_t b0, uint32_t
             const tk *k = (const tk *)kp + j * a.own.ts;
             x = 0.f;
             for (int d = 0; d < D; ++d)
-                x = fmaf((float)q[d], (float)k[d], x);
-            x *= a.r.cexp;
+                x = fmaf((float)q[d] * a.r.cexp, (float)k[d], x);
         }
         const uint64_t any = __ballot(seen);
         const float top = wave_max(x);
@@ -1216,7 +1225,7 @@ template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const
                 *(vec *)(qs[buf][0] + to) = hi;
                 *(vec *)(qs[buf][1] + to) = lo_;
                 if (tid % PIECES == 0)
-                    rows[buf][x].c = a.r.cexp * ldexpf(1.f, -up);
+                    rows[buf][x].c = a.r.cfrac * power_back(a.r, up);
             }
         }
     };

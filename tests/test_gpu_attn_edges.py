@@ -42,3 +42,70 @@ def test_rows_of_16_byte_alignment(gpu, kind, dim):
         check_scored(gpu, many, cache, start, None)
         check_prefix(gpu, single, prefix, cache)
         check_prefix(gpu, many, prefix, cache, start)
+
+
+def tight_scored(gpu, r, cache, start=None, scale=None, acc_in=None, nan_rows=None):
+    """Runs the scored operator and checks out, lse and acc; acc with a bound of its own for
+    every slot: each pair's weight times that pair's relative error (its score and its lse, the
+    exponentials, the sum over the slots it sees), and the adding up of the sequence's pairs
+    of one kv head, in 32 bits in any order.  nan_rows: [row][head] whose outputs are not checked."""
+    n, kv, slots, dim = cache.k.shape
+    rows, heads, _ = r.shape
+    g = heads // kv
+    st = None if start is None else i32(start)
+    dst = f32(np.full((n, kv, slots), 55.0, np.float32))
+    ws = workspace(gpu, gpu.attn_scored_workspace(r.q, cache.view, start=st))
+    gpu.attn_scored(r.q, cache.view, r.out, None if acc_in is None else f32(acc_in), dst, ws, start=st, lse=r.lse,
+                    scale=scale)
+    got = dst.download().reshape(n, kv, slots).astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        out, lse, acc, extra = U.reference(r.values, cache, start, scale=scale)
+    size, reach, seen = extra
+    first = np.arange(n + 1) if start is None else np.asarray(start)
+    all_rows = slice(first[0], first[-1])
+    fine = np.ones((rows, heads), bool) if nan_rows is None else ~nan_rows
+    o, tol = r.result(), U.out_tolerance(np.nan_to_num(out), tuple(np.nan_to_num(x) for x in extra), r.kind, dim)
+    bad = ~(np.abs(o - out) <= tol) & fine[..., None]
+    assert not bad[all_rows].any(), (np.argwhere(bad)[:5], o[bad][:5], out[bad][:5], tol[bad][:5])
+    z, ztol = r.lse.download().reshape(rows, heads), U.lse_tolerance(lse, extra, dim)
+    with np.errstate(invalid="ignore"):
+        assert ((np.abs(z - lse) <= ztol) | ((lse == -np.inf) & (z == -np.inf)))[all_rows].all()
+    rel = 2.2 * U.score_error(reach, dim) + 2.0 ** -20 + (seen + 16) * 2.0 ** -24 + \
+        2.0 ** -21 * np.abs(np.where(np.isfinite(lse), lse, 0))
+    for b in range(n):
+        lo, hi, length = first[b], first[b + 1], min(max(int(cache.length[b]), 0), slots)
+        err = np.zeros((kv, slots))
+        for row in range(lo, hi):
+            p = length - hi + row
+            for h in range(heads):
+                if p >= 0:
+                    s = cache.k[b, h // g, :p + 1] @ r.values[row, h] * (
+                        dim ** -0.5 if scale is None else float(np.float32(scale)))
+                    err[h // g, :p + 1] += rel[row, h] * np.exp(s - lse[row, h])
+        base = np.zeros((kv, slots)) if acc_in is None else acc_in[b].astype(np.float64)
+        err += ((hi - lo) * g + 16) * 2.0 ** -24 * acc[b] + 2.0 ** -23 * np.abs(base + acc[b]) + 1e-12
+        bad = ~(np.abs(got[b] - base - acc[b]) <= err)
+        bad[:, length:] = got[b][:, length:] != 55.0
+        assert not bad.any(), (b, np.argwhere(bad)[:5], got[b][bad][:5], (base + acc[b])[bad][:5], err[bad][:5])
+    return got
+
+
+@pytest.mark.parametrize("spread, scale", [(1e-38, 1e-8), (0.0, 3e38), (1e38, 1e-38), (1e36, 2e-37), (2e-38, 5e37),
+                                           (1.0, 1e-45)])
+def test_scales_and_rows_at_the_ends_of_32_bits(gpu, spread, scale):
+    """Rows times scale are in range where neither is: masked slots stay masked (an infinity
+    times a factor that has become 0 is no number), and kept scores are in range too."""
+    rng = np.random.default_rng(31)
+    cache = Cache(rng, [77, 5, 40], 2, 101, 64, "f16")
+    prefix = Cache(rng, [130], 2, 131, 64, "f16")
+    for kind in ("f32",) if 0 < spread != 1 else ("f32", "f16"):
+        for start, n in ((None, 3), ([0, 60, 65, 100], 100)):
+            # of as many normal numbers as 100 rows have some are past 3.4
+            r = Rows(gpu, rng, n, 6, 64, kind, spread=spread if n == 3 else min(spread, 1e37))
+            check_window(gpu, r, cache, start, 30, 3, scale=scale)
+            tight_scored(gpu, r, cache, start, scale=scale)
+            st = None if start is None else i32(start)
+            ws = workspace(gpu, gpu.attn_prefix_workspace(r.q, prefix.view, cache.view, start=st))
+            gpu.attn_prefix(r.q, prefix.view, cache.view, r.out, ws, start=st, lse=r.lse, scale=scale)
+            out, _, _, extra = U.reference(r.values, cache, start, prefix=prefix, scale=scale)
+            check_out(r.result(), out, extra, kind, 64)
