@@ -653,8 +653,9 @@ __device__ __forceinline__ void join(const AttnOpArgs &a, uint32_t id, uint32_t 
                 x[j][i] = a.o[((size_t)min(s0 + j, n - 1) * pairs + id) * D + lane * E + i];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
+            // a range whose weights vanish beside the others' counts too: its NaN stays
             const float w = lane_f32(f, min(s0 + j, 63u));
-            if (s0 + j < n && w > 0.f)
+            if (s0 + j < n)
 #pragma unroll
                 for (int i = 0; i < E; ++i)
                     o[i] += w * x[j][i];

@@ -109,3 +109,43 @@ def test_scales_and_rows_at_the_ends_of_32_bits(gpu, spread, scale):
             gpu.attn_prefix(r.q, prefix.view, cache.view, r.out, ws, start=st, lse=r.lse, scale=scale)
             out, _, _, extra = U.reference(r.values, cache, start, prefix=prefix, scale=scale)
             check_out(r.result(), out, extra, kind, 64)
+
+
+@pytest.mark.parametrize("kind, dim", [("f32", 64), ("f16", 128), ("bf16", 64)])
+@pytest.mark.parametrize("n_rows", [1, 40])
+def test_nan_where_weights_vanish(gpu, kind, dim, n_rows):
+    """V is no number in seen slots whose weights are 0 beside the others': 0 times NaN is NaN,
+    however the slots are cut into ranges (2000 slots: several), and all other dims are fine."""
+    rng = np.random.default_rng([dim, 32])
+    cached = "bf16" if kind == "bf16" else "f16"
+    q = rng.standard_normal(dim)
+    for slots in (400, 2000):
+        def near(k, v):
+            k[:] = np.where(np.arange(k.shape[2]) < slots // 2, 10.0, -10.0)[:, None] * q
+            v[:, :, slots - 60, :3] = np.nan
+
+        cache = Cache(rng, [slots], 1, slots, dim, cached, edit=near)
+        r = Rows(gpu, rng, n_rows, 2, dim, kind)
+        r.values[:] = decode(encode(np.broadcast_to(q, r.shape), kind), kind)
+        r.q = U.tensor(r.values, kind)[0]
+        start = None if n_rows == 1 else i32([0, n_rows])
+        for run in ("window", "scored", "prefix"):
+            if run == "window":
+                ws = workspace(gpu, gpu.attn_window_workspace(r.q, cache.view, start=start))
+                gpu.attn_window(r.q, cache.view, r.out, ws, start=start)
+            elif run == "scored":
+                ws = workspace(gpu, gpu.attn_scored_workspace(r.q, cache.view, start=start))
+                acc = f32(np.zeros((1, 1, slots)))
+                gpu.attn_scored(r.q, cache.view, r.out, None, acc, ws, start=start)
+                a = acc.download()
+                # each of the 2 n_rows pairs' weights add up to 1, but for each one's relative error
+                reach = 10 * np.abs(q).max() * np.abs(q).sum() * dim ** -0.5
+                err = 2.2 * U.score_error(reach, dim) + 2.0 ** -20 + (slots + 2 * n_rows + 32) * 2.0 ** -24
+                assert np.isfinite(a).all() and abs(a.astype(np.float64).sum() - 2 * n_rows) < 2 * n_rows * err
+            else:
+                own = Cache(rng, [n_rows], 1, n_rows, dim, cached, edit=lambda k, v: k.fill(0))
+                ws = workspace(gpu, gpu.attn_prefix_workspace(r.q, cache.view, own.view, start=start))
+                gpu.attn_prefix(r.q, cache.view, own.view, r.out, ws, start=start)
+            got = r.result()
+            where = np.argwhere(np.isnan(got) != (np.arange(dim) < 3))
+            assert not len(where), (slots, run, len(where), where[:3])
