@@ -22,8 +22,7 @@ struct RowsView {
     const int32_t *start;
     int64_t q_rs, q_hs, o_rs, o_hs;
     uint32_t heads, n_rows;
-    float cexp, cfrac; // scale * log2(e), a normal number; cexp = cfrac * 2^cpow, cfrac in [0.5, 1)
-    int32_t cpow;
+    float cfrac, cexp; // cexp = scale * log2(e), a normal number = cfrac * 2^cpow, cfrac in [0.5, 1)
 };
 
 #define MAX_GROUP 128     // query heads of a kv head

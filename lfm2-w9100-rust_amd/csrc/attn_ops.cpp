@@ -249,9 +249,8 @@ static RowsView view(const lfm_rows *r)
     // 0 stay such; the scores of 16-bit rows are no others for it.
     const double c = (double)r->scale * 1.4426950408889634;
     v.cexp = (float)std::min(std::max(c, (double)FLT_MIN), (double)FLT_MAX);
-    int pow;
-    v.cfrac = frexpf(v.cexp, &pow);
-    v.cpow = pow;
+    int cpow;
+    v.cfrac = frexpf(v.cexp, &cpow);
     return v;
 }
 

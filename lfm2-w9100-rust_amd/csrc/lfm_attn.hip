@@ -174,7 +174,9 @@ __device__ __forceinline__ int power_up(float top)
 // an infinity and no 0 becomes NaN.
 __device__ __forceinline__ float power_back(const RowsView &r, int up)
 {
-    return ldexpf(1.f, max(-125, min(r.cpow - up, 127)));
+    int cpow;
+    frexpf(r.cexp, &cpow);
+    return ldexpf(1.f, max(-125, min(cpow - up, 127)));
 }
 
 template <typename TQ, int D, int RT>
@@ -848,8 +850,14 @@ __device__ void attn_row(const AttnOpArgs &a, const B &bl, uint32_t b0, uint32_t
         if (seen) {
             const tk *k = (const tk *)kp + j * a.own.ts;
             x = 0.f;
-            for (int d = 0; d < D; ++d)
-                x = fmaf((float)q[d] * a.r.cexp, (float)k[d], x);
+            if constexpr (TQ::parts == 2) { // q . k alone may be out of range
+                for (int d = 0; d < D; ++d)
+                    x = fmaf(q[d] * a.r.cexp, (float)k[d], x);
+            } else {
+                for (int d = 0; d < D; ++d)
+                    x = fmaf((float)q[d], (float)k[d], x);
+                x *= a.r.cexp;
+            }
         }
         const uint64_t any = __ballot(seen);
         const float top = wave_max(x);
