@@ -759,6 +759,19 @@ def _space(workspace):
     return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
+def _stream(stream: Optional[int], *tensors) -> int:
+    """A call's stream: the one given, or else torch's current stream for torch tensors (whose
+    contents may still be on their way there) and the default stream for others."""
+    if stream is not None:
+        return stream
+    for t in tensors:
+        if getattr(t, "is_cuda", False):
+            import torch
+
+            return torch.cuda.current_stream(t.device).cuda_stream
+    return 0
+
+
 def attn_window_workspace(q, cache: KvCache, *, window: int = 0, sinks: int = 0, start=None) -> int:
     n = C.c_size_t()
     _check(lib().lfm_attn_window_workspace(cache._ref, _rows(q, cache, None, start, None, None), window,
@@ -767,15 +780,17 @@ def attn_window_workspace(q, cache: KvCache, *, window: int = 0, sinks: int = 0,
 
 
 def attn_window(q, cache: KvCache, out, workspace, *, window: int = 0, sinks: int = 0, start=None,
-                scale: Optional[float] = None, lse=None, stream: int = 0):
+                scale: Optional[float] = None, lse=None, stream: Optional[int] = None):
     """out[row][head] = softmax(scale q K^T) V over the newest ``window`` positions up to the
     row's own (0: all) and the first ``sinks`` (lfm_attn_window).  q and out are
     [n_rows][heads][head_dim]; start (int32 [n_seq + 1], device) gives each sequence's rows,
-    None one row per sequence.  Enqueued on ``stream`` (a HIP stream's address); workspace:
-    attn_window_workspace(...) bytes for the same arguments."""
+    None one row per sequence.  Enqueued on ``stream`` (a HIP stream's address; None: torch's
+    current stream for torch tensors, else the default stream; 0: the default stream);
+    workspace: attn_window_workspace(...) bytes for the same arguments."""
     r = _rows(q, cache, out, start, scale, lse)
     p, n = _space(workspace)
-    _check(lib().lfm_attn_window(cache._ref, r, window, sinks, p, n, stream))
+    _check(lib().lfm_attn_window(cache._ref, r, window, sinks, p, n,
+                                 _stream(stream, q, cache.k)))
 
 
 def attn_scored_workspace(q, cache: KvCache, *, start=None) -> int:
@@ -786,7 +801,7 @@ def attn_scored_workspace(q, cache: KvCache, *, start=None) -> int:
 
 
 def attn_scored(q, cache: KvCache, out, acc_in, acc_out, workspace, *, start=None,
-                scale: Optional[float] = None, lse=None, stream: int = 0):
+                scale: Optional[float] = None, lse=None, stream: Optional[int] = None):
     """Attention over all positions, and acc_out = acc_in + the weights that every slot in
     use receives from its kv head's query heads and the sequence's rows (lfm_attn_scored).
     acc [n_seq][kv_heads][slots] float32; acc_in None counts as zeros, and may be acc_out."""
@@ -795,7 +810,8 @@ def attn_scored(q, cache: KvCache, out, acc_in, acc_out, workspace, *, start=Non
     p, n = _space(workspace)
     _check(lib().lfm_attn_scored(cache._ref, r,
                                  None if acc_in is None else _dense(acc_in, "acc_in", "f32", shape),
-                                 _dense(acc_out, "acc_out", "f32", shape), p, n, stream))
+                                 _dense(acc_out, "acc_out", "f32", shape), p, n,
+                                 _stream(stream, q, cache.k)))
 
 
 def attn_prefix_workspace(q, prefix: KvCache, cache: KvCache, *, start=None) -> int:
@@ -806,12 +822,12 @@ def attn_prefix_workspace(q, prefix: KvCache, cache: KvCache, *, start=None) -> 
 
 
 def attn_prefix(q, prefix: KvCache, cache: KvCache, out, workspace, *, start=None,
-                scale: Optional[float] = None, lse=None, stream: int = 0):
+                scale: Optional[float] = None, lse=None, stream: Optional[int] = None):
     """Attention of a batch that shares a prefix (a KvCache of one sequence): every row sees
     the whole prefix, then its own sequence up to its position (lfm_attn_prefix)."""
     r = _rows(q, cache, out, start, scale, lse)
     p, n = _space(workspace)
-    _check(lib().lfm_attn_prefix(prefix._ref, cache._ref, r, p, n, stream))
+    _check(lib().lfm_attn_prefix(prefix._ref, cache._ref, r, p, n, _stream(stream, q, cache.k)))
 
 
 def kv_evict_workspace(cache: KvCache, keep: int) -> int:
@@ -821,7 +837,7 @@ def kv_evict_workspace(cache: KvCache, keep: int) -> int:
 
 
 def kv_evict(cache: KvCache, acc, pos, keep: int, out: KvCache, acc_out, pos_out, workspace, *,
-             sinks: int = 0, recent: int = 0, stream: int = 0):
+             sinks: int = 0, recent: int = 0, stream: Optional[int] = None):
     """Keeps ``keep`` slots of every longer sequence, per kv head: the first ``sinks`` and the
     newest ``recent`` positions, then the slots of highest acc (lfm_kv_evict).  In place
     where out is cache, acc_out is acc and pos_out is pos."""
@@ -829,7 +845,7 @@ def kv_evict(cache: KvCache, acc, pos, keep: int, out: KvCache, acc_out, pos_out
     p, n = _space(workspace)
     _check(lib().lfm_kv_evict(cache._ref, _dense(acc, "acc", "f32", a), _dense(pos, "pos", "i32", a), keep, sinks,
                               recent, out._ref, _dense(acc_out, "acc_out", "f32", b),
-                              _dense(pos_out, "pos_out", "i32", b), p, n, stream))
+                              _dense(pos_out, "pos_out", "i32", b), p, n, _stream(stream, acc, cache.k)))
 
 
 # ------------------------------------------------------------------ Q6_K operator API

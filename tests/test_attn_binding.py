@@ -1,0 +1,39 @@
+"""The Python binding of the cache-attention operators, without a device."""
+from test_attn_ops import Host
+
+
+class OnGpu(Host):
+    """Stands for a torch tensor on a device."""
+    is_cuda, device = True, "cuda:0"
+
+
+def test_binding_takes_torchs_current_stream(lfm, monkeypatch):
+    """Without a stream, calls on torch tensors go to torch's current stream, where those are
+    made; calls on others to the default stream; a stream that is given is taken as it is."""
+    import torch
+
+    calls, devices = [], []
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: calls.append((name, args[-1])) or 0
+
+    class Stream:
+        cuda_stream = 4711
+
+    monkeypatch.setattr(lfm, "lib", Library)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: devices.append(device) or Stream)
+    for tensor, given, want in ((OnGpu, None, 4711), (OnGpu, 0, 0), (OnGpu, 99, 99), (Host, None, 0), (Host, 99, 99)):
+        kw = {} if given is None else {"stream": given}
+        k, ws = tensor((3, 8, 100, 64)), tensor((1 << 20,))
+        cache = lfm.KvCache(k, k, tensor((3,), "torch.int32"))
+        prefix = lfm.KvCache(tensor((1, 8, 100, 64)), tensor((1, 8, 100, 64)), tensor((1,), "torch.int32"))
+        q, acc = tensor((3, 32, 64)), tensor((3, 8, 100), "torch.float32")
+        pos = tensor((3, 8, 100), "torch.int32")
+        del calls[:]
+        lfm.attn_window(q, cache, q, ws, window=5, **kw)
+        lfm.attn_scored(q, cache, q, None, acc, ws, **kw)
+        lfm.attn_prefix(q, prefix, cache, q, ws, **kw)
+        lfm.kv_evict(cache, acc, pos, 50, cache, acc, pos, ws, **kw)
+        assert calls == [(n, want) for n in ("lfm_attn_window", "lfm_attn_scored", "lfm_attn_prefix", "lfm_kv_evict")]
+    assert set(devices) == {"cuda:0"}

@@ -1,0 +1,15 @@
+"""The cache-attention binding over torch tensors (attn_torch_child.py, a process of its own)."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def test_torch_tensors(gpu):
+    child = os.path.join(os.path.dirname(os.path.abspath(__file__)), "attn_torch_child.py")
+    p = subprocess.run([sys.executable, child], capture_output=True, text=True, timeout=100)
+    assert p.returncode == 0, p.stdout + p.stderr
+    assert [x for x in p.stdout.splitlines()] == ["views ok", "side stream ok", "graph ok", "host tensor refused"]
