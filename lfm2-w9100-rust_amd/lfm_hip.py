@@ -759,16 +759,25 @@ def _space(workspace):
     return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
+_torch_stream = None  # device index -> address of torch's current stream there
+
+
 def _stream(stream: Optional[int], *tensors) -> int:
     """A call's stream: the one given, or else torch's current stream for torch tensors (whose
     contents may still be on their way there) and the default stream for others."""
+    global _torch_stream
     if stream is not None:
         return stream
     for t in tensors:
         if getattr(t, "is_cuda", False):
-            import torch
+            if _torch_stream is None:
+                import torch
 
-            return torch.cuda.current_stream(t.device).cuda_stream
+                # the address alone, where torch offers it: torch.cuda.current_stream takes
+                # 2.7 us, a quarter of a small call's time
+                _torch_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+                    lambda index: torch.cuda.current_stream(index).cuda_stream)
+            return _torch_stream(t.get_device())
     return 0
 
 

@@ -4,25 +4,23 @@ from test_attn_ops import Host
 
 class OnGpu(Host):
     """Stands for a torch tensor on a device."""
-    is_cuda, device = True, "cuda:0"
+    is_cuda = True
+
+    def get_device(self):
+        return 0
 
 
 def test_binding_takes_torchs_current_stream(lfm, monkeypatch):
     """Without a stream, calls on torch tensors go to torch's current stream, where those are
     made; calls on others to the default stream; a stream that is given is taken as it is."""
-    import torch
-
     calls, devices = [], []
 
     class Library:
         def __getattr__(self, name):
             return lambda *args: calls.append((name, args[-1])) or 0
 
-    class Stream:
-        cuda_stream = 4711
-
     monkeypatch.setattr(lfm, "lib", Library)
-    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: devices.append(device) or Stream)
+    monkeypatch.setattr(lfm, "_torch_stream", lambda index: devices.append(index) or 4711)
     for tensor, given, want in ((OnGpu, None, 4711), (OnGpu, 0, 0), (OnGpu, 99, 99), (Host, None, 0), (Host, 99, 99)):
         kw = {} if given is None else {"stream": given}
         k, ws = tensor((3, 8, 100, 64)), tensor((1 << 20,))
@@ -36,4 +34,4 @@ def test_binding_takes_torchs_current_stream(lfm, monkeypatch):
         lfm.attn_prefix(q, prefix, cache, q, ws, **kw)
         lfm.kv_evict(cache, acc, pos, 50, cache, acc, pos, ws, **kw)
         assert calls == [(n, want) for n in ("lfm_attn_window", "lfm_attn_scored", "lfm_attn_prefix", "lfm_kv_evict")]
-    assert set(devices) == {"cuda:0"}
+    assert set(devices) == {0}
