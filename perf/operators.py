@@ -177,7 +177,6 @@ def _own(s):
     case, op = s["case"], s["case"]["op"]
     start = s["start"] if s["most"] > 1 else None
     if "cache" not in s:  # made once by a program: the views of its caches and a workspace
-        s["stream"] = torch.cuda.current_stream().cuda_stream
         cache = s["cache"] = lfm_hip.KvCache(s["k"], s["v"], s["length"])
         if op == "evict":
             s["kept"] = lfm_hip.KvCache(s["k_out"], s["v_out"], s["length_out"])
@@ -190,22 +189,21 @@ def _own(s):
             s["prefix"] = lfm_hip.KvCache(s["pk"], s["pv"], s["plength"])
             n = lfm_hip.attn_prefix_workspace(s["q"], s["prefix"], cache, start=start)
         s["workspace"] = torch.empty(max(n, 1), dtype=torch.uint8, device="cuda")
-    cache, workspace, stream = s["cache"], s["workspace"], s["stream"]
+    cache, workspace = s["cache"], s["workspace"]
     if op == "evict":
         lfm_hip.kv_evict(cache, s["acc"], s["pos"], case["keep"], s["kept"], s["acc_out"], s["pos_out"], workspace,
-                         sinks=case["sinks"], recent=case["recent"], stream=stream)
+                         sinks=case["sinks"], recent=case["recent"])
         return {"k": s["k_out"], "v": s["v_out"], "acc": s["acc_out"], "pos": s["pos_out"],
                 "length": s["length_out"]}
     if op == "window":
         lfm_hip.attn_window(s["q"], cache, s["out"], workspace, window=case["window"], sinks=case["sinks"],
-                            start=start, scale=s["scale"], lse=s["lse"], stream=stream)
+                            start=start, scale=s["scale"], lse=s["lse"])
         return {"out": s["out"], "lse": s["lse"]}
     if op == "scored":
         lfm_hip.attn_scored(s["q"], cache, s["out"], s["acc"], s["acc_out"], workspace, start=start,
-                            scale=s["scale"], stream=stream)
+                            scale=s["scale"])
         return {"out": s["out"], "acc": s["acc_out"]}
-    lfm_hip.attn_prefix(s["q"], s["prefix"], cache, s["out"], workspace, start=start, scale=s["scale"],
-                        stream=stream)
+    lfm_hip.attn_prefix(s["q"], s["prefix"], cache, s["out"], workspace, start=start, scale=s["scale"])
     return {"out": s["out"]}
 
 
