@@ -759,6 +759,13 @@ def _space(workspace):
     return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
+def _u32(what: str, *values) -> None:
+    """Refuses what ctypes would cut down to its low 32 bits."""
+    for v in values:
+        if not isinstance(v, (int, np.integer)) or not 0 <= v <= 0xFFFFFFFF:
+            raise LfmError(LFM_EINVAL, f"{what}: {v!r} (a whole number of 32 bits, not negative, expected)")
+
+
 _torch_stream = None  # device index -> address of torch's current stream there
 
 
@@ -782,6 +789,7 @@ def _stream(stream: Optional[int], *tensors) -> int:
 
 
 def attn_window_workspace(q, cache: KvCache, *, window: int = 0, sinks: int = 0, start=None) -> int:
+    _u32("window, sinks", window, sinks)
     n = C.c_size_t()
     _check(lib().lfm_attn_window_workspace(cache._ref, _rows(q, cache, None, start, None, None), window,
                                            sinks, C.byref(n)))
@@ -796,6 +804,7 @@ def attn_window(q, cache: KvCache, out, workspace, *, window: int = 0, sinks: in
     None one row per sequence.  Enqueued on ``stream`` (a HIP stream's address; None: torch's
     current stream for torch tensors, else the default stream; 0: the default stream);
     workspace: attn_window_workspace(...) bytes for the same arguments."""
+    _u32("window, sinks", window, sinks)
     r = _rows(q, cache, out, start, scale, lse)
     p, n = _space(workspace)
     _check(lib().lfm_attn_window(cache._ref, r, window, sinks, p, n,
@@ -840,6 +849,7 @@ def attn_prefix(q, prefix: KvCache, cache: KvCache, out, workspace, *, start=Non
 
 
 def kv_evict_workspace(cache: KvCache, keep: int) -> int:
+    _u32("keep", keep)
     n = C.c_size_t()
     _check(lib().lfm_kv_evict_workspace(cache._ref, keep, C.byref(n)))
     return n.value
@@ -850,6 +860,7 @@ def kv_evict(cache: KvCache, acc, pos, keep: int, out: KvCache, acc_out, pos_out
     """Keeps ``keep`` slots of every longer sequence, per kv head: the first ``sinks`` and the
     newest ``recent`` positions, then the slots of highest acc (lfm_kv_evict).  In place
     where out is cache, acc_out is acc and pos_out is pos."""
+    _u32("keep, sinks, recent", keep, sinks, recent)
     a, b = cache._acc_shape, out._acc_shape
     p, n = _space(workspace)
     _check(lib().lfm_kv_evict(cache._ref, _dense(acc, "acc", "f32", a), _dense(pos, "pos", "i32", a), keep, sinks,

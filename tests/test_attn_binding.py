@@ -1,4 +1,7 @@
 """The Python binding of the cache-attention operators, without a device."""
+import numpy as np
+import pytest
+
 from test_attn_ops import Host
 
 
@@ -35,3 +38,26 @@ def test_binding_takes_torchs_current_stream(lfm, monkeypatch):
         lfm.kv_evict(cache, acc, pos, 50, cache, acc, pos, ws, **kw)
         assert calls == [(n, want) for n in ("lfm_attn_window", "lfm_attn_scored", "lfm_attn_prefix", "lfm_kv_evict")]
     assert set(devices) == {0}
+
+
+def test_binding_refuses_numbers_past_32_bits(lfm):
+    """ctypes would take their low 32 bits: window -1 as a large one, keep 2^32 + 50 as 50."""
+    k, ws = Host((3, 8, 100, 64)), Host((1 << 20,))
+    cache = lfm.KvCache(k, k, Host((3,), "torch.int32"))
+    q, acc, pos = Host((3, 32, 64)), Host((3, 8, 100), "torch.float32"), Host((3, 8, 100), "torch.int32")
+
+    def evict(**kw):
+        a = dict(keep=50, sinks=0, recent=0)
+        a.update(kw)
+        lfm.kv_evict(cache, acc, pos, a.pop("keep"), cache, acc, pos, ws, **a)
+
+    for bad in (-1, 1 << 32, (1 << 32) + 50, 3.0, None):
+        for call in (lambda: lfm.attn_window_workspace(q, cache, window=bad),
+                     lambda: lfm.attn_window_workspace(q, cache, sinks=bad),
+                     lambda: lfm.attn_window(q, cache, q, ws, window=bad), lambda: lfm.attn_window(q, cache, q, ws, sinks=bad),
+                     lambda: lfm.kv_evict_workspace(cache, bad), lambda: evict(keep=bad), lambda: evict(sinks=bad),
+                     lambda: evict(recent=bad)):
+            with pytest.raises(lfm.LfmError) as e:
+                call()
+            assert e.value.code == lfm.LFM_EINVAL and "32 bits" in str(e.value)
+    assert lfm.attn_window_workspace(q, cache, window=np.int64(7), sinks=0xFFFFFFFF) >= 0
