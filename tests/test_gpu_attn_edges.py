@@ -149,3 +149,177 @@ def test_nan_where_weights_vanish(gpu, kind, dim, n_rows):
             got = r.result()
             where = np.argwhere(np.isnan(got) != (np.arange(dim) < 3))
             assert not len(where), (slots, run, len(where), where[:3])
+
+
+# ------------------------------------------------------------------ rows of many tokens in key ranges
+@pytest.mark.parametrize("kind, dim", [("f32", 64), ("f16", 64), ("bf16", 64), ("f32", 128), ("f16", 128), ("bf16", 128)])
+def test_scored_chunks_in_ranges(gpu, kind, dim):
+    """Few rows over more than 1024 slots: their states come from joined key ranges."""
+    rng = np.random.default_rng([dim, 33])
+    cache = Cache(rng, [2203, 1, 1025, 40, 0], 2, 2207, dim, "bf16" if kind == "bf16" else "f16", "slot")
+    start = np.concatenate([[1], 1 + np.cumsum([37, 1, 3, 45, 2])])
+    r = Rows(gpu, rng, int(start[-1]) + 2, 6, dim, kind)
+    tight_scored(gpu, r, cache, start, acc_in=rng.random((5, 2, 2207), dtype=np.float32))
+    assert r.untouched([0, -1, -2])
+
+
+@pytest.mark.parametrize("kind, dim", [("f32", 64), ("f16", 64), ("bf16", 128)])
+def test_scored_prompt_in_parts_and_ranges(gpu, kind, dim):
+    """A prompt whose weights are added in 16 parts, its rows in three key ranges."""
+    rng = np.random.default_rng([dim, 34])
+    cache = Cache(rng, [2100], 1, 2101, dim, "bf16" if kind == "bf16" else "f16")
+    r = Rows(gpu, rng, 2060, 4, dim, kind)
+    a = tight_scored(gpu, r, cache, [0, 2060])
+    assert np.array_equal(a, tight_scored(gpu, r, cache, [0, 2060]))
+
+
+@pytest.mark.parametrize("kind, dim", [("f16", 64), ("bf16", 128)])
+def test_scored_many_prompts_slot_by_slot(gpu, kind, dim):
+    """The larger tiles over many short sequences: what one slot receives from its sequence's
+    rows, each of which weighs far more than the bound."""
+    rng = np.random.default_rng([dim, 35])
+    counts = rng.integers(40, 80, 68 if dim == 64 else 50)
+    start = np.concatenate([[0], np.cumsum(counts)])
+    cache = Cache(rng, counts + rng.integers(-20, 40, len(counts)), 8, 120, dim, kind)
+    tight_scored(gpu, Rows(gpu, rng, int(start[-1]), 24, dim, kind), cache, start)
+
+
+@pytest.mark.parametrize("group", [1, 7, 16, 17, 50, 128])
+def test_scored_groups(gpu, group):
+    rng = np.random.default_rng([group, 36])
+    cache = Cache(rng, [90, 300, 5], 2, 301, 64, "f16")
+    tight_scored(gpu, Rows(gpu, rng, 3, 2 * group, 64, "f16"), cache)
+    tight_scored(gpu, Rows(gpu, rng, 24, 2 * group, 64, "f32"), cache, [0, 13, 19, 24])
+
+
+def check_seen(got, want, extra, kind, dim, rows, slots_nan, dims=3):
+    """got of rows: no number in the first dims where a row sees one of slots_nan, else the
+    formula's."""
+    out, size, reach, seen = want.copy(), *(x.copy() for x in extra)
+    hit = np.zeros(got.shape[0], bool)
+    for row, see in rows:
+        hit[row] = any(see(j) for j in slots_nan)
+    listed = np.array([row for row, _ in rows])
+    assert hit[listed].any() and not hit[listed].all()
+    expected = hit[:, None, None] & (np.arange(dim) < dims) & np.ones(got.shape, bool)
+    assert np.array_equal(np.isnan(out)[listed], expected[listed])  # the formula's NaN are these
+    assert np.array_equal(np.isnan(got)[listed], expected[listed])
+    tol = U.out_tolerance(np.nan_to_num(out), tuple(np.nan_to_num(x) for x in (size, reach, seen)), kind, dim)
+    bad = ~(np.abs(got - out) <= tol) & ~expected
+    assert not bad[listed].any(), (np.argwhere(bad)[:5], got[bad][:5], out[bad][:5], tol[bad][:5])
+
+
+@pytest.mark.parametrize("kind, dim", [("f32", 64), ("f16", 64), ("bf16", 64), ("f32", 128), ("f16", 128), ("bf16", 128)])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (300, 4)])
+def test_masked_nan_in_ranges(gpu, kind, dim, window, sinks):
+    """V is no number in slots that some rows of a chunk see and others do not, over more than
+    1024 slots: those rows' partial outputs come from the rows computed one by one."""
+    rng = np.random.default_rng([dim, window, 37])
+    length, counts, heads = [2000, 1300, 1100], [40, 25, 30], 3
+    odd = {0: [1975], 1: [1290]}
+    if window:  # and one that the window of later rows has passed
+        odd[0].append(1672), odd[1].append(981)
+
+    def edit(k, v):
+        for b, js in odd.items():
+            v[b, :, js, :3] = np.nan
+
+    cache = Cache(rng, length, 1, 2003, dim, "bf16" if kind == "bf16" else "f16", "slot", edit)
+    start = np.concatenate([[0], np.cumsum(counts)])
+    r = Rows(gpu, rng, int(start[-1]), heads, dim, kind)
+    check = []
+    for b in odd:
+        for row in range(start[b], start[b + 1]):
+            p = length[b] - int(start[b + 1]) + row
+            check.append((row, lambda j, p=p, b=b: j in odd[b] and j <= p and (
+                not window or j < sinks or j > p - window)))
+    ws = workspace(gpu, gpu.attn_window_workspace(r.q, cache.view, window=window, sinks=sinks, start=i32(start)))
+    gpu.attn_window(r.q, cache.view, r.out, ws, window=window, sinks=sinks, start=i32(start), lse=r.lse)
+    with np.errstate(invalid="ignore"):
+        out, lse, _, extra = U.reference(r.values, cache, start, window, sinks)
+    js = sorted({j for b in odd for j in odd[b]})
+    check_seen(r.result(), out, extra, kind, dim, check, js)
+    rest = slice(start[2], start[3])
+    check_out(r.result()[rest], out[rest], tuple(x[rest] for x in extra), kind, dim)
+    assert (np.abs(r.lse.download().reshape(lse.shape) - lse) <= U.lse_tolerance(lse, extra, dim)).all()
+    if window:
+        return
+    # the same scored: what slots receive has nothing to do with V
+    nan = np.zeros(r.shape[:2], bool)
+    for row, see in check:
+        nan[row] = any(see(j) for j in js)
+    tight_scored(gpu, r, cache, start, nan_rows=nan)
+    check_seen(r.result(), out, extra, kind, dim, check, js)
+
+
+@pytest.mark.parametrize("kind, dim", [("f32", 64), ("f16", 64), ("bf16", 64), ("f32", 128), ("f16", 128), ("bf16", 128)])
+@pytest.mark.parametrize("slots", [200, 1300])
+def test_masked_nan_behind_a_prefix(gpu, kind, dim, slots):
+    """The same for own slots behind a shared prefix, in one range of their own and in several."""
+    rng = np.random.default_rng([dim, slots, 38])
+    cached = "bf16" if kind == "bf16" else "f16"
+    length, counts, heads = [slots, slots - 40], [40, 25], 3
+    odd = [slots - 20, slots - 50]
+
+    def edit(k, v):
+        v[0, :, odd[0], :3] = v[1, :, odd[1], :3] = np.nan
+
+    prefix = Cache(rng, [600], 2, 610, dim, cached)
+    cache = Cache(rng, length, 2, slots + 3, dim, cached, "head", edit)
+    start = np.concatenate([[0], np.cumsum(counts)])
+    r = Rows(gpu, rng, int(start[-1]), 2 * heads, dim, kind)
+    ws = workspace(gpu, gpu.attn_prefix_workspace(r.q, prefix.view, cache.view, start=i32(start)))
+    gpu.attn_prefix(r.q, prefix.view, cache.view, r.out, ws, start=i32(start), lse=r.lse)
+    with np.errstate(invalid="ignore"):
+        out, lse, _, extra = U.reference(r.values, cache, start, prefix=prefix)
+    check = []
+    for b in range(2):
+        for row in range(start[b], start[b + 1]):
+            p = length[b] - int(start[b + 1]) + row
+            check.append((row, lambda j, p=p, b=b: j == odd[b] and j <= p))
+    check_seen(r.result(), out, extra, kind, dim, check, odd)
+    assert (np.abs(r.lse.download().reshape(lse.shape) - lse) <= U.lse_tolerance(lse, extra, dim)).all()
+
+
+@pytest.mark.parametrize("kind, dim", [("f32", 64), ("bf16", 128)])
+def test_masked_infinite_keys_in_ranges(gpu, kind, dim):
+    """K is no number or infinite in a slot that later rows of a chunk see: earlier ones do not
+    take part."""
+    rng = np.random.default_rng([dim, 39])
+
+    def edit(k, v):
+        k[0, :, 1980] = np.nan
+        k[0, :, 1990] = np.inf
+
+    cache = Cache(rng, [2000], 1, 2003, dim, "bf16" if kind == "bf16" else "f16", "slot", edit)
+    r = Rows(gpu, rng, 40, 3, dim, kind)
+    ws = workspace(gpu, gpu.attn_window_workspace(r.q, cache.view, start=i32([0, 40])))
+    gpu.attn_window(r.q, cache.view, r.out, ws, start=i32([0, 40]), lse=r.lse)
+    got = r.result()
+    assert np.isnan(got[20:]).all() and np.isfinite(got[:20]).all()
+    sane = Cache(np.random.default_rng([dim, 39]), [1980], 1, 2003, dim, "bf16" if kind == "bf16" else "f16", "slot")
+    out, lse, _, extra = U.reference(r.values[:20], sane, [0, 20])
+    check_out(got[:20], out, extra, kind, dim)
+    z = r.lse.download().reshape(40, 3)[:20]
+    assert (np.abs(z - lse) <= U.lse_tolerance(lse, extra, dim)).all()
+
+
+@pytest.mark.parametrize("kind, dim", [("f32", 64), ("f16", 128), ("bf16", 64)])
+def test_equal_calls_give_equal_bits(gpu, kind, dim):
+    rng = np.random.default_rng([dim, 40])
+    cached = "bf16" if kind == "bf16" else "f16"
+    cache = Cache(rng, [2500, 700], 2, 2500, dim, cached)
+    prefix = Cache(rng, [3001], 2, 3001, dim, cached)
+    for n, start in ((2, None), (900, [0, 600, 900])):
+        r = Rows(gpu, rng, n, 8, dim, kind)
+        st = None if start is None else i32(start)
+        acc = f32(np.zeros((2, 2, 2500)))
+        for call in (lambda ws: gpu.attn_window(r.q, cache.view, r.out, ws, window=900, sinks=3, start=st, lse=r.lse),
+                     lambda ws: gpu.attn_scored(r.q, cache.view, r.out, None, acc, ws, start=st, lse=r.lse),
+                     lambda ws: gpu.attn_prefix(r.q, prefix.view, cache.view, r.out, ws, start=st, lse=r.lse)):
+            bits = []
+            for fill in (0xFF, 0x00, 0x3C):  # whatever the workspace held
+                ws = workspace(gpu, 1 << 26, fill)
+                call(ws)
+                bits.append([x.download().tobytes() for x in (r.out, r.lse, acc)])
+            assert bits[0] == bits[1] == bits[2]
