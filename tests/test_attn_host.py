@@ -35,7 +35,7 @@ def call(host, lfm):
         host.stub_reset(0)
         host.stub_memory(MB, 63 * MB, 0)
         f = getattr(host, name)
-        f.argtypes = lfm.lib().__getattr__(name).argtypes
+        f.argtypes = getattr(lfm.lib(), name).argtypes
         rc = f(*args)
         grid, block, names = (C.c_uint32 * 3)(), C.c_uint32(), []
         for i in range(host.stub_launches()):
@@ -72,3 +72,98 @@ def test_scored_checks_start_without_rows(call, lfm, start):
     assert scored(call, kv(lfm), rows(lfm, n_rows=0, start=start)) == (lfm.LFM_EINVAL, [])
     # q, out and lse are not read then
     assert scored(call, kv(lfm), rows(lfm, n_rows=0, start=7 * MB, q=None, out=None))[0] == 0
+
+
+# ------------------------------------------------------------------ every pointer of every call
+def window(call, p):
+    return call("lfm_attn_window", C.byref(p["kv"]), C.byref(p["rows"]), 0, 0, *p["ws"], None)
+
+
+def scored_of(call, p):
+    return call("lfm_attn_scored", C.byref(p["kv"]), C.byref(p["rows"]), p["acc_in"], p["acc_out"], *p["ws"], None)
+
+
+def prefix(call, p):
+    return call("lfm_attn_prefix", C.byref(p["prefix"]), C.byref(p["kv"]), C.byref(p["rows"]), *p["ws"], None)
+
+
+def evict(call, p):
+    return call("lfm_kv_evict", C.byref(p["kv"]), p["acc_in"], p["pos"], 50, 4, 8, C.byref(p["out"]), p["acc_out"],
+                p["pos_out"], *p["ws"], None)
+
+
+def arguments(lfm, **kw):
+    a = dict(kv=kv(lfm, slots=2000), rows=rows(lfm, lse=11 * MB, start=7 * MB, n_rows=9), ws=(16 * MB, 40 * MB),
+             prefix=kv(lfm, n_seq=1, k=8 * MB, v=9 * MB, len=10 * MB), acc_in=6 * MB, acc_out=12 * MB, pos=13 * MB,
+             pos_out=14 * MB, out=kv(lfm, k=8 * MB, v=9 * MB, len=10 * MB))
+    a.update(kw)
+    return a
+
+
+POINTERS = [(window, s, f) for s, f in (("kv", "k"), ("kv", "v"), ("kv", "len"), ("rows", "q"), ("rows", "out"),
+                                        ("rows", "lse"), ("rows", "start"), ("ws", None))]
+POINTERS += [(scored_of, s, f) for s, f in (("kv", "k"), ("rows", "start"), ("acc_in", None), ("acc_out", None), ("ws", None))]
+POINTERS += [(prefix, s, f) for s, f in (("kv", "v"), ("rows", "q"), ("prefix", "k"), ("prefix", "v"), ("prefix", "len"),
+                                         ("ws", None))]
+POINTERS += [(evict, s, f) for s, f in (("kv", "k"), ("kv", "v"), ("kv", "len"), ("out", "k"), ("out", "v"), ("out", "len"),
+                                        ("acc_in", None), ("acc_out", None), ("pos", None), ("pos_out", None), ("ws", None))]
+OPTIONAL = {("rows", "lse"), ("acc_in", None)}
+
+
+@pytest.mark.parametrize("op, struct, field", POINTERS,
+                         ids=lambda v: v if isinstance(v, str) else "" if v is None else v.__name__)
+def test_every_pointer_is_checked(host, call, lfm, op, struct, field):
+    """A host address, another device's memory, one byte off and null: refused, nothing enqueued."""
+    rc, names = op(call, arguments(lfm))
+    assert rc == 0 and names, host.stub_error()
+    far = 100 * MB  # memory of device 1
+    for bad in (HOST, far, 1, None):
+        if bad is None and (op is not evict and (struct, field) in OPTIONAL or (struct, field) == ("rows", "start")):
+            continue
+        a = arguments(lfm)
+
+        def change(old):
+            return old + 1 if bad == 1 else bad
+        if field:
+            setattr(a[struct], field, change(getattr(a[struct], field)))
+        else:
+            a[struct] = (change(a[struct][0]), a[struct][1]) if struct == "ws" else change(a[struct])
+
+        def run(name, *args):
+            host.stub_reset(0)
+            host.stub_memory(MB, 63 * MB, 0)
+            host.stub_memory(far, MB, 1)
+            f = getattr(host, name)
+            f.argtypes = getattr(lfm.lib(), name).argtypes
+            return f(*args), [None] * host.stub_launches()
+        assert op(run, a) == (lfm.LFM_EINVAL, []), (bad, host.stub_error())
+        assert host.stub_error()
+
+
+def test_workspaces_one_byte_short(host, call, lfm):
+    n = C.c_size_t()
+    a = arguments(lfm)
+    k, r, p = C.byref(a["kv"]), C.byref(a["rows"]), C.byref(a["prefix"])
+    for op, size in ((window, lambda: host.lfm_attn_window_workspace(k, r, 0, 0, C.byref(n))),
+                     (scored_of, lambda: host.lfm_attn_scored_workspace(k, r, C.byref(n))),
+                     (prefix, lambda: host.lfm_attn_prefix_workspace(p, k, r, C.byref(n))),
+                     (evict, lambda: host.lfm_kv_evict_workspace(k, 50, C.byref(n)))):
+        a["ws"] = (16 * MB, 1 << 40)
+        assert size() == 0 and op(call, a)[0] == 0
+        a["ws"] = (16 * MB, n.value)
+        assert op(call, a)[0] == 0
+        if n.value:
+            a["ws"] = (16 * MB, n.value - 1)
+            assert op(call, a) == (lfm.LFM_EINVAL, [])
+
+
+def test_nothing_to_do_enqueues_nothing(call, lfm):
+    """No sequences, or no rows: fine, whatever the pointers are."""
+    none = arguments(lfm, kv=kv(lfm, n_seq=0, k=None, v=None, len=None), out=kv(lfm, n_seq=0, k=None, v=None, len=None),
+                     rows=rows(lfm, n_rows=0, q=None, out=None), ws=(None, 0), acc_in=None, acc_out=None, pos=None,
+                     pos_out=None)
+    # k and v alike are in place there
+    for op in (window, scored_of, prefix, evict):
+        assert op(call, none) == (0, []), op.__name__
+    rowless = arguments(lfm, rows=rows(lfm, n_rows=0, start=7 * MB, q=None, out=None))
+    assert window(call, rowless) == (0, []) and prefix(call, rowless) == (0, [])
