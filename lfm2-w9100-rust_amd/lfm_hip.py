@@ -736,7 +736,7 @@ def _rows(q, cache: KvCache, out, start, scale, lse) -> bytes:
     if kind is None or qs[2] != 1:
         raise LfmError(LFM_EINVAL, f"q: {_dtype(q)} with strides {tuple(qs)} (float32, binary16 or bfloat16, the last "
                        "dimension contiguous)")
-    os_, optr = qs, 0
+    os_, optr = (heads * dim, dim, 1), 0  # of a workspace query
     if out is not None:
         os_ = out.stride()
         if tuple(out.shape) != shape or _dtype(out) != _dtype(q) or os_[2] != 1:

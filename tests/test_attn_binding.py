@@ -61,3 +61,18 @@ def test_binding_refuses_numbers_past_32_bits(lfm):
                 call()
             assert e.value.code == lfm.LFM_EINVAL and "32 bits" in str(e.value)
     assert lfm.attn_window_workspace(q, cache, window=np.int64(7), sinks=0xFFFFFFFF) >= 0
+
+
+def test_workspace_of_one_query_for_all(lfm):
+    """q may have strides of 0 (one query for all rows, or all heads); outputs may not."""
+    cache = lfm.KvCache(Host((3, 8, 100, 64)), Host((3, 8, 100, 64)), Host((3,), "torch.int32"))
+    prefix = lfm.KvCache(Host((1, 8, 100, 64)), Host((1, 8, 100, 64)), Host((1,), "torch.int32"))
+    dense = Host((3, 32, 64))
+    for strides in ((0, 0, 1), (0, 64, 1), (64 * 32, 0, 1)):
+        q = Host((3, 32, 64), strides=strides)
+        assert lfm.attn_window_workspace(q, cache) == lfm.attn_window_workspace(dense, cache)
+        assert lfm.attn_scored_workspace(q, cache) == lfm.attn_scored_workspace(dense, cache)
+        assert lfm.attn_prefix_workspace(q, prefix, cache) == lfm.attn_prefix_workspace(dense, prefix, cache)
+        with pytest.raises(lfm.LfmError) as e:
+            lfm.attn_window(dense, cache, q, Host((1,)))
+        assert e.value.code == lfm.LFM_EINVAL and "out stride" in str(e.value)
