@@ -756,6 +756,9 @@ def _space(workspace):
     """Address and bytes of a workspace: a DeviceBuffer or a torch tensor of bytes."""
     if isinstance(workspace, DeviceBuffer):
         return workspace.ptr, workspace.nbytes
+    contiguous = getattr(workspace, "is_contiguous", None)
+    if contiguous is not None and not contiguous():
+        raise LfmError(LFM_EINVAL, "workspace: a strided view (contiguous bytes expected)")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 

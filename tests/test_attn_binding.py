@@ -76,3 +76,21 @@ def test_workspace_of_one_query_for_all(lfm):
         with pytest.raises(lfm.LfmError) as e:
             lfm.attn_window(dense, cache, q, Host((1,)))
         assert e.value.code == lfm.LFM_EINVAL and "out stride" in str(e.value)
+
+
+def test_workspaces_that_are_strided_views_are_refused(lfm):
+    """A call would write the bytes between the view's own."""
+    cache = lfm.KvCache(Host((3, 8, 100, 64)), Host((3, 8, 100, 64)), Host((3,), "torch.int32"))
+    q, acc, pos = Host((3, 32, 64)), Host((3, 8, 100), "torch.float32"), Host((3, 8, 100), "torch.int32")
+
+    class View(Host):
+        def is_contiguous(self):
+            return False
+
+    ws = View((1 << 20,))
+    for call in (lambda: lfm.attn_window(q, cache, q, ws), lambda: lfm.attn_scored(q, cache, q, None, acc, ws),
+                 lambda: lfm.attn_prefix(q, cache, cache, q, ws),
+                 lambda: lfm.kv_evict(cache, acc, pos, 50, cache, acc, pos, ws)):
+        with pytest.raises(lfm.LfmError) as e:
+            call()
+        assert e.value.code == lfm.LFM_EINVAL and "workspace" in str(e.value)
