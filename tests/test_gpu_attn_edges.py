@@ -323,3 +323,229 @@ def test_equal_calls_give_equal_bits(gpu, kind, dim):
                 call(ws)
                 bits.append([x.download().tobytes() for x in (r.out, r.lse, acc)])
             assert bits[0] == bits[1] == bits[2]
+
+
+# ------------------------------------------------------------------ what else the calls allow
+@pytest.mark.parametrize("kind, dim", [("f32", 64), ("bf16", 128)])
+def test_one_cache_shared_by_all_sequences(gpu, kind, dim):
+    """A sequence stride of 0, and a head stride of 0 (one kv head for several)."""
+    rng = np.random.default_rng([dim, 50])
+    cached = "bf16" if kind == "bf16" else "f16"
+    one = Cache(rng, [1], 1, 901, dim, cached)
+    cache = Cache(rng, [900, 3, 0, 77], 2, 901, dim, cached)
+    cache.k, cache.v = (np.broadcast_to(x, cache.k.shape) for x in (one.k, one.v))
+    cache.view = gpu.KvCache(*(gpu.DeviceTensor(x.buf, cache.k.shape, x.dtype, 0, (0, 0, dim, 1))
+                               for x in (one.tk, one.tv)), cache.tl)
+    check_window(gpu, Rows(gpu, rng, 4, 6, dim, kind), cache, None, 90, 2)
+    check_window(gpu, Rows(gpu, rng, 50, 6, dim, kind), cache, [0, 30, 33, 40, 50], 90, 2)
+    tight_scored(gpu, Rows(gpu, rng, 4, 6, dim, kind), cache)
+    tight_scored(gpu, Rows(gpu, rng, 50, 6, dim, kind), cache, [0, 30, 33, 40, 50])
+
+
+@pytest.mark.parametrize("kind, dim", [("f32", 128), ("f16", 64)])
+def test_one_query_for_all_rows_and_heads(gpu, kind, dim):
+    rng = np.random.default_rng([dim, 51])
+    cache = Cache(rng, [90, 7, 41], 2, 101, dim, "f16")
+    for n, start in ((3, None), (60, [0, 30, 37, 60])):
+        r = Rows(gpu, rng, n, 6, dim, kind)
+        r.values[:] = r.values[0, 0]
+        r.q = gpu.DeviceTensor(r.q.buf, r.shape, r.q.dtype, 0, (0, 0, 1))
+        check_window(gpu, r, cache, start, 30, 3)
+        tight_scored(gpu, r, cache, start)
+
+
+class Space:
+    """A workspace of exactly n bytes with a guard behind it."""
+
+    def __init__(self, gpu, n):
+        self.n, self.buf = n, gpu.DeviceBuffer.from_array(np.full(n + 4096, 0x5A, np.uint8))
+
+    def data_ptr(self):
+        return self.buf.ptr
+
+    def numel(self):
+        return self.n
+
+    def element_size(self):
+        return 1
+
+    def intact(self):
+        return (self.buf.download(np.uint8)[self.n:] == 0x5A).all()
+
+
+@pytest.mark.parametrize("heads, kv, dim, kind", [(6, 2, 64, "f32"), (34, 2, 64, "f16"), (9, 3, 128, "bf16"),
+                                                  (128, 1, 128, "f32")])
+def test_workspaces_are_large_enough(gpu, heads, kv, dim, kind):
+    rng = np.random.default_rng([heads, dim, 52])
+    cached = "bf16" if kind == "bf16" else "f16"
+    cache = Cache(rng, [1499, 700, 1033], kv, 1499, dim, cached)
+    prefix = Cache(rng, [2300], kv, 2300, dim, cached)
+    for n, start in ((3, None), (70, [0, 30, 30, 70]), (1100, [0, 700, 1000, 1100])):
+        r = Rows(gpu, rng, n, heads, dim, kind)
+        st = None if start is None else i32(start)
+        acc = f32(np.zeros((3, kv, 1499)))
+        ws = [Space(gpu, x) for x in (gpu.attn_window_workspace(r.q, cache.view, start=st),
+                                      gpu.attn_window_workspace(r.q, cache.view, window=1100, sinks=3, start=st),
+                                      gpu.attn_scored_workspace(r.q, cache.view, start=st),
+                                      gpu.attn_prefix_workspace(r.q, prefix.view, cache.view, start=st))]
+        gpu.attn_window(r.q, cache.view, r.out, ws[0], start=st)
+        gpu.attn_window(r.q, cache.view, r.out, ws[1], window=1100, sinks=3, start=st)
+        gpu.attn_scored(r.q, cache.view, r.out, None, acc, ws[2], start=st)
+        gpu.attn_prefix(r.q, prefix.view, cache.view, r.out, ws[3], start=st)
+        assert all(w.intact() for w in ws), n
+    for keep in (1, 77, 1499):
+        w = Space(gpu, gpu.kv_evict_workspace(cache.view, keep))
+        pos = i32(np.tile(np.arange(1499), (3, kv, 1)))
+        cache.tl.buf.upload(np.array([1499, 700, 1033], np.int32))
+        gpu.kv_evict(cache.view, acc, pos, keep, cache.view, acc, pos, w)
+        assert w.intact()
+
+
+@pytest.mark.parametrize("kind, dim", [("f32", 64), ("f16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_a_bad_row_stays_alone(gpu, kind, dim, bad):
+    """Queries that are no numbers, between others: the rest are the formula's."""
+    rng = np.random.default_rng([dim, 53])
+    cached = "bf16" if kind == "bf16" else "f16"
+    cache = Cache(rng, [90, 700, 41], 2, 701, dim, cached)
+    prefix = Cache(rng, [130], 2, 131, dim, cached)
+    for n, start in ((3, None), (100, [0, 40, 60, 100])):
+        r = Rows(gpu, rng, n, 6, dim, kind)
+        r.values[1, 2, 5] = r.values[1, 3] = bad
+        r.q = U.tensor(r.values, kind)[0]
+        st = None if start is None else i32(start)
+        rest = np.ones((n, 6), bool)
+        rest[1, 2:4] = False
+        for pre in (None, prefix):
+            if pre is None:
+                ws = workspace(gpu, gpu.attn_window_workspace(r.q, cache.view, start=st))
+                gpu.attn_window(r.q, cache.view, r.out, ws, start=st)
+            else:
+                ws = workspace(gpu, gpu.attn_prefix_workspace(r.q, pre.view, cache.view, start=st))
+                gpu.attn_prefix(r.q, pre.view, cache.view, r.out, ws, start=st)
+            with np.errstate(invalid="ignore"):
+                out, _, _, extra = U.reference(r.values, cache, start, prefix=pre)
+            got = r.result()
+            assert np.isnan(got[~rest]).all()
+            check_out(got[rest], out[rest], tuple(x[rest] for x in extra), kind, dim)
+        acc = f32(np.zeros((3, 2, 701)))
+        ws = workspace(gpu, gpu.attn_scored_workspace(r.q, cache.view, start=st))
+        gpu.attn_scored(r.q, cache.view, r.out, None, acc, ws, start=st)
+        a = acc.download().reshape(3, 2, 701)
+        b, p = (1, 699) if start is None else (0, 90 - 40 + 1)  # the bad row's sequence and position
+        used = np.arange(701) < cache.length[:, None]
+        nan = np.zeros(a.shape, bool)
+        nan[b, :, :p + 1] = True  # heads 2 and 3 are of kv heads 0 and 1
+        assert np.array_equal(np.isnan(a), nan & used[:, None])
+
+
+def test_captured_prompts_follow_their_starts(gpu):
+    """Graphs of ragged calls: lengths, starts and rows change between replays, and eager calls
+    of the same run between them."""
+    from test_gpu_attn import Hip
+    hip = Hip()
+    rng = np.random.default_rng(54)
+    cache = Cache(rng, [1400, 900, 2], 2, 1400, 64, "f16")
+    prefix = Cache(rng, [700], 2, 700, 64, "f16")
+    n, heads = 90, 6
+    st = i32([0, 50, 80, 90])
+    outs = [Rows(gpu, rng, n, heads, 64, "f32") for _ in range(3)]
+    q = outs[0].q
+    acc = f32(np.zeros((3, 2, 1400)))
+
+    def spaces():
+        return [workspace(gpu, m) for m in (gpu.attn_window_workspace(q, cache.view, window=1200, sinks=4, start=st),
+                                            gpu.attn_scored_workspace(q, cache.view, start=st),
+                                            gpu.attn_prefix_workspace(q, prefix.view, cache.view, start=st))]
+
+    def calls(ws, stream):
+        gpu.attn_window(q, cache.view, outs[0].out, ws[0], window=1200, sinks=4, start=st, lse=outs[0].lse, stream=stream)
+        gpu.attn_scored(q, cache.view, outs[1].out, acc, acc, ws[1], start=st, stream=stream)
+        gpu.attn_prefix(q, prefix.view, cache.view, outs[2].out, ws[2], start=st, stream=stream)
+
+    def clear():
+        for x in (outs[0].out, outs[1].out, outs[2].out, outs[0].lse, acc):
+            x.buf.upload(np.zeros(x.buf.nbytes, np.uint8))
+
+    def state():
+        gpu.lib().lfm_dev_synchronize()
+        return [x.download().tobytes() for x in (outs[0].out, outs[1].out, outs[2].out, outs[0].lse, acc)]
+
+    eager, own = spaces(), spaces()
+    calls(eager, 0)
+    gpu.lib().lfm_dev_synchronize()
+    s = hip.stream()
+    graph = hip.graph(s, lambda: calls(own, s.value))
+    for turn in range(5):
+        cuts = np.sort(rng.integers(0, n + 1, 2))
+        st.buf.upload(np.array([0, *cuts, n] if turn % 2 else [3, *np.maximum(cuts, 3), n], np.int32))
+        cache.tl.buf.upload(rng.integers(0, 1401, 3).astype(np.int32))
+        q.buf.upload(rng.standard_normal((n, heads, 64)).astype(np.float32))
+        clear()
+        calls(eager, 0)
+        want = state()
+        clear()
+        hip.ok("hipGraphLaunch", graph, s)
+        hip.ok("hipStreamSynchronize", s)
+        assert state() == want, turn
+
+
+@pytest.mark.parametrize("place", ["acc", "pos", "both"])
+def test_evict_apart_with_acc_or_pos_in_place(gpu, place):
+    rng = np.random.default_rng(55)
+    n, kv, slots, keep, dim = 3, 2, 400, 150, 64
+    length = [400, 151, 90]
+    cache, out = Cache(rng, length, kv, slots, dim, "f16"), Cache(rng, [0] * n, kv, slots, dim, "f16", "slot")
+    acc = rng.random((n, kv, slots), dtype=np.float32)
+    pos = np.cumsum(rng.integers(1, 4, acc.shape), -1).astype(np.int32)
+    ta, tp, oa, op = f32(acc), i32(pos), f32(np.full(acc.shape, 9.0)), i32(np.full(acc.shape, 9))
+    da, dp = ta if place != "pos" else oa, tp if place != "acc" else op
+    want_a, want_p = (acc.copy() if place != "pos" else np.full_like(acc, 9)), (pos.copy() if place != "acc" else np.full_like(pos, 9))
+    ws = workspace(gpu, gpu.kv_evict_workspace(cache.view, keep))
+    gpu.kv_evict(cache.view, ta, tp, keep, out.view, da, dp, ws, sinks=5, recent=30)
+    from test_gpu_attn import read_cache
+    got = read_cache(out.view, "f16", "slot")
+    for b in range(n):
+        for h in range(kv):
+            s = U.keep_slots(acc[b, h], pos[b, h], length[b], keep, 5, 30)
+            s = np.arange(length[b]) if s is None else s
+            want_a[b, h, :len(s)], want_p[b, h, :len(s)] = acc[b, h][s], pos[b, h][s]
+            for x, w in zip(got, (cache.k, cache.v)):
+                assert np.array_equal(x[b, h, :len(s)], w[b, h][s])
+    assert np.array_equal(da.download().reshape(acc.shape), want_a)
+    assert np.array_equal(dp.download().reshape(acc.shape), want_p)
+    assert np.array_equal(out.tl.download(), [150, 150, 90])
+
+
+def test_evict_positions_at_the_ends_of_32_bits(gpu):
+    """Positions that are negative, the largest and the smallest; keep larger than the cache."""
+    rng = np.random.default_rng(56)
+    n, kv, slots, dim = 4, 1, 130, 64
+    acc = rng.random((n, kv, slots), dtype=np.float32)
+    pos = rng.integers(-(1 << 31), 1 << 31, (n, kv, slots)).astype(np.int32)
+    pos[0, 0, 7], pos[0, 0, 9] = (1 << 31) - 1, -(1 << 31)
+    pos[1] = np.abs(pos[1])
+    pos[2] = -1 - np.abs(pos[2] // 2)
+    pos[3] = np.arange(slots)
+    length = [slots] * n
+    for keep, sinks, recent in ((60, 0, 60), (60, 60, 0), (60, 7, 9), (1, 0, 1), (500, 3, 400)):
+        cache = Cache(rng, length, kv, slots, dim, "f16")
+        out = Cache(rng, [0] * n, kv, 501, dim, "f16")
+        oa, op = f32(np.zeros((n, kv, 501))), i32(np.zeros((n, kv, 501)))
+        ws = workspace(gpu, gpu.kv_evict_workspace(cache.view, keep))
+        gpu.kv_evict(cache.view, f32(acc), i32(pos), keep, out.view, oa, op, ws, sinks=sinks, recent=recent)
+        p = op.download().reshape(n, kv, 501)
+        for b in range(n):
+            s = U.keep_slots(acc[b, 0], pos[b, 0], slots, keep, sinks, recent)
+            s = np.arange(slots) if s is None else s
+            assert np.array_equal(p[b, 0, :len(s)], pos[b, 0][s]), (b, keep, sinks, recent)
+        assert np.array_equal(out.tl.download(), [min(slots, keep)] * n)
+
+
+@pytest.mark.parametrize("kind, dim", [("f32", 64), ("bf16", 128)])
+def test_window_of_chunks_in_ranges(gpu, kind, dim):
+    rng = np.random.default_rng([dim, 57])
+    cache = Cache(rng, [2400, 1300, 40], 2, 2407, dim, "bf16" if kind == "bf16" else "f16", "mixed")
+    r = Rows(gpu, rng, 90, 6, dim, kind)
+    for window, sinks in ((1500, 0), (1100, 70), (2300, 2000)):
+        check_window(gpu, r, cache, [0, 40, 75, 90], window, sinks)
