@@ -38,18 +38,24 @@ struct AttnKernels {
 static std::mutex g_mu;
 static std::unordered_map<int, AttnKernels *> g_attn;
 
+// A call of the runtime that failed: its error is not left for the caller's next check.
+static int device_error(const char *what, const char *of, hipError_t e)
+{
+    (void)hipGetLastError();
+    return fail(LFM_EDEVICE, "%s%s: %s", what, of, hipGetErrorString(e));
+}
+
 static int load_attn(int dev)
 {
     const std::string path = lfm_beside_code_object("lfm_attn.hsaco");
     AttnKernels k;
     hipError_t e = hipModuleLoad(&k.mod, path.c_str());
     if (e != hipSuccess)
-        return fail(LFM_EDEVICE, "hipModuleLoad(%s): %s", path.c_str(), hipGetErrorString(e));
+        return device_error("hipModuleLoad of ", path.c_str(), e);
     static const char *const types[3] = {"f32", "f16", "bf16"};
     auto get = [&](hipFunction_t *f, const std::string &name) -> int {
         const hipError_t r = hipModuleGetFunction(f, k.mod, name.c_str());
-        return r == hipSuccess ? LFM_OK
-                               : fail(LFM_EDEVICE, "hipModuleGetFunction(%s): %s", name.c_str(), hipGetErrorString(r));
+        return r == hipSuccess ? LFM_OK : device_error("hipModuleGetFunction of ", name.c_str(), r);
     };
     int rc = LFM_OK;
     for (int t = 0; t < 3 && rc == LFM_OK; ++t)
@@ -105,7 +111,7 @@ template <typename A> static int launch(hipFunction_t f, dim3 grid, uint32_t thr
 {
     void *params[] = {(void *)&args};
     const hipError_t e = hipModuleLaunchKernel(f, grid.x, grid.y, grid.z, threads, 1, 1, 0, s, params, nullptr);
-    return e == hipSuccess ? LFM_OK : fail(LFM_EDEVICE, "kernel launch failed: %s", hipGetErrorString(e));
+    return e == hipSuccess ? LFM_OK : device_error("kernel launch", "", e);
 }
 
 // ------------------------------------------------------------------ argument checks

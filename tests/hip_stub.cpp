@@ -23,6 +23,17 @@ static std::vector<std::string *> g_functions;
 static std::vector<Launch> g_launches;
 static char g_error[512];
 static size_t g_args_bytes;
+static int g_refuse; // which call fails: 1 hipModuleLoad, 2 hipModuleGetFunction, 3 hipModuleLaunchKernel
+static hipError_t g_left; // what the runtime would report next
+
+static hipError_t answer(int call)
+{
+    if (g_refuse == call)
+        g_left = hipErrorUnknown;
+    return g_refuse == call ? hipErrorUnknown : hipSuccess;
+}
+extern "C" void stub_refuse(int call) { g_refuse = call; }
+extern "C" int stub_left() { return (int)g_left; }
 
 extern "C" void stub_reset(size_t args_bytes)
 {
@@ -58,7 +69,12 @@ hipError_t hipStreamGetDevice(hipStream_t, hipDevice_t *d)
     *d = 0;
     return hipSuccess;
 }
-hipError_t hipGetLastError() { return hipSuccess; }
+hipError_t hipGetLastError()
+{
+    const hipError_t e = g_left;
+    g_left = hipSuccess;
+    return e;
+}
 const char *hipGetErrorString(hipError_t) { return "stub"; }
 hipError_t hipPointerGetAttributes(hipPointerAttribute_t *a, const void *p)
 {
@@ -68,23 +84,25 @@ hipError_t hipPointerGetAttributes(hipPointerAttribute_t *a, const void *p)
             a->device = r.device;
             return hipSuccess;
         }
-    return hipErrorInvalidValue;
+    return g_left = hipErrorInvalidValue;
 }
 hipError_t hipModuleLoad(hipModule_t *m, const char *)
 {
     *m = (hipModule_t)&g_functions;
-    return hipSuccess;
+    return answer(1);
 }
 hipError_t hipModuleUnload(hipModule_t) { return hipSuccess; }
 hipError_t hipModuleGetFunction(hipFunction_t *f, hipModule_t, const char *name)
 {
     g_functions.push_back(new std::string(name));
     *f = (hipFunction_t)g_functions.back();
-    return hipSuccess;
+    return answer(2);
 }
 hipError_t hipModuleLaunchKernel(hipFunction_t f, unsigned gx, unsigned gy, unsigned gz, unsigned bx, unsigned,
                                  unsigned, unsigned, hipStream_t, void **params, void **)
 {
+    if (answer(3) != hipSuccess)
+        return hipErrorUnknown;
     Launch l;
     l.name = *(const std::string *)f;
     l.grid[0] = gx, l.grid[1] = gy, l.grid[2] = gz, l.block = bx;

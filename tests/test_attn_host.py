@@ -167,3 +167,27 @@ def test_nothing_to_do_enqueues_nothing(call, lfm):
         assert op(call, none) == (0, []), op.__name__
     rowless = arguments(lfm, rows=rows(lfm, n_rows=0, start=7 * MB, q=None, out=None))
     assert window(call, rowless) == (0, []) and prefix(call, rowless) == (0, [])
+
+
+def test_a_failing_runtime_leaves_no_error_behind(host, call, lfm, tmp_path):
+    """A call that the runtime fails returns LFM_EDEVICE, and the error is not there for the
+    caller's next check to find; a refused pointer leaves none either."""
+    import shutil
+    so = shutil.copy(host._name, tmp_path / "fresh.so")  # one that has loaded no code object yet
+    fresh = C.CDLL(str(so))
+    a = arguments(lfm)
+    for which in (1, 2, 3, 0):
+        fresh.stub_reset.argtypes, fresh.stub_memory.argtypes = [C.c_size_t], [C.c_size_t, C.c_size_t, C.c_int]
+        fresh.stub_reset(0)
+        fresh.stub_memory(MB, 63 * MB, 0)
+        fresh.stub_refuse(which)
+
+        def run(name, *args):
+            f = getattr(fresh, name)
+            f.argtypes = getattr(lfm.lib(), name).argtypes
+            return f(*args)
+        for op in (window, scored_of, prefix, evict):
+            assert op(run, a) == (lfm.LFM_EDEVICE if which else 0)
+            assert fresh.stub_left() == 0, (which, op.__name__)
+    assert window(call, arguments(lfm, rows=rows(lfm, q=HOST)))[0] == lfm.LFM_EINVAL
+    assert host.stub_left() == 0
