@@ -57,8 +57,8 @@ struct AttnOpArgs {
     float *acc_out;   // [n_seq][kv_heads][slots]
 };
 
-// Eviction, first step: per (sequence, kv head) the source slot of each of the `keep`
-// slots that stay.
+// Eviction, both steps: the choice, per (sequence, kv head) the source slot of each of the
+// `keep` slots that stay, and the move.
 struct EvictArgs {
     KvView c;
     void *k_out, *v_out; // may be c.k and c.v (then with its strides): in place

@@ -257,6 +257,11 @@ template <typename TQ, int D, int RT> struct State {
 // the first block hardly ever, and a weight stays at or below 2^15.  So their sum, which is
 // needed anyway, stands for the maximum (2700 tokens of 64 dims 54.8 us with it, 53.1 without).
 // Two tiles share a check, where four would keep more in registers than there are.
+//
+// The matrix instruction takes V and the weights as 16-bit numbers, so a weight is rounded to 11 or
+// 8 bits, half a step of the rows' own type, while the sum keeps 32: outputs of 16-bit rows are
+// 1.3 to 1.4 times as far from 64 bits as their own rounding alone.  Two numbers a weight would
+// double the products with V; F32 rows, whose outputs would show it, have them (22 bits).
 #define RISE 8.f
 template <int NT, typename TQ, int D, int RT>
 __device__ __forceinline__ void weigh(State<TQ, D, RT> &S, const floatx4 (&s)[RT][2], const Queries<TQ, D, RT> &Q,
@@ -901,10 +906,14 @@ __device__ void attn_row(const AttnOpArgs &a, const B &bl, uint32_t b0, uint32_t
 // The next block's loads are in flight while a block is used.  Blocks that no row of a wave
 // sees are passed over by it, those that all its rows see whole are used without masks.
 //
-// Bound by a SIMD's issue, which softmax and matrix work share: for 32 rows and 32 slots of 64
-// dims a wave has 16 products of 16 cycles, 16 exponentials of 10 and some 55 other
-// instructions, and products and other work hardly overlap (8 products and 32 multiply-adds
-// of four waves take 194 cycles together, 132 and 82 alone).  4096 tokens, window 1024, 32
+// Bound by a SIMD's issue, which vector and matrix work share: products and other work hardly
+// overlap (8 products and 32 multiply-adds of four waves take 194 cycles together, 132 and 82
+// alone).  For 32 rows and 32 slots a wave has 16 products of 16 cycles at 64 dims, 32 at 128, and
+// 111 and 123 other vector instructions (4096 tokens, window 1024; chunks, window 2048): some 70
+// are the softmax, 16 exponentials among them; the rest are the loads' addresses, masks at the
+// diagonal and the window's edge, and the loop's own.  Products and vector issue fill 30 and 68 %
+// of the cycles at 64 dims, 37 and 49 (the products' own issue among them) at 128, where shared
+// memory is busy for 28 % and a fifth is neither's.  4096 tokens, window 1024, 32
 // heads over 8 of 64 dims: 50 us, 600 TFLOP/s; 8192 causal: 323 us, 850; of 128 dims, with
 // half as much softmax a product, 589 us, 930.  Two groups of 32 slots in one softmax take more
 // registers than four waves a SIMD have (72 us for 60), four row tiles a wave leave two waves
@@ -1135,8 +1144,9 @@ __device__ __forceinline__ void attn_tile(const AttnOpArgs &a, TileShared<D> &sh
 // end, all in a fixed order.  (Rows read as operands by every wave for itself, 16 rows a load,
 // kept the first-level cache busy with 64-byte pieces: a prompt of 2048 tokens, 32 heads over
 // 8 of 64 dims, took 42 us so, 28 this way and 5 for the adding of the parts.)  Bound by vector
-// instructions, three a score and one of them an exponential: they fill 31 of 50 thousand cycles
-// of a SIMD, the products 8.
+// instructions, 5.9 a score at 64 dims: three are the softmax, one of them an exponential, most of
+// the rest the addresses and the staging of rows.  They fill 31 of 50 thousand cycles of a SIMD,
+// the products 8; waits at a step's barrier and for loads are the rest.
 template <typename TQ, int D> __device__ __forceinline__ void attn_weights(const AttnOpArgs &a)
 {
     typedef typename TQ::vec vec;

@@ -1,5 +1,6 @@
-// wave_ops.h -- wave64 reductions and the MoE routing rule, shared by the
-// decode (lfm_kernels.hip) and prefill (lfm_prefill.hip) code objects.
+// wave_ops.h -- wave64 reductions, shared by the decode (lfm_kernels.hip), prefill
+// (lfm_prefill.hip) and cache-attention (lfm_attn.hip) code objects, and the MoE routing
+// rule of the first two.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
