@@ -762,11 +762,14 @@ def _space(workspace):
     return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
-def _u32(what: str, *values) -> None:
+def _u32(what: str, a, b=0, c=0) -> None:
     """Refuses what ctypes would cut down to its low 32 bits."""
-    for v in values:
-        if not isinstance(v, (int, np.integer)) or not 0 <= v <= 0xFFFFFFFF:
-            raise LfmError(LFM_EINVAL, f"{what}: {v!r} (a whole number of 32 bits, not negative, expected)")
+    try:
+        if not (a | b | c) >> 32:  # of a negative number the sign stays
+            return
+    except TypeError:
+        pass
+    raise LfmError(LFM_EINVAL, f"{what}: {(a, b, c)} (whole numbers of 32 bits, not negative, expected)")
 
 
 _torch_stream = None  # device index -> address of torch's current stream there
