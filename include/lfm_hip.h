@@ -357,7 +357,8 @@ int lfm_attn_prefix_workspace(const lfm_kv *prefix, const lfm_kv *kv, const lfm_
  * kv->v (and equal strides) the eviction is in place and moves only what changes place;
  * acc_out == acc and pos_out == pos likewise (with equal slots), len_out may be kv->len.
  * Apart from that outputs and inputs are apart.  Output slots past the new length are
- * left as they are. */
+ * left as they are.  Afterwards slots are no longer in the order of their tokens: calls
+ * that see all of them are right as they are, a window and its first tokens count slots. */
 int lfm_kv_evict(const lfm_kv *kv, const float *acc, const int32_t *pos, uint32_t keep,
                  uint32_t sinks, uint32_t recent, const lfm_kv *out, float *acc_out,
                  int32_t *pos_out, void *workspace, size_t workspace_bytes, void *stream);
