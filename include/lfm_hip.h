@@ -323,7 +323,8 @@ typedef struct lfm_rows {
 /* out = softmax(scale * q K^T) V over the slots a row sees: of the positions up to its
  * own, the newest `window` (0: all) and the first `sinks`.  A row that sees nothing gets
  * zeros and an lse of -infinity.  Scores, weights' sums and outputs are held in 32 bits;
- * weights meet V as 16-bit numbers, as two of them (22 bits) for F32 rows. */
+ * weights meet V as 16-bit numbers, as two of them (22 bits) for F32 rows.  Weights are
+ * divided by their sum at the end: BF16 values of V from 2^89 on may overflow before. */
 int lfm_attn_window(const lfm_kv *kv, const lfm_rows *rows, uint32_t window, uint32_t sinks,
                     void *workspace, size_t workspace_bytes, void *stream);
 int lfm_attn_window_workspace(const lfm_kv *kv, const lfm_rows *rows, uint32_t window,

@@ -119,10 +119,24 @@ __device__ __forceinline__ bool find_row(const AttnOpArgs &a, uint32_t row, uint
     return false;
 }
 
+// An output before its rounding to the rows' type.  A mean of binary16 numbers is no larger than
+// the largest of them, but rounded weights may carry it past that, from where it would round to an
+// infinity.  (An infinity that V holds stays one.)
+template <typename TQ> __device__ __forceinline__ float in_range(float v)
+{
+    constexpr float MOST = 65504.f;
+    if constexpr (__is_same(typename TQ::type, _Float16))
+        return fabsf(v) < INFINITY ? fminf(fmaxf(v, -MOST), MOST) : v;
+    return v;
+}
+
 // Four outputs of a row and head, rounded to the rows' type.
 template <typename TQ>
 __device__ __forceinline__ void store_out(const RowsView &r, uint32_t row, uint32_t h, uint32_t d, floatx4 v)
 {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        v[e] = in_range<TQ>(v[e]);
     typedef typename TQ::type tq;
     typedef tq tq4 __attribute__((ext_vector_type(4)));
     *(tq4 *)((tq *)r.out + (int64_t)row * r.o_rs + (int64_t)h * r.o_hs + d) = __builtin_convertvector(v, tq4);
@@ -681,7 +695,7 @@ __device__ __forceinline__ void store_row(const AttnOpArgs &a, uint32_t row, uin
     const float f = inverse(sum);
 #pragma unroll
     for (int i = 0; i < E; ++i)
-        to[i] = (tq)(empty ? 0.f : o[i] * f);
+        to[i] = (tq)(empty ? 0.f : in_range<TQ>(o[i] * f));
     if (lane == 0)
         finish_row(a, (size_t)row * a.r.heads + h, empty, top, sum);
 }

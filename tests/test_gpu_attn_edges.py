@@ -549,3 +549,52 @@ def test_window_of_chunks_in_ranges(gpu, kind, dim):
     r = Rows(gpu, rng, 90, 6, dim, kind)
     for window, sinks in ((1500, 0), (1100, 70), (2300, 2000)):
         check_window(gpu, r, cache, [0, 40, 75, 90], window, sinks)
+
+
+@pytest.mark.parametrize("kind, dim", [("f32", 64), ("f16", 64), ("f16", 128)])
+@pytest.mark.parametrize("size", [65504.0, 60000.0, 3e-5, 6e-8])
+def test_values_at_the_ends_of_binary16(gpu, kind, dim, size):
+    """V of one size, the largest number and subnormal ones among them: the outputs are that size
+    and no infinity, in every kernel that writes some."""
+    rng = np.random.default_rng([dim, 60])
+
+    def edit(k, v):
+        v[:] = np.where(rng.random(v.shape[:2] + (1, v.shape[3])) < 0.5, size, -size)
+
+    cache = Cache(rng, [1900, 45, 301], 2, 1900, dim, "f16", edit=edit)
+    prefix = Cache(rng, [700], 2, 700, dim, "f16")
+    prefix.v[:] = cache.v[:1, :, :1]
+    prefix.tv.buf.upload(np.broadcast_to(prefix.v, prefix.k.shape).astype(np.float16))
+    cache.v[1:] = cache.v[:1]
+    cache.tv.buf.upload(cache.v.astype(np.float16))
+    want = np.repeat(cache.v[0, :, 0], 3, axis=0)  # [heads][dim], every row's
+    for n, start in ((3, None), (100, [0, 40, 70, 100])):
+        r = Rows(gpu, rng, n, 6, dim, kind)
+        st = None if start is None else i32(start)
+        acc = f32(np.zeros((3, 2, 1900)))
+        for call in (lambda: gpu.attn_window(r.q, cache.view, r.out, ws, start=st),
+                     lambda: gpu.attn_window(r.q, cache.view, r.out, ws, window=40, start=st),
+                     lambda: gpu.attn_scored(r.q, cache.view, r.out, None, acc, ws, start=st),
+                     lambda: gpu.attn_prefix(r.q, prefix.view, cache.view, r.out, ws, start=st)):
+            ws = workspace(gpu, 1 << 25)
+            call()
+            # |sum w v| is |v| but for the weights' rounding; the output's own (of a subnormal an absolute one)
+            rel = U.WEIGHT[kind] + 2.0 ** -20 + 2 * (2600 + 16) * 2.0 ** -24
+            tol = rel * np.abs(want) + 1.01 * (U.HALF[kind] * np.abs(want) + (2.0 ** -25 if kind == "f16" else 2.0 ** -149))
+            got = r.result()
+            bad = ~(np.abs(got - want) <= tol)
+            assert not bad.any(), (n, int(bad.sum()), got[bad][:5], np.broadcast_to(want, got.shape)[bad][:5])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_keys_that_are_subnormal(gpu, kind):
+    rng = np.random.default_rng(61)
+
+    def edit(k, v):
+        k *= 1e-6
+
+    cache = Cache(rng, [190, 45, 3], 2, 190, 64, "f16", edit=edit)
+    for n, start in ((3, None), (100, [0, 67, 97, 100])):
+        r = Rows(gpu, rng, n, 6, 64, kind)
+        check_window(gpu, r, cache, start, 60, 3, scale=1e5)
+        tight_scored(gpu, r, cache, start, scale=1e5)
